@@ -270,6 +270,102 @@ okq_status okq_mlp_gated_silu_q(const float *x, int64_t rows, int64_t hidden, in
                                 const void *up_w, uint64_t up_bytes, uint32_t down_type, const void *down_w,
                                 uint64_t down_bytes, float *gate_buf, float *up_buf, float *out, void *stream);
 
+/* ---- the decode step around the projections ----------------------------- */
+
+/* A paged key-value cache in device memory: n_pages pages, each holding
+ * page_tokens rows of head_dim values for every one of kv_heads heads, keys at
+ * `k` and values at `v`.  Row (page p, head h, token t) starts at
+ * p * page_stride + h * head_stride + t * token_stride bytes, in both, so
+ * pages may be laid out head by head or token by token.  `type` is
+ * OKQ_TYPE_F32, F16, BF16, or Q8_0 (head_dim / 32 GGUF blocks a row, head_dim
+ * a multiple of 32).  Strides and bases are multiples of 4 bytes (F32) or 2.
+ * head_dim is at most 512.  Slot s of a cache is token s % page_tokens of page
+ * s / page_tokens.  The struct is read during the call only.  The reference's
+ * paged cache is host memory of f32 (crates/runtime, kv_cache.rs:125). */
+typedef struct okq_kv_pages {
+    uint32_t type;
+    int64_t n_pages, page_tokens, kv_heads, head_dim;
+    int64_t page_stride, head_stride, token_stride; /* bytes */
+    void *k, *v;
+} okq_kv_pages;
+
+/* The step between the q/k/v projections and attention, for `tokens` tokens
+ * in one pass: RMS norm of every query and key head, the position rotation,
+ * and the store of keys and values into the paged cache.
+ *   y = q_norm ? x * (1 / sqrt(sum(x^2) / head_dim + epsilon)) * q_norm : x
+ *   (y[a], y[b]) -> (y[a] cos t - y[b] sin t, y[b] cos t + y[a] sin t),
+ *   t = positions[token] * inv_freq[i] for i < rotary / 2, formed and reduced
+ *   in 64 bits, (a, b) = (2i, 2i + 1) if `interleaved`, else (i, i + rotary/2);
+ * values from `rotary` on pass through.  q, k, v: device f32, row t of each at
+ * t * its stride (in elements), its heads side by side (q/k/v may lie in one
+ * buffer).  q_norm, k_norm [head_dim] f32 or NULL (that norm is left out);
+ * positions [tokens] int32; inv_freq [rotary / 2] f32, NULL if rotary is 0.
+ * Outputs: q_out [tokens, q_heads, head_dim] f32 (may be q itself with q's
+ * stride); k_out likewise [tokens, kv_heads, head_dim], or NULL; the cache's
+ * rows at slots[token] (int64; a slot outside the cache, -1 say, stores
+ * nothing), or cache NULL (then v and slots are not read).  Keys and values
+ * are rounded to the cache's type, to nearest even; Q8_0 blocks are
+ * okq_quantize's bytes.  Tokens that share a slot leave either one's row.
+ * tokens == 0 is a no-op.  The rotation follows crates/kernels/src/rope.rs
+ * (its pairs are the halves); no counterpart in the reference fuses the three. */
+okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                            int64_t v_stride, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                            const float *q_norm, const float *k_norm, float epsilon, const int32_t *positions,
+                            const float *inv_freq, int64_t rotary, int interleaved, float *q_out, int64_t q_out_stride,
+                            float *k_out, int64_t k_out_stride, const okq_kv_pages *cache, const int64_t *slots,
+                            void *stream);
+
+/* Attention of one new token of each of `seqs` sequences over a paged cache:
+ *   out[s, h] = sum_t softmax_t(f(scale * q[s, h] . K[t])) V[t]
+ * over the sequence's cached tokens t < lengths[s] (the new token's own key
+ * and value already stored), the last `window` of them if window > 0;
+ * f(x) = softcap * tanh(x / softcap) if softcap > 0, else x.  Query head h
+ * reads key/value head h / (q_heads / kv_heads).  q, out: device f32, row s at
+ * s * its stride (elements), heads side by side, head_dim each.  block_table
+ * [seqs, table_width] int32: the page of tokens j * page_tokens on of sequence
+ * s is block_table[s, j]; entries outside [0, n_pages) hide their tokens and
+ * are never followed.  lengths [seqs] int32 (device), read as at most
+ * max_length and table_width * page_tokens; max_length bounds the launch and
+ * the workspace.  lse [seqs, q_heads] f32 or NULL: log of the sum of
+ * exp(f(scale * q . K)).  A sequence with nothing to see (length 0, hidden pages)
+ * gets zeros and lse -inf; tokens outside the length or the window may hold
+ * anything, NaN too; a visible infinity or NaN leaves no finite number in what
+ * it reaches (a key: its heads' lse; a value: its column of out).  Products and sums are f32 on the cached values; a row's
+ * result depends on the call's shape and lengths only, not on timing.
+ * seqs == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
+ * reference, whose attention is on contiguous host rows
+ * (crates/kernels/src/attention.rs). */
+okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, int64_t q_heads,
+                               const okq_kv_pages *cache, const int32_t *block_table, int64_t table_width,
+                               const int32_t *lengths, int64_t max_length, float scale, float softcap, int64_t window,
+                               float *out, int64_t out_stride, float *lse, void *stream);
+
+/* What happens to the output head's logits before a token is chosen, and the
+ * greedy choice.  Per row r of logits [rows, vocab] (row stride in elements):
+ *   n(i) = how often token i is in history[r, history_start[r] .. history_len[r])
+ *   if i is in history[r, 0 .. history_len[r]):
+ *     x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   x = x - frequency[r] * n(i) - (n(i) > 0 ? presence[r] : 0)
+ *   x = x + (sum of the biases listed for i, in list order)
+ *   x = -inf if bit i % 32 of mask word i / 32 is 0
+ * each operation rounded on its own, and best[r] the lowest index of the
+ * largest result, -1 if all are -inf or one is NaN.  history [rows,
+ * history_stride] int32 with history_len (at most the stride) and
+ * history_start [rows] int32, the latter NULL for 0; repetition, frequency,
+ * presence [rows] f32, each NULL for none; bias_ids and bias [rows,
+ * bias_stride] with bias_len [rows]; mask [rows, mask_stride] uint32 words,
+ * least significant bit first.  history, bias_ids and mask may be NULL (none).
+ * Token ids outside the vocabulary are passed over.  out may be logits with
+ * its stride; best [rows] int32 or NULL.  rows == 0 is a no-op.  Uses a
+ * per-stream workspace for best.  The reference chooses greedily
+ * from unprocessed logits on the host (crates/runtime). */
+okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_t rows, int64_t vocab,
+                              const int32_t *history, int64_t history_stride, const int32_t *history_len,
+                              const int32_t *history_start, const float *repetition, const float *frequency,
+                              const float *presence, const int32_t *bias_ids, const float *bias, int64_t bias_stride,
+                              const int32_t *bias_len, const uint32_t *mask, int64_t mask_stride, float *out,
+                              int64_t out_stride, int32_t *best, void *stream);
+
 /* The next compute kernel this thread launches through okq_dequantize,
  * okq_linear_out_by_in_q*, okq_gemv or okq_gemm* records `start` and `stop`
  * (hipEvent_t, created with timing enabled) at the begin and end of its

@@ -122,6 +122,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   return (r0 + r1) + (r2 + r3);
 }
 
+// Orders a wave's own LDS accesses before and after it, lane against lane
+// (its LDS instructions execute in order, so this costs no wait).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Activation quantisation for the integer dot path.  A run of floats is
 // scaled by a power of two 2^-e chosen so that max|x| * 2^-e <= 0.99 * 2^23,
 // rounded to an integer q and split into three signed int8 limbs

@@ -220,4 +220,57 @@ hipError_t launch_prefill_multi(const void *x, int64_t M, int64_t K, int count, 
 hipError_t launch_gemm_f32(int type, const _Float16 *xhi, const _Float16 *xlo, const void *xsum, const float *rscale,
                            int64_t M, int64_t K, PrefillMats &mats, int count, hipStream_t s);
 
+// ---- the decode step around the projections ---------------------------------
+
+// A paged cache as the kernels take it (okq_kv_pages, validated).
+struct KvPages {
+  int type;  // an OKQ_TYPE_*: F32, F16, BF16 or Q8_0
+  int n_pages, page_tokens, kv_heads, head_dim;
+  int64_t page_stride, head_stride, token_stride;  // bytes
+  uint8_t *k, *v;
+};
+constexpr int kMaxHeadDim = 512;
+
+// okq_qk_norm_rope's arguments; cache.k null: no cache, k_out null: no copy.
+struct RopeArgs {
+  const float *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  float *q_out, *k_out;
+  const float *q_norm, *k_norm, *inv_freq;
+  const int32_t *positions;
+  const int64_t *slots;
+  int tokens, q_heads, kv_heads, head_dim, rotary, interleaved;
+  float eps;
+  KvPages cache;
+};
+hipError_t launch_rope(const RopeArgs &a, int cu_count, hipStream_t s);
+
+struct AttnArgs {
+  const float *q;
+  int64_t q_stride, out_stride;
+  int seqs, q_heads, group;  // group: query heads of a key/value head
+  const int32_t *table, *lengths;
+  int table_width, max_len;  // max_len: at most table_width * page_tokens
+  float scale, softcap;
+  int window;  // 0: none
+  float *out, *lse;
+  KvPages cache;
+};
+hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
+
+struct LogitsArgs {
+  const float *x;
+  float *out;
+  int64_t x_stride, out_stride, hist_stride, bias_stride, mask_stride;
+  int rows, vocab;
+  const int32_t *hist, *hist_len, *hist_start, *bias_ids, *bias_len;
+  const float *rep, *freq, *pres, *bias;
+  const uint32_t *mask;
+  int32_t *best;
+};
+// The largest-value keys of a row's slices lie in the workspace until the row
+// is whole; none is needed without `best`.
+size_t logits_workspace(int64_t rows, int64_t vocab);
+hipError_t launch_logits(const LogitsArgs &a, void *workspace, hipStream_t s);
+
 }  // namespace okq

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -422,6 +423,59 @@ okq_status linear_impl(const void *x, bool x_bf16, int64_t rows, int64_t K, uint
   hipError_t e = okq::launch_gemv_multi((int)type, xf, K, rows, 1, &w, &N, &bias, &out, info.cu_count, s,
                                         okq::GemvPro{});
   return hip_status(e, "gemv launch");
+}
+
+// ---- decode-step validation ----------------------------------------------------
+
+// A cache's own fields, and the form that the kernels take.
+okq_status validate_pages(const char *what, const okq_kv_pages &c, okq::KvPages &out) {
+  if (c.type != OKQ_TYPE_F32 && c.type != OKQ_TYPE_F16 && c.type != OKQ_TYPE_BF16 && c.type != OKQ_TYPE_Q8_0)
+    return fail(OKQ_E_TYPE, "unsupported %s cache: tensor type %s (%u); supported: F32, F16, BF16, Q8_0", what,
+                type_name(c.type), c.type);
+  if (c.n_pages < 1 || c.page_tokens < 1 || c.kv_heads < 1 || c.head_dim < 1 || c.n_pages > INT32_MAX ||
+      c.page_tokens > INT32_MAX || c.kv_heads > INT32_MAX || c.head_dim > okq::kMaxHeadDim)
+    return fail(OKQ_E_SHAPE,
+                "%s cache of %lld pages of %lld tokens, %lld heads of %lld: each must be at least 1, head_dim at most %d",
+                what, (long long)c.n_pages, (long long)c.page_tokens, (long long)c.kv_heads, (long long)c.head_dim,
+                okq::kMaxHeadDim);
+  if (c.type == OKQ_TYPE_Q8_0 && c.head_dim % 32 != 0)
+    return fail(OKQ_E_SHAPE, "%s Q8_0 cache head_dim=%lld is not a multiple of 32", what, (long long)c.head_dim);
+  TypeInfo ti;
+  type_info(c.type, ti);
+  const int64_t row = c.head_dim / ti.elems * ti.bytes, align = c.type == OKQ_TYPE_F32 ? 4 : 2;
+  const int64_t count[3] = {c.n_pages, c.kv_heads, c.page_tokens};
+  const int64_t stride[3] = {c.page_stride, c.head_stride, c.token_stride};
+  int64_t end = row;
+  for (int i = 0; i < 3; ++i) {
+    int64_t span;
+    if (stride[i] < (count[i] > 1 ? row : 0))
+      return fail(OKQ_E_SHAPE, "%s cache stride %lld is smaller than a row of %lld bytes", what, (long long)stride[i],
+                  (long long)row);
+    if (stride[i] % align != 0)
+      return fail(OKQ_E_ALIGN, "%s cache stride %lld is not a multiple of %lld bytes", what, (long long)stride[i],
+                  (long long)align);
+    if (!mul_ok(count[i] - 1, stride[i], span) || span > INT64_MAX - end)
+      return fail(OKQ_E_SHAPE, "%s cache byte length overflows", what);
+    end += span;
+  }
+  if (!c.k || !c.v) return fail(OKQ_E_ARG, "%s cache null pointer (k=%p v=%p)", what, c.k, c.v);
+  if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % (uintptr_t)align != 0)
+    return fail(OKQ_E_ALIGN, "%s cache k and v must be %lld-byte aligned", what, (long long)align);
+  out = {(int)c.type, (int)c.n_pages, (int)c.page_tokens, (int)c.kv_heads, (int)c.head_dim, c.page_stride,
+         c.head_stride, c.token_stride, static_cast<uint8_t *>(c.k), static_cast<uint8_t *>(c.v)};
+  return ok();
+}
+
+// `rows` rows of `width` 4-byte elements, `stride` apart.
+okq_status validate_rows(const char *what, const char *name, const void *p, int64_t rows, int64_t width,
+                         int64_t stride) {
+  int64_t n;
+  if (stride < (rows > 1 ? width : 0) || !mul_ok(rows, std::max(stride, width), n) || n > INT64_MAX / 8)
+    return fail(OKQ_E_SHAPE, "%s %s stride=%lld does not hold rows of %lld, or overflows", what, name,
+                (long long)stride, (long long)width);
+  if (!p) return fail(OKQ_E_ARG, "%s %s is null", what, name);
+  if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(OKQ_E_ALIGN, "%s %s must be 4-byte aligned", what, name);
+  return ok();
 }
 
 }  // namespace
@@ -1085,6 +1139,196 @@ okq_status okq_mlp_gated_silu_q(const float *x, int64_t rows, int64_t hidden, in
   }
   return linear_impl(gate_buf, false, rows, intermediate, down_type, down_w, down_bytes, hidden, nullptr, out, stream,
                      Path::Auto);
+}
+
+okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                            int64_t v_stride, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                            const float *q_norm, const float *k_norm, float epsilon, const int32_t *positions,
+                            const float *inv_freq, int64_t rotary, int interleaved, float *q_out, int64_t q_out_stride,
+                            float *k_out, int64_t k_out_stride, const okq_kv_pages *cache, const int64_t *slots,
+                            void *stream) {
+  const char *what = "qk_norm_rope";
+  if (tokens < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || tokens > INT32_MAX || head_dim > okq::kMaxHeadDim)
+    return fail(OKQ_E_SHAPE,
+                "%s tokens=%lld q_heads=%lld kv_heads=%lld head_dim=%lld: heads must be at least 1, head_dim 1 to %d",
+                what, (long long)tokens, (long long)q_heads, (long long)kv_heads, (long long)head_dim, okq::kMaxHeadDim);
+  int64_t rows;
+  if (q_heads > INT32_MAX / 4 || kv_heads > INT32_MAX / 4 || !mul_ok(tokens, q_heads + 2 * kv_heads, rows) ||
+      rows > INT32_MAX)
+    return fail(OKQ_E_SHAPE, "%s tokens*heads exceeds u32 launch limits", what);
+  if (rotary < 0 || rotary > head_dim || rotary % 2 != 0)
+    return fail(OKQ_E_SHAPE, "%s rotary=%lld must be even and at most head_dim=%lld", what, (long long)rotary,
+                (long long)head_dim);
+  if (!(epsilon >= 0.0f) || epsilon == INFINITY)
+    return fail(OKQ_E_ARG, "%s epsilon must be finite and non-negative, got %g", what, epsilon);
+  okq::RopeArgs a{};
+  okq_status st;
+  if (cache) {
+    st = validate_pages(what, *cache, a.cache);
+    if (st != OKQ_OK) return st;
+    if (cache->kv_heads != kv_heads || cache->head_dim != head_dim)
+      return fail(OKQ_E_SHAPE, "%s cache of %lld heads of %lld does not match kv_heads=%lld head_dim=%lld", what,
+                  (long long)cache->kv_heads, (long long)cache->head_dim, (long long)kv_heads, (long long)head_dim);
+  }
+  if (tokens == 0) return ok();
+  st = validate_rows(what, "q", q, tokens, q_heads * head_dim, q_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "k", k, tokens, kv_heads * head_dim, k_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "q_out", q_out, tokens, q_heads * head_dim, q_out_stride);
+  if (st == OKQ_OK && k_out) st = validate_rows(what, "k_out", k_out, tokens, kv_heads * head_dim, k_out_stride);
+  if (st == OKQ_OK && cache) st = validate_rows(what, "v", v, tokens, kv_heads * head_dim, v_stride);
+  if (st == OKQ_OK && rotary) st = validate_rows(what, "positions", positions, 1, tokens, tokens);
+  if (st == OKQ_OK && rotary) st = validate_rows(what, "inv_freq", inv_freq, 1, rotary / 2, rotary / 2);
+  if (st != OKQ_OK) return st;
+  if (!cache && !k_out) return fail(OKQ_E_ARG, "%s needs a cache or k_out for the keys", what);
+  if (cache && !slots) return fail(OKQ_E_ARG, "%s slots is null", what);
+  if (((reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm)) & 3u) ||
+      (reinterpret_cast<uintptr_t>(slots) & 7u))
+    return fail(OKQ_E_ALIGN, "%s norm weights must be 4-byte and slots 8-byte aligned", what);
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_out_stride = q_out_stride;
+  a.k_out_stride = k_out_stride;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.slots = slots;
+  a.tokens = (int)tokens;
+  a.q_heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.rotary = (int)rotary;
+  a.interleaved = interleaved != 0;
+  a.eps = epsilon;
+  return hip_status(okq::launch_rope(a, info.cu_count, static_cast<hipStream_t>(stream)), "qk_norm_rope launch");
+}
+
+okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, int64_t q_heads,
+                               const okq_kv_pages *cache, const int32_t *block_table, int64_t table_width,
+                               const int32_t *lengths, int64_t max_length, float scale, float softcap, int64_t window,
+                               float *out, int64_t out_stride, float *lse, void *stream) {
+  const char *what = "paged_attention";
+  if (!cache) return fail(OKQ_E_ARG, "%s cache is null", what);
+  okq::AttnArgs a{};
+  okq_status st = validate_pages(what, *cache, a.cache);
+  if (st != OKQ_OK) return st;
+  int64_t rows, span;
+  if (seqs < 0 || q_heads < 1 || q_heads % cache->kv_heads != 0)
+    return fail(OKQ_E_SHAPE, "%s seqs=%lld q_heads=%lld: q_heads must be a positive multiple of kv_heads=%lld", what,
+                (long long)seqs, (long long)q_heads, (long long)cache->kv_heads);
+  if (!mul_ok(seqs, q_heads, rows) || rows > INT32_MAX || q_heads > INT32_MAX)
+    return fail(OKQ_E_SHAPE, "%s seqs*q_heads exceeds u32 launch limits", what);
+  if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > INT32_MAX)
+    return fail(OKQ_E_SHAPE, "%s table_width=%lld max_length=%lld window=%lld must not be negative nor exceed 32 bits",
+                what, (long long)table_width, (long long)max_length, (long long)window);
+  if (!std::isfinite(scale) || !(softcap >= 0.0f) || softcap == INFINITY)
+    return fail(OKQ_E_ARG, "%s scale must be finite and softcap finite and non-negative, got %g and %g", what, scale,
+                softcap);
+  if (seqs == 0) return ok();
+  const int64_t width = q_heads * cache->head_dim;
+  st = validate_rows(what, "q", q, seqs, width, q_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "out", out, seqs, width, out_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "lengths", lengths, 1, seqs, seqs);
+  if (st == OKQ_OK && table_width) st = validate_rows(what, "block_table", block_table, seqs, table_width, table_width);
+  if (st == OKQ_OK && lse) st = validate_rows(what, "lse", lse, seqs, q_heads, q_heads);
+  if (st != OKQ_OK) return st;
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.seqs = (int)seqs;
+  a.q_heads = (int)q_heads;
+  a.group = (int)(q_heads / cache->kv_heads);
+  a.table = block_table;
+  a.lengths = lengths;
+  a.table_width = (int)table_width;
+  a.max_len = (int)(mul_ok(table_width, cache->page_tokens, span) ? std::min(max_length, span) : max_length);
+  a.scale = scale;
+  a.softcap = softcap;
+  a.window = (int)std::min<int64_t>(window, INT32_MAX);
+  a.out = out;
+  a.lse = lse;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
+  return hip_status(okq::launch_attention(a, s), "paged_attention launch");
+}
+
+okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_t rows, int64_t vocab,
+                              const int32_t *history, int64_t history_stride, const int32_t *history_len,
+                              const int32_t *history_start, const float *repetition, const float *frequency,
+                              const float *presence, const int32_t *bias_ids, const float *bias, int64_t bias_stride,
+                              const int32_t *bias_len, const uint32_t *mask, int64_t mask_stride, float *out,
+                              int64_t out_stride, int32_t *best, void *stream) {
+  const char *what = "logits_process";
+  if (rows < 0 || vocab < 1 || vocab > INT32_MAX - 65536)
+    return fail(OKQ_E_SHAPE, "%s rows=%lld vocab=%lld: vocab must be at least 1 and below 2^31 - 65536", what,
+                (long long)rows, (long long)vocab);
+  if (rows > INT32_MAX / (vocab / 1024 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
+  if (history_stride < 0 || bias_stride < 0 || mask_stride < 0 || history_stride > INT32_MAX || bias_stride > INT32_MAX)
+    return fail(OKQ_E_SHAPE,
+                "%s history_stride=%lld bias_stride=%lld mask_stride=%lld must not be negative nor exceed 32 bits", what,
+                (long long)history_stride, (long long)bias_stride, (long long)mask_stride);
+  if (rows == 0) return ok();
+  okq_status st = validate_rows(what, "logits", logits, rows, vocab, logits_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "out", out, rows, vocab, out_stride);
+  if (st == OKQ_OK && history) st = validate_rows(what, "history", history, rows, history_stride, history_stride);
+  if (st == OKQ_OK && history) st = validate_rows(what, "history_len", history_len, 1, rows, rows);
+  if (st == OKQ_OK && history_start) st = validate_rows(what, "history_start", history_start, 1, rows, rows);
+  if (st == OKQ_OK && repetition) st = validate_rows(what, "repetition", repetition, 1, rows, rows);
+  if (st == OKQ_OK && frequency) st = validate_rows(what, "frequency", frequency, 1, rows, rows);
+  if (st == OKQ_OK && presence) st = validate_rows(what, "presence", presence, 1, rows, rows);
+  if (st == OKQ_OK && bias_ids) st = validate_rows(what, "bias_ids", bias_ids, rows, bias_stride, bias_stride);
+  if (st == OKQ_OK && bias_ids) st = validate_rows(what, "bias", bias, rows, bias_stride, bias_stride);
+  if (st == OKQ_OK && bias_ids) st = validate_rows(what, "bias_len", bias_len, 1, rows, rows);
+  if (st == OKQ_OK && mask) st = validate_rows(what, "mask", mask, rows, (vocab + 31) / 32, mask_stride);
+  if (st == OKQ_OK && best) st = validate_rows(what, "best", best, 1, rows, rows);
+  if (st != OKQ_OK) return st;
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  okq::LogitsArgs a{};
+  a.x = logits;
+  a.out = out;
+  a.x_stride = logits_stride;
+  a.out_stride = out_stride;
+  a.hist_stride = history_stride;
+  a.bias_stride = bias_stride;
+  a.mask_stride = mask_stride;
+  a.rows = (int)rows;
+  a.vocab = (int)vocab;
+  a.hist = history;
+  a.hist_len = history_len;
+  a.hist_start = history_start;
+  a.bias_ids = bias_ids;
+  a.bias_len = bias_len;
+  a.rep = repetition;
+  a.freq = frequency;
+  a.pres = presence;
+  a.bias = bias;
+  a.mask = mask;
+  a.best = best;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
+  void *ws = nullptr;
+  if (best) {
+    st = get_workspace(dev, s, okq::logits_workspace(rows, vocab), &ws, 2);
+    if (st != OKQ_OK) return st;
+  }
+  return hip_status(okq::launch_logits(a, ws, s), "logits_process launch");
 }
 
 okq_status okq_linear_out_by_in_q_noalloc(const float *x, int64_t rows, int64_t in_features, uint32_t w_type,

@@ -24,6 +24,15 @@ _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint32
 _int = ctypes.c_int
+_f32 = ctypes.c_float
+
+
+class KvPages(ctypes.Structure):
+    """okq_kv_pages: a paged key-value cache (strides in bytes, k and v device pointers)."""
+    _fields_ = [("type", _u32), ("n_pages", _i64), ("page_tokens", _i64), ("kv_heads", _i64), ("head_dim", _i64),
+                ("page_stride", _i64), ("head_stride", _i64), ("token_stride", _i64), ("k", _vp), ("v", _vp)]
+
+
 _linear_sig = (_int, [_vp, _i64, _i64, _u32, _vp, _u64, _i64, _vp, _vp, _vp])
 SIGNATURES = {
     "okq_backend_name": (ctypes.c_char_p, []),
@@ -53,6 +62,12 @@ SIGNATURES = {
                                           _vp, _vp]),
     "okq_mlp_gated_silu_q": (_int, [_vp, _i64, _i64, _i64, _u32, _vp, _u64, _u32, _vp, _u64, _u32, _vp, _u64,
                                     _vp, _vp, _vp, _vp]),
+    "okq_qk_norm_rope": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _vp,
+                                _i64, _int, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "okq_paged_attention": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _f32, _f32, _i64, _vp, _i64,
+                                   _vp, _vp]),
+    "okq_logits_process": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
+                                  _vp, _i64, _vp, _i64, _vp, _vp]),
     "okq_set_launch_events": (_int, [_vp, _vp]),
     "okq_quantize": (_int, [_u32, _vp, _i64, _vp, _vp]),
     "okq_fill_normal": (_int, [_u64, _i64, _i64, ctypes.c_float, _vp, _vp]),
