@@ -3,6 +3,14 @@
 //   out = sum_t p_t V[t] / sum_t p_t,  p_t = exp(s_t - max s),
 //   s_t = scale * q . K[t]  (softcap * tanh(s_t / softcap) where capped),
 // over the visible tokens, in one pass with the running maximum and sum.
+//
+// attention_tiles_kernel: matrix instructions over tiles of cached rows, a
+// long cache split over workgroups and joined by the last of them.
+// attention_rows_kernel: rows that the tiles' vector loads do not reach
+// (head_dim or addresses that are no multiple of 16 bytes, head_dim above
+// 256), one value at a time.
+#include <algorithm>
+
 #include "okq_device.h"
 #include "okq_internal.h"
 
@@ -10,7 +18,7 @@ namespace okq {
 
 namespace {
 
-constexpr int kF32 = 0, kF16 = 1;
+constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
 
 // Value i of a cached row.
 __device__ __forceinline__ float cached(int type, const uint8_t *row, int i) {
@@ -81,8 +89,667 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(AttnArgs a) {
   if (a.lse && threadIdx.x == 0) a.lse[(int64_t)seq * a.q_heads + h] = top == INFINITY ? top : base + logf(sum);
 }
 
-hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
-  launch_timed(attention_rows_kernel, dim3((unsigned)(a.seqs * a.q_heads)), dim3(256), 0u, s, a);
+
+// ---- tiles ---------------------------------------------------------------------
+//
+// A wave takes tiles of 32 cached tokens (16 of f32) of one key/value head and
+// the up to 16 query heads that read it, which share every cached byte.
+//
+//   S[token][head] = K Q^T        A = K: lane (token = l & 15, 8 dims from 8 (l >> 4))
+//   O[dim][head]  += V^T P        B = P: lane (head = l & 15, 8 tokens of l >> 4)
+//
+// S leaves the matrix unit with lane (head = l & 15) holding tokens
+// 4 (l >> 4) + 0..3 of each 16, which is what the second product wants as its
+// B operand if tokens {4g..4g+3, 16+4g..16+4g+3} are called its k-slots
+// 8g..8g+7: the probabilities never leave their lane.  Maxima, sums and the
+// rescaling of O are per head, so per lane too.  V comes in rows (a lane takes
+// 8 dims of its 8 tokens, 16 lanes a row's 128) and is turned by v_perm.
+//
+// The queries and probabilities are f32, the matrix instructions' operands 16
+// bits: each is split into limbs whose sum is the f32 value -- three bf16
+// (exactly), two f16 (to 2^-23, scaled by a power of two into f16's range) --
+// and each limb gets its product.  The cached values are exact operands as they
+// are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
+// against the 16 KB that a SIMD's share of the memory takes 5000 cycles for.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr int kWaves = 8;             // of a workgroup
+constexpr int kHeads = 16;            // query heads of a tile
+constexpr int kMergeFloats = 8192;    // LDS for the waves' outputs
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+struct TileArgs {
+  AttnArgs a;
+  uint32_t page_mul, page_shift;  // token / page_tokens = umulhi(2 token, mul) >> shift
+  int head_tiles;                 // tiles of kHeads query heads in a group
+  int units;                      // at least total chunks of all sequences that the split aims at
+  int min_tiles;                  // of a chunk
+  float *part;                    // a slot for each chunk of a split sequence and head tile: O, maxima, sums
+  uint32_t *arrived;              // at a sequence's first slot: chunks that are done; zero between calls
+};
+
+template <int kType>
+constexpr bool kIsF32 = kType == kF32;
+
+__device__ __forceinline__ float cross_max(float v) {  // over the four 16-lane rows
+  auto a = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+  v = fmaxf(as_f32(a[0]), as_f32(a[1]));
+  a = __builtin_amdgcn_permlane16_swap(as_u32(v), as_u32(v), false, false);
+  return fmaxf(as_f32(a[0]), as_f32(a[1]));
+}
+__device__ __forceinline__ float cross_sum(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+  v = as_f32(a[0]) + as_f32(a[1]);
+  a = __builtin_amdgcn_permlane16_swap(as_u32(v), as_u32(v), false, false);
+  return as_f32(a[0]) + as_f32(a[1]);
+}
+// Lane `kLane` of the own 16-lane row.
+template <int kLane>
+__device__ __forceinline__ float row_lane(float v) {
+  return as_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)as_u32(v), 0x150 + kLane, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint32_t hi16s(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t lo16s(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+
+// Eight f32 values as three bf16 limbs (cut off, so their sum is exact).
+__device__ __forceinline__ void limbs_bf16(const float (&x)[8], u32x4 (&limb)[3]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      limb[k][j] = hi16s(as_u32(a), as_u32(b));
+      a -= as_f32(as_u32(a) & 0xffff0000u);
+      b -= as_f32(as_u32(b) & 0xffff0000u);
+    }
+  }
+}
+// Eight f32 values below 2^15 as two f16 limbs, off by at most 2^-23 of the
+// value (2^-25 for what lies below f16's normal range).
+__device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+    const f16x2 lo = {(_Float16)(x[2 * j] - (float)hi[0]), (_Float16)(x[2 * j + 1] - (float)hi[1])};
+    limb[0][j] = __builtin_bit_cast(uint32_t, hi);
+    limb[1][j] = __builtin_bit_cast(uint32_t, lo);
+  }
+}
+// Two codes, in bytes 0 and 2 (the others zero), as f16: with its top bit
+// flipped a code is code + 128, and 0x6400 | b is the f16 1024 + b.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
+  const f16x2 c = {(_Float16)1152.0f, (_Float16)1152.0f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, two ^ 0x64806480u) - c);
+}
+// x[j] = p[j] * (lane j, or 8 + j, of the own row's d): a block's scales of the
+// lane's eight token slots.
+__device__ __forceinline__ void scale_slots(const float (&p)[8], float d, int upper, float (&x)[8]) {
+  if (!upper) {
+    x[0] = p[0] * row_lane<0>(d), x[1] = p[1] * row_lane<1>(d), x[2] = p[2] * row_lane<2>(d);
+    x[3] = p[3] * row_lane<3>(d), x[4] = p[4] * row_lane<4>(d), x[5] = p[5] * row_lane<5>(d);
+    x[6] = p[6] * row_lane<6>(d), x[7] = p[7] * row_lane<7>(d);
+  } else {
+    x[0] = p[0] * row_lane<8>(d), x[1] = p[1] * row_lane<9>(d), x[2] = p[2] * row_lane<10>(d);
+    x[3] = p[3] * row_lane<11>(d), x[4] = p[4] * row_lane<12>(d), x[5] = p[5] * row_lane<13>(d);
+    x[6] = p[6] * row_lane<14>(d), x[7] = p[7] * row_lane<15>(d);
+  }
+}
+template <int kType>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (kType == kBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+template <class T>
+__device__ __forceinline__ T load_any(const uint8_t *p) {  // any alignment
+  T v;
+  __builtin_memcpy(&v, p, sizeof v);
+  return v;
+}
+
+}  // namespace
+
+template <int kType, int NC>  // head_dim <= 32 NC
+__global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_kernel(TileArgs ta) {
+  constexpr bool kF = kIsF32<kType>, kQ = kType == kQ8_0;
+  constexpr int kL = kType == kBF16 ? 3 : 2;                       // limbs
+  constexpr int kSub = kF ? 1 : 2;                                  // 16-token products of a tile
+  constexpr int kTile = 16 * kSub, kSlots = 4 * kSub;               // tokens of a tile, of a lane
+  constexpr int kQC = kF ? 2 * NC : NC;                             // chunks of 16 (f32) or 32 dims
+  // dims of a lane's load of V; Q8_0: two, so that a product's 16 rows (one
+  // dim of each lane) lie in one block and its scales can go with P
+  constexpr int kVD = kQ ? 2 : kF || NC <= 2 ? 4 : 8;
+  constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such loads
+  constexpr int kQLimbs = kF ? 1 : kL;
+  __shared__ u32x4 q_lds[kQC * kQLimbs * 64];
+  __shared__ float merge[kMergeFloats];
+  __shared__ int64_t offs[kWaves][kTile];
+  __shared__ float m_lds[kWaves][kHeads], l_lds[kWaves][kHeads];
+  __shared__ f32x4 joined[64 * kWaves];
+  __shared__ int last;
+
+  const AttnArgs &a = ta.a;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int D = a.cache.head_dim, heads_kv = a.cache.kv_heads * ta.head_tiles;
+
+  // ---- which chunk: all tiles in order, a sequence's shared out evenly over
+  // its chunks; every wave counts them by itself
+  const int head_at = (int)(blockIdx.x % (unsigned)heads_kv), unit = (int)(blockIdx.x / (unsigned)heads_kv);
+  auto visible = [&](int s, int &first) {  // tokens of sequence s, and where they begin
+    int len = s < a.seqs ? a.lengths[s] : 0;
+    len = len < a.max_len ? len : a.max_len;
+    len = len > 0 ? len : 0;
+    first = a.window && len > a.window ? len - a.window : 0;
+    return len - first;
+  };
+  int64_t total = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    int first;
+    int64_t t = (visible(s0 + lane, first) + kTile - 1) / kTile;
+    for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
+    total += t;
+  }
+  const int64_t even = (total + ta.units - 1) / ta.units;
+  const int chunk = __builtin_amdgcn_readfirstlane(even < ta.min_tiles ? ta.min_tiles : (int)even);
+  int seq = -1, at = 0, chunks = 0, slot = 0, lo = 0, hi = 0, before = 0, alone = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    int first;
+    const int tokens = visible(s0 + lane, first), tiles = (tokens + kTile - 1) / kTile;
+    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? (tiles + chunk - 1) / chunk : 1;
+    int sum = c;
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const uint64_t who = __ballot(unit >= before + sum - c && unit < before + sum), ones = __ballot(c == 1);
+    if (who) {
+      const int w = __builtin_ctzll(who);
+      seq = s0 + w;
+      chunks = __builtin_amdgcn_readlane(c, w);
+      slot = before + __builtin_amdgcn_readlane(sum - c, w);
+      at = unit - slot;
+      slot -= alone + __builtin_popcountll(ones & ((1ull << w) - 1));  // sequences of one chunk need no slot
+      const int per = (__builtin_amdgcn_readlane(tiles, w) + chunks - 1) / chunks;
+      const int begin = __builtin_amdgcn_readlane(first, w), end = begin + __builtin_amdgcn_readlane(tokens, w);
+      lo = begin + at * per * kTile;
+      hi = lo + per * kTile < end ? lo + per * kTile : end;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    alone += __builtin_popcountll(ones);
+  }
+  if (seq < 0) return;  // the split needs fewer workgroups than it may
+  const int kvh = head_at / ta.head_tiles, ht = head_at % ta.head_tiles;
+  const int heads = a.group - ht * kHeads < kHeads ? a.group - ht * kHeads : kHeads;
+  const int h0 = kvh * a.group + ht * kHeads;
+
+  // ---- queries into LDS, as the product's B operand
+  const float *q = a.q + (int64_t)seq * a.q_stride + (int64_t)h0 * D;
+  float s_scale = a.scale;  // of this lane's head
+  {
+    constexpr int kPer = kF ? 4 : 8;  // a lane's dims of a chunk
+    float mx = 0.0f;
+    if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
+      for (int i = g; i < D; i += 4) mx = fmaxf(mx, n < heads ? fabsf(q[(int64_t)n * D + i]) : 0.0f);
+      mx = cross_max(mx);
+    }
+    const int e = mx > 0.0f && mx < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(mx) : 0;
+    s_scale = ldexpf(s_scale, -e);
+    for (int c = wave; c < kQC; c += kWaves) {
+      float x[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = 4 * kPer * c + kPer * g + j;
+        x[j] = n < heads && i < D ? q[(int64_t)n * D + i] : 0.0f;
+        if constexpr (!kF && kType != kBF16) x[j] = ldexpf(x[j], e);
+      }
+      if constexpr (kF) {
+        q_lds[c * 64 + lane] = u32x4{as_u32(x[0]), as_u32(x[1]), as_u32(x[2]), as_u32(x[3])};
+      } else {
+        u32x4 limb[kL];
+        if constexpr (kType == kBF16) limbs_bf16(x, limb);
+        else limbs_f16(x, limb);
+#pragma unroll
+        for (int k = 0; k < kL; ++k) q_lds[(c * kL + k) * 64 + lane] = limb[k];
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- the chunk's tiles
+  const float to_log2 = a.softcap > 0.0f ? s_scale : s_scale * kLog2e;
+  f32x4 o[kVG * kVD];
+#pragma unroll
+  for (int t = 0; t < kVG * kVD; ++t) o[t] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+  int d_exp = -100;  // Q8_0: O is scaled so that scales of up to 2^d_exp keep P's limbs in range
+  const int32_t *table = a.table + (int64_t)seq * a.table_width;
+  const uint8_t *kb = a.cache.k + (int64_t)kvh * a.cache.head_stride, *vb = a.cache.v + (int64_t)kvh * a.cache.head_stride;
+  const int pt = a.cache.page_tokens;
+  auto page_of = [&](int t) { return (int)(__umulhi(2u * (uint32_t)t, ta.page_mul) >> ta.page_shift); };
+  int page = 0;
+  {
+    const int t = lo + wave * kTile + (lane & (kTile - 1));
+    if (t < hi) page = table[page_of(t)];
+  }
+  for (int t0 = lo + wave * kTile; t0 < hi; t0 += kWaves * kTile) {
+    // this tile's row offsets, lane i the i-th token's
+    const int t = t0 + (lane & (kTile - 1));
+    int64_t off = -1;
+    if (t < hi && (unsigned)page < (unsigned)a.cache.n_pages)
+      off = page * a.cache.page_stride + (int64_t)(t - page_of(t) * pt) * a.cache.token_stride;
+    const bool whole = __ballot(off < 0) == 0;
+    if (lane < kTile) offs[wave][lane] = off;
+    wave_sync();
+    const int tn = t + kWaves * kTile;
+    if (tn < hi) page = table[page_of(tn)];
+    int64_t ko[kSub], vo[kSlots];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) ko[s] = offs[wave][16 * s + n];
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) vo[j] = offs[wave][16 * (j >> 2) + 4 * g + (j & 3)];
+    float dk[(NC + 1) / 2], dv[(NC + 1) / 2];  // Q8_0: scale of token slot n & 7, block 2 i + (n >> 3)
+    if constexpr (kQ) {
+      const int64_t own = offs[wave][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
+      const int64_t row = own < 0 ? 0 : own;
+#pragma unroll
+      for (int i = 0; i < (NC + 1) / 2; ++i) {
+        const int b = 2 * i + (n >> 3), bb = 32 * b < D ? kQ8Bytes * b : 0;
+        dk[i] = f16_bits_hw(load_any<uint16_t>(kb + row + bb));
+        dv[i] = own < 0 ? 0.0f : f16_bits_hw(load_any<uint16_t>(vb + row + bb));
+      }
+    }
+    wave_sync();  // the next tile overwrites the offsets
+    unsigned seen = 0;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      seen |= (vo[j] >= 0 ? 1u : 0u) << j;
+      vo[j] = vo[j] < 0 ? 0 : vo[j];
+    }
+    // rows: K in the A operand's order, V in rows; dims past head_dim repeat
+    // dim 0 (their queries are zero, their outputs dropped)
+    u32x4 kr[kSub][kQC];
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      const uint8_t *row = kb + (ko[s] < 0 ? 0 : ko[s]);
+#pragma unroll
+      for (int c = 0; c < kQC; ++c) {
+        if constexpr (kQ) {
+          const u32x2 v = load_any<u32x2>(row + (32 * c < D ? kQ8Bytes * c + 8 * g + 2 : 2));
+          kr[s][c] = u32x4{v[0], v[1], 0, 0};
+        } else {
+          const int i = kF ? 16 * c + 4 * g : 32 * c + 8 * g;
+          kr[s][c] = *reinterpret_cast<const u32x4 *>(row + (i < D ? i * (kF ? 4 : 2) : 0));
+        }
+      }
+    }
+    u32x4 vr[kSlots][kVG];
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+#pragma unroll
+      for (int v = 0; v < kVG; ++v) {
+        const int i = 16 * kVD * v + kVD * n, ii = i < D ? i : 0;
+        const uint8_t *row = vb + vo[j];
+        if constexpr (kQ) {
+          vr[j][v] = u32x4{load_any<uint16_t>(row + (ii >> 5) * kQ8Bytes + 2 + (ii & 31)), 0, 0, 0};
+        } else if constexpr (kF || kVD == 8) {
+          vr[j][v] = *reinterpret_cast<const u32x4 *>(row + ii * (kF ? 4 : 2));
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2 *>(row + ii * 2);
+          vr[j][v] = u32x4{w[0], w[1], 0, 0};
+        }
+      }
+    }
+    // scores
+    float p[kSlots];
+    if constexpr (kQ) {  // a block's products, times its keys' scales
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) p[j] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kQC; ++c) {
+        float b[8];
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) {
+          u32x4 op;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            op[2 * w] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c010c00u));
+            op[2 * w + 1] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c030c02u));
+          }
+          f32x4 t = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < kL; ++k) t = mfma<kType>(op, q_lds[(c * kL + k) * 64 + lane], t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[4 * s + i] = t[i];
+        }
+        float x[8];
+        scale_slots(b, dk[c >> 1], c & 1, x);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) p[j] += x[j];
+      }
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
+    }
+#pragma unroll
+    for (int s = 0; s < kSub && !kQ; ++s) {
+      f32x4 acc = {0, 0, 0, 0};
+      if constexpr (kF) {
+#pragma unroll
+        for (int c = 0; c < kQC; ++c) {
+          const u32x4 qq = q_lds[c * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc = mfma4(as_f32(kr[s][c][e]), as_f32(qq[e]), acc);
+        }
+      } else {
+        f32x4 part[kL];
+#pragma unroll
+        for (int k = 0; k < kL; ++k) part[k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kQC; ++c)
+#pragma unroll
+          for (int k = 0; k < kL; ++k) part[k] = mfma<kType>(kr[s][c], q_lds[(c * kL + k) * 64 + lane], part[k]);
+        acc = part[kL - 1];
+#pragma unroll
+        for (int k = kL - 2; k >= 0; --k) acc += part[k];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i] * to_log2;
+    }
+    if (a.softcap > 0.0f) {
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) p[j] = a.softcap * tanhf(p[j] / a.softcap) * kLog2e;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        const bool in = seen >> j & 1u;
+        p[j] = in ? p[j] : -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kVG; ++v)
+          if constexpr (!kQ) vr[j][v] = in ? vr[j][v] : u32x4{0, 0, 0, 0};
+      }
+    }
+    float top = p[0];
+#pragma unroll
+    for (int j = 1; j < kSlots; ++j) top = fmaxf(top, p[j]);
+    top = fmaxf(m, cross_max(top));
+    float keep = 1.0f;
+    bool grown = __ballot(top > m) != 0;
+    if (grown) keep = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+    int d_new = d_exp;
+    if constexpr (kQ) {
+      // the largest scale of the tile against what O's scaling allows for
+      float dm = 0.0f;
+#pragma unroll
+      for (int i = 0; i < (NC + 1) / 2; ++i) dm = fmaxf(dm, fabsf(dv[i]));
+      const int de = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) : -100;
+      if (__ballot(de > d_exp) != 0) {
+        int w = de;
+        for (int d = 1; d < 64; d *= 2) {
+          const int x = __shfl_xor(w, d);
+          w = x > w ? x : w;
+        }
+        d_new = __builtin_amdgcn_readfirstlane(w);
+        grown = true;
+      }
+    }
+    if (grown) {
+      l *= keep;
+      float f = keep;
+      if constexpr (kQ) f = ldexpf(keep, d_exp - d_new);
+      d_exp = d_new;
+#pragma unroll
+      for (int t = 0; t < kVG * kVD; ++t) o[t] *= f;
+    }
+    m = top;
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(p[j] - base);
+      l += p[j];
+    }
+    // outputs
+    if constexpr (kF) {
+#pragma unroll
+      for (int v = 0; v < kVG; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[4 * v + e] = mfma4(as_f32(vr[j][v][e]), p[j], o[4 * v + e]);
+    } else if constexpr (kQ) {
+      const float up = ldexpf(1.0f, 14 - d_exp);
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) p[j] *= up;
+#pragma unroll
+      for (int v = 0; v < kVG; ++v) {  // block v
+        float x[8];
+        scale_slots(p, dv[v >> 1], v & 1, x);
+        u32x4 limb[kL];
+        limbs_f16(x, limb);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          u32x4 op;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            op[j] = codes_f16(__builtin_amdgcn_perm(vr[2 * j + 1][v][0], vr[2 * j][v][0], d ? 0x0c050c01u : 0x0c040c00u));
+#pragma unroll
+          for (int k = 0; k < kL; ++k) o[2 * v + d] = mfma<kType>(op, limb[k], o[2 * v + d]);
+        }
+      }
+    } else {
+      u32x4 limb[kL];
+      if constexpr (kType == kBF16) {
+        limbs_bf16(p, limb);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] *= 16384.0f;
+        limbs_f16(p, limb);
+      }
+#pragma unroll
+      for (int v = 0; v < kVG; ++v)
+#pragma unroll
+        for (int d = 0; d < kVD; ++d) {
+          u32x4 op;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            op[j] = d & 1 ? hi16s(vr[2 * j][v][d / 2], vr[2 * j + 1][v][d / 2])
+                          : lo16s(vr[2 * j][v][d / 2], vr[2 * j + 1][v][d / 2]);
+#pragma unroll
+          for (int k = 0; k < kL; ++k) o[v * kVD + d] = mfma<kType>(op, limb[k], o[v * kVD + d]);
+        }
+    }
+  }
+
+  // ---- the waves' results into one
+  l = cross_sum(l);
+  if (g == 0) {
+    m_lds[wave][n] = m;
+    l_lds[wave][n] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY, L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m_lds[w][n]);
+  const float M0 = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) L += l_lds[w][n] * __builtin_amdgcn_exp2f(m_lds[w][n] - M0);
+  float f = __builtin_amdgcn_exp2f(m - M0);
+  if constexpr (kQ) f = ldexpf(f, d_exp - 14);
+  else if constexpr (kType == kF16) f *= 1.0f / 16384.0f;
+  const int DS = D + 4, fit = kMergeFloats / (kWaves * DS);  // heads that fit at once
+  const int slot_floats = (a.group < kHeads ? a.group : kHeads) * (D + 2);
+  float *part = ta.part + ((int64_t)(slot + at) * heads_kv + head_at) * slot_floats;
+  float *out = a.out + (int64_t)seq * a.out_stride + (int64_t)h0 * D;
+  __syncthreads();
+  if (wave == 0 && g == 0) {
+    m_lds[0][n] = M;
+    l_lds[0][n] = L;
+  }
+  for (int p0 = 0; p0 < heads; p0 += fit) {
+    const int count = heads - p0 < fit ? heads - p0 : fit;
+    if (n >= p0 && n < p0 + count) {
+      float *row = merge + (wave * fit + n - p0) * DS;
+#pragma unroll
+      for (int v = 0; v < kVG; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int dim = 16 * kVD * v + kVD * (4 * g + i);
+#pragma unroll
+          for (int d = 0; d < kVD; d += 2)
+            if (dim + d < D) {
+              row[dim + d] = o[v * kVD + d][i] * f;
+              row[dim + d + 1] = o[v * kVD + d + 1][i] * f;
+            }
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < count * D; e += 64 * kWaves) {
+      const int h = e / D, dim = e - h * D;
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) v += merge[(w * fit + h) * DS + dim];
+      const float sum = l_lds[0][p0 + h];
+      if (chunks > 1) part[(p0 + h) * D + dim] = v;
+      else out[(p0 + h) * D + dim] = sum == 0.0f ? 0.0f : v / sum;
+    }
+    __syncthreads();
+  }
+  if (chunks == 1) {
+    if (a.lse && tid < heads) {
+      const float top = m_lds[0][tid];
+      a.lse[(int64_t)seq * a.q_heads + h0 + tid] =
+          top == -INFINITY ? top : (top + __builtin_amdgcn_logf(l_lds[0][tid])) * kLn2;
+    }
+    return;
+  }
+
+  // ---- the chunks' results into one, by the workgroup that finishes last, in
+  // the chunks' order
+  if (tid < heads) {
+    part[heads * D + tid] = m_lds[0][tid];
+    part[heads * D + heads + tid] = l_lds[0][tid];
+  }
+  __threadfence();
+  __syncthreads();
+  uint32_t *arrived = ta.arrived + (int64_t)slot * heads_kv + head_at;
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)chunks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  if (tid == 0) *arrived = 0;
+  const float *first = ta.part + ((int64_t)slot * heads_kv + head_at) * slot_floats;
+  const int64_t step = (int64_t)heads_kv * slot_floats;
+  float *weight = merge;  // [heads][chunks] (the launch keeps chunks * kHeads within kMergeFloats)
+  for (int h = wave; h < heads; h += kWaves) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < chunks; i += 64) top = fmaxf(top, first[i * step + heads * D + h]);
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (int i = lane; i < chunks; i += 64) {
+      const float w = __builtin_amdgcn_exp2f(first[i * step + heads * D + h] - base);
+      weight[h * chunks + i] = w;
+      sum += w * first[i * step + heads * D + heads + h];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) {
+      l_lds[0][h] = sum;
+      if (a.lse)
+        a.lse[(int64_t)seq * a.q_heads + h0 + h] =
+            top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+  }
+  __syncthreads();
+  const int quads = heads * D / 4, teams = 64 * kWaves / quads > 1 ? 64 * kWaves / quads : 1;
+  const int team = tid / quads < teams ? tid / quads : 0;  // threads past the teams repeat the first's work
+  for (int q0 = teams > 1 ? tid % quads : tid; q0 < quads; q0 += teams > 1 ? quads : 64 * kWaves) {
+    const int h = 4 * q0 / D;
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = team; i < chunks; i += teams)
+      v += weight[h * chunks + i] * load_any<f32x4>(reinterpret_cast<const uint8_t *>(first + i * step + 4 * q0));
+    if (teams > 1) {
+      joined[tid] = v;
+      continue;
+    }
+    const float sum = l_lds[0][h];
+    for (int i = 0; i < 4; ++i) out[4 * q0 + i] = sum == 0.0f ? 0.0f : v[i] / sum;
+  }
+  if (teams > 1) {
+    __syncthreads();
+    if (tid < quads) {
+      f32x4 v = joined[tid];
+      for (int t = 1; t < teams; ++t) v += joined[t * quads + tid];
+      const float sum = l_lds[0][4 * tid / D];
+      for (int i = 0; i < 4; ++i) out[4 * tid + i] = sum == 0.0f ? 0.0f : v[i] / sum;
+    }
+  }
+}
+
+namespace {
+
+template <int kType>
+void launch_tiles(const TileArgs &ta, unsigned grid, hipStream_t s) {
+  const int D = ta.a.cache.head_dim;
+  if (D <= 64) launch_timed(attention_tiles_kernel<kType, 2>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
+  else if (D <= 96) launch_timed(attention_tiles_kernel<kType, 3>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
+  else if (D <= 128) launch_timed(attention_tiles_kernel<kType, 4>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
+  else launch_timed(attention_tiles_kernel<kType, 8>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
+}
+
+}  // namespace
+
+AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
+  AttnPlan p{};
+  const KvPages &c = a.cache;
+  const uint64_t strides = (uint64_t)(c.page_stride | c.head_stride | c.token_stride);
+  const bool aligned = ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | strides) & 15u) == 0;
+  p.tiles = c.head_dim <= 256 && (c.type == kQ8_0 || (aligned && c.head_dim % (c.type == kF32 ? 4 : 8) == 0));
+  if (!p.tiles) return p;
+  const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
+  const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
+  const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;  // workgroups that run at once
+  p.min_tiles = kWaves;
+  p.units = (int)std::max<int64_t>(1, std::min<int64_t>(aim / pairs, kMergeFloats / kHeads));
+  const int64_t chunks = std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles);
+  p.grid = pairs * std::min<int64_t>(a.seqs + (chunks > 1 ? p.units : 0), a.seqs * chunks);
+  if (chunks > 1) {
+    p.arrived_bytes = (size_t)(2 * p.units * pairs) * sizeof(uint32_t);
+    p.part_bytes = (size_t)(2 * p.units * pairs) * (size_t)(std::min(a.group, kHeads) * (c.head_dim + 2)) * sizeof(float);
+  }
+  return p;
+}
+
+hipError_t launch_attention(const AttnArgs &a, const AttnPlan &p, void *part, void *arrived, hipStream_t s) {
+  if (!p.tiles) {
+    launch_timed(attention_rows_kernel, dim3((unsigned)(a.seqs * a.q_heads)), dim3(256), 0u, s, a);
+    return hipGetLastError();
+  }
+  // token / page_tokens for tokens below 2^31: floor(2^(31 + n) / d) + 1 with
+  // 2^n >= d, times the token, loses nothing above bit 31 + n
+  const uint32_t d = (uint32_t)a.cache.page_tokens;
+  uint32_t n = 0;
+  while (((uint64_t)1 << n) < d) ++n;
+  TileArgs ta{a, (uint32_t)(((uint64_t)1 << (31 + n)) / d + 1), n, (a.group + kHeads - 1) / kHeads, p.units, p.min_tiles,
+              static_cast<float *>(part), static_cast<uint32_t *>(arrived)};
+  const unsigned grid = (unsigned)p.grid;
+  if (a.cache.type == kF32) launch_tiles<kF32>(ta, grid, s);
+  else if (a.cache.type == kF16) launch_tiles<kF16>(ta, grid, s);
+  else if (a.cache.type == kBF16) launch_tiles<kBF16>(ta, grid, s);
+  else launch_tiles<kQ8_0>(ta, grid, s);
   return hipGetLastError();
 }
 

@@ -256,7 +256,17 @@ struct AttnArgs {
   float *out, *lse;
   KvPages cache;
 };
-hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
+// How a call runs, and the workspace that it takes: chunks' results, and
+// counters that are zero before and after every call.
+struct AttnPlan {
+  bool tiles;  // else one value at a time, without workspace
+  int units, min_tiles;
+  int64_t grid;
+  size_t part_bytes, arrived_bytes;
+};
+AttnPlan attention_plan(const AttnArgs &a, int cu_count);
+hipError_t launch_attention(const AttnArgs &a, const AttnPlan &plan, void *part, void *arrived, hipStream_t s);
+hipError_t launch_zero(void *p, size_t bytes, hipStream_t s);  // bytes a multiple of 4
 
 struct LogitsArgs {
   const float *x;

@@ -118,4 +118,15 @@ hipError_t launch_swiglu(const float *gate, const float *up, int64_t n, float *o
   return hipGetLastError();
 }
 
+__global__ __launch_bounds__(256) void zero_kernel(uint32_t *p, size_t n) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0;
+}
+
+hipError_t launch_zero(void *p, size_t bytes, hipStream_t s) {
+  const size_t n = bytes / 4, blocks = (n + 255) / 256;
+  hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s,
+                     static_cast<uint32_t *>(p), n);
+  return hipGetLastError();
+}
+
 }  // namespace okq

@@ -223,6 +223,7 @@ okq_status validate_rmsnorm(const float *x, int64_t rows, int64_t hidden, const 
 // process ends, also after the stream is destroyed.
 struct Workspace {
   void *ptr = nullptr;
+  void *zeroed = nullptr;  // == ptr: filled with zeros once (slots that are kept zero)
   size_t bytes = 0;
   size_t refused = SIZE_MAX;  // an allocation that failed: asked for again only where a call needs it all
 };
@@ -231,7 +232,8 @@ std::map<std::tuple<int, hipStream_t, int>, Workspace> g_ws;
 
 // Slot 0 serves the linear itself (GEMM planes, bf16 widening); slot 1 holds
 // a neighbour's output (normalised or gated activations) that a linear then
-// reads, so the two never alias.
+// reads, so the two never alias; slot 2 the keys of okq_logits_process, slots
+// 3 and 4 the chunks' results and the counters of okq_paged_attention.
 enum class Grow { Ok, Capture, Alloc };
 
 // At least `bytes`; a buffer that has to grow, or could outside a capture,
@@ -272,6 +274,22 @@ okq_status workspace_status(Grow g, size_t bytes) {
 
 okq_status get_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot = 0) {
   return workspace_status(grow_workspace(dev, s, bytes, bytes, out, slot), bytes);
+}
+
+// A slot whose kernels leave it zero: filled on the stream when it is new.
+okq_status get_zeroed_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot) {
+  okq_status st = get_workspace(dev, s, bytes, out, slot);
+  if (st != OKQ_OK) return st;
+  size_t fresh = 0;
+  {
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    Workspace &w = g_ws[{dev, s, slot}];
+    if (w.zeroed != w.ptr) {
+      w.zeroed = w.ptr;
+      fresh = w.bytes;
+    }
+  }
+  return fresh ? hip_status(okq::launch_zero(*out, fresh / 4 * 4, s), "workspace fill") : ok();
 }
 
 // The workspace of a plan, its K split lowered where it cannot be had.
@@ -1154,7 +1172,7 @@ okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, in
                 what, (long long)tokens, (long long)q_heads, (long long)kv_heads, (long long)head_dim, okq::kMaxHeadDim);
   int64_t rows;
   if (q_heads > INT32_MAX / 4 || kv_heads > INT32_MAX / 4 || !mul_ok(tokens, q_heads + 2 * kv_heads, rows) ||
-      rows > INT32_MAX)
+      rows > (1 << 25))  // waves
     return fail(OKQ_E_SHAPE, "%s tokens*heads exceeds u32 launch limits", what);
   if (rotary < 0 || rotary > head_dim || rotary % 2 != 0)
     return fail(OKQ_E_SHAPE, "%s rotary=%lld must be even and at most head_dim=%lld", what, (long long)rotary,
@@ -1226,9 +1244,9 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   if (seqs < 0 || q_heads < 1 || q_heads % cache->kv_heads != 0)
     return fail(OKQ_E_SHAPE, "%s seqs=%lld q_heads=%lld: q_heads must be a positive multiple of kv_heads=%lld", what,
                 (long long)seqs, (long long)q_heads, (long long)cache->kv_heads);
-  if (!mul_ok(seqs, q_heads, rows) || rows > INT32_MAX || q_heads > INT32_MAX)
+  if (!mul_ok(seqs, q_heads, rows) || rows > (1 << 22))  // workgroups of up to 512 threads
     return fail(OKQ_E_SHAPE, "%s seqs*q_heads exceeds u32 launch limits", what);
-  if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > INT32_MAX)
+  if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > INT32_MAX - 65536)
     return fail(OKQ_E_SHAPE, "%s table_width=%lld max_length=%lld window=%lld must not be negative nor exceed 32 bits",
                 what, (long long)table_width, (long long)max_length, (long long)window);
   if (!std::isfinite(scale) || !(softcap >= 0.0f) || softcap == INFINITY)
@@ -1263,7 +1281,14 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   a.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
   std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
-  return hip_status(okq::launch_attention(a, s), "paged_attention launch");
+  const okq::AttnPlan plan = okq::attention_plan(a, info.cu_count);
+  void *part = nullptr, *arrived = nullptr;
+  if (plan.part_bytes) {
+    st = get_workspace(dev, s, plan.part_bytes, &part, 3);
+    if (st == OKQ_OK) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 4);
+    if (st != OKQ_OK) return st;
+  }
+  return hip_status(okq::launch_attention(a, plan, part, arrived, s), "paged_attention launch");
 }
 
 okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_t rows, int64_t vocab,
@@ -1276,7 +1301,7 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
   if (rows < 0 || vocab < 1 || vocab > INT32_MAX - 65536)
     return fail(OKQ_E_SHAPE, "%s rows=%lld vocab=%lld: vocab must be at least 1 and below 2^31 - 65536", what,
                 (long long)rows, (long long)vocab);
-  if (rows > INT32_MAX / (vocab / 1024 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
+  if (rows > (1 << 23) / (vocab / 4096 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
   if (history_stride < 0 || bias_stride < 0 || mask_stride < 0 || history_stride > INT32_MAX || bias_stride > INT32_MAX)
     return fail(OKQ_E_SHAPE,
                 "%s history_stride=%lld bias_stride=%lld mask_stride=%lld must not be negative nor exceed 32 bits", what,
