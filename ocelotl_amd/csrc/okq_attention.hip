@@ -219,6 +219,25 @@ __device__ __forceinline__ T load_any(const uint8_t *p) {  // any alignment
   return v;
 }
 
+// Chunks' results go between workgroups past the XCDs' own L2 caches, by stores
+// and loads of agent scope; the writer waits for its stores (results_stored)
+// before it counts itself done.  A release fence in their place writes the
+// XCD's whole L2 back, for every wave: 303 us instead of 64 on a ragged
+// batch of 64 sequences, 177 instead of 98 on one of 131072 tokens.
+__device__ __forceinline__ void put(float *p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 get4(const float *p) {  // p 8-byte aligned
+  const uint64_t *u = reinterpret_cast<const uint64_t *>(p);
+  const uint64_t a = __hip_atomic_load(u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t b = __hip_atomic_load(u + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return f32x4{as_f32((uint32_t)a), as_f32((uint32_t)(a >> 32)), as_f32((uint32_t)b), as_f32((uint32_t)(b >> 32))};
+}
+__device__ __forceinline__ void results_stored() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 }  // namespace
 
 template <int kType, int NC>  // head_dim <= 32 NC
@@ -622,7 +641,7 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) v += merge[(w * fit + h) * DS + dim];
       const float sum = l_lds[0][p0 + h];
-      if (chunks > 1) part[(p0 + h) * D + dim] = v;
+      if (chunks > 1) put(part + (p0 + h) * D + dim, v);
       else out[(p0 + h) * D + dim] = sum == 0.0f ? 0.0f : v / sum;
     }
     __syncthreads();
@@ -639,30 +658,29 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
   // ---- the chunks' results into one, by the workgroup that finishes last, in
   // the chunks' order
   if (tid < heads) {
-    part[heads * D + tid] = m_lds[0][tid];
-    part[heads * D + heads + tid] = l_lds[0][tid];
+    put(part + heads * D + tid, m_lds[0][tid]);
+    put(part + heads * D + heads + tid, l_lds[0][tid]);
   }
-  __threadfence();
+  results_stored();
   __syncthreads();
   uint32_t *arrived = ta.arrived + (int64_t)slot * heads_kv + head_at;
   if (tid == 0)
-    last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)chunks - 1;
+    last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)chunks - 1;
   __syncthreads();
   if (!last) return;
-  __threadfence();
-  if (tid == 0) *arrived = 0;
+  if (tid == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const float *first = ta.part + ((int64_t)slot * heads_kv + head_at) * slot_floats;
   const int64_t step = (int64_t)heads_kv * slot_floats;
   float *weight = merge;  // [heads][chunks] (the launch keeps chunks * kHeads within kMergeFloats)
   for (int h = wave; h < heads; h += kWaves) {
     float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < chunks; i += 64) top = fmaxf(top, first[i * step + heads * D + h]);
+    for (int i = lane; i < chunks; i += 64) top = fmaxf(top, get(first + i * step + heads * D + h));
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
     const float base = top == -INFINITY ? 0.0f : top;
     for (int i = lane; i < chunks; i += 64) {
-      const float w = __builtin_amdgcn_exp2f(first[i * step + heads * D + h] - base);
+      const float w = __builtin_amdgcn_exp2f(get(first + i * step + heads * D + h) - base);
       weight[h * chunks + i] = w;
-      sum += w * first[i * step + heads * D + heads + h];
+      sum += w * get(first + i * step + heads * D + heads + h);
     }
     sum = wave_sum(sum);
     if (lane == 0) {
@@ -680,7 +698,7 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
     f32x4 v = {0, 0, 0, 0};
 #pragma unroll 8
     for (int i = team; i < chunks; i += teams)
-      v += weight[h * chunks + i] * load_any<f32x4>(reinterpret_cast<const uint8_t *>(first + i * step + 4 * q0));
+      v += weight[h * chunks + i] * get4(first + i * step + 4 * q0);
     if (teams > 1) {
       joined[tid] = v;
       continue;
