@@ -121,9 +121,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int kWaves = 8;             // of a workgroup
 constexpr int kHeads = 16;            // query heads of a tile
-constexpr int kMergeFloats = 8192;    // LDS for the waves' outputs
+constexpr int kMergeFloats = 4096;    // LDS for the waves' outputs
+constexpr int kWaves = 4;             // of a workgroup
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct TileArgs {
@@ -136,9 +136,19 @@ struct TileArgs {
   uint32_t *arrived;              // at a sequence's first slot: chunks that are done; zero between calls
 };
 
-template <int kType>
-constexpr bool kIsF32 = kType == kF32;
+constexpr int kGridY = 32768;
 
+// Inclusive sum over the lanes: within 16 lanes by shifts, then each row's last
+// lane added to the rows after it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
+  return v;
+}
 __device__ __forceinline__ float cross_max(float v) {  // over the four 16-lane rows
   auto a = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
   v = fmaxf(as_f32(a[0]), as_f32(a[1]));
@@ -241,8 +251,8 @@ __device__ __forceinline__ void results_stored() { asm volatile("s_waitcnt vmcnt
 }  // namespace
 
 template <int kType, int NC>  // head_dim <= 32 NC
-__global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_kernel(TileArgs ta) {
-  constexpr bool kF = kIsF32<kType>, kQ = kType == kQ8_0;
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArgs ta) {
+  constexpr bool kF = kType == kF32, kQ = kType == kQ8_0;
   constexpr int kL = kType == kBF16 ? 3 : 2;                       // limbs
   constexpr int kSub = kF ? 1 : 2;                                  // 16-token products of a tile
   constexpr int kTile = 16 * kSub, kSlots = 4 * kSub;               // tokens of a tile, of a lane
@@ -252,10 +262,12 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
   constexpr int kVD = kQ ? 2 : kF || NC <= 2 ? 4 : 8;
   constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such loads
   constexpr int kQLimbs = kF ? 1 : kL;
+  constexpr int kSB = (NC + 1) / 2;                                 // registers of Q8_0 scales
   __shared__ u32x4 q_lds[kQC * kQLimbs * 64];
   __shared__ float merge[kMergeFloats];
-  __shared__ int64_t offs[kWaves][kTile];
+  __shared__ int64_t offs[kWaves][2][kTile];
   __shared__ float m_lds[kWaves][kHeads], l_lds[kWaves][kHeads];
+  __shared__ float q_max[kQC][kHeads];
   __shared__ f32x4 joined[64 * kWaves];
   __shared__ int last;
 
@@ -266,33 +278,28 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
 
   // ---- which chunk: all tiles in order, a sequence's shared out evenly over
   // its chunks; every wave counts them by itself
-  const int head_at = (int)(blockIdx.x % (unsigned)heads_kv), unit = (int)(blockIdx.x / (unsigned)heads_kv);
-  auto visible = [&](int s, int &first) {  // tokens of sequence s, and where they begin
-    int len = s < a.seqs ? a.lengths[s] : 0;
+  const int head_at = (int)blockIdx.x, unit = (int)(blockIdx.z * (unsigned)kGridY + blockIdx.y);
+  int tokens = 0, first = 0, tiles = 0;  // of sequence s0 + lane
+  auto look = [&](int s0) {
+    int len = s0 + lane < a.seqs ? a.lengths[s0 + lane] : 0;
     len = len < a.max_len ? len : a.max_len;
     len = len > 0 ? len : 0;
     first = a.window && len > a.window ? len - a.window : 0;
-    return len - first;
+    tokens = len - first;
+    tiles = (tokens + kTile - 1) / kTile;
   };
-  int64_t total = 0;
+  int total = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    int first;
-    int64_t t = (visible(s0 + lane, first) + kTile - 1) / kTile;
-    for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
-    total += t;
+    look(s0);
+    total += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   }
-  const int64_t even = (total + ta.units - 1) / ta.units;
-  const int chunk = __builtin_amdgcn_readfirstlane(even < ta.min_tiles ? ta.min_tiles : (int)even);
+  int chunk = (int)(((uint32_t)total + (uint32_t)ta.units - 1) / (uint32_t)ta.units);
+  chunk = chunk < ta.min_tiles ? ta.min_tiles : chunk;
   int seq = -1, at = 0, chunks = 0, slot = 0, lo = 0, hi = 0, before = 0, alone = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    int first;
-    const int tokens = visible(s0 + lane, first), tiles = (tokens + kTile - 1) / kTile;
-    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? (tiles + chunk - 1) / chunk : 1;
-    int sum = c;
-    for (int d = 1; d < 64; d *= 2) {
-      const int o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
+    if (a.seqs > 64) look(s0);
+    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? (int)(((uint32_t)(tiles + chunk) - 1) / (uint32_t)chunk) : 1;
+    const int sum = wave_scan(c);
     const uint64_t who = __ballot(unit >= before + sum - c && unit < before + sum), ones = __ballot(c == 1);
     if (who) {
       const int w = __builtin_ctzll(who);
@@ -301,7 +308,8 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
       slot = before + __builtin_amdgcn_readlane(sum - c, w);
       at = unit - slot;
       slot -= alone + __builtin_popcountll(ones & ((1ull << w) - 1));  // sequences of one chunk need no slot
-      const int per = (__builtin_amdgcn_readlane(tiles, w) + chunks - 1) / chunks;
+      const int per = chunks == 1 ? __builtin_amdgcn_readlane(tiles, w)
+                                  : (int)((uint32_t)(__builtin_amdgcn_readlane(tiles, w) + chunks - 1) / (uint32_t)chunks);
       const int begin = __builtin_amdgcn_readlane(first, w), end = begin + __builtin_amdgcn_readlane(tokens, w);
       lo = begin + at * per * kTile;
       hi = lo + per * kTile < end ? lo + per * kTile : end;
@@ -311,99 +319,42 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
     alone += __builtin_popcountll(ones);
   }
   if (seq < 0) return;  // the split needs fewer workgroups than it may
-  const int kvh = head_at / ta.head_tiles, ht = head_at % ta.head_tiles;
+  const int kvh = ta.head_tiles == 1 ? head_at : head_at / ta.head_tiles, ht = head_at - kvh * ta.head_tiles;
   const int heads = a.group - ht * kHeads < kHeads ? a.group - ht * kHeads : kHeads;
   const int h0 = kvh * a.group + ht * kHeads;
 
-  // ---- queries into LDS, as the product's B operand
-  const float *q = a.q + (int64_t)seq * a.q_stride + (int64_t)h0 * D;
-  float s_scale = a.scale;  // of this lane's head
-  {
-    constexpr int kPer = kF ? 4 : 8;  // a lane's dims of a chunk
-    float mx = 0.0f;
-    if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
-      for (int i = g; i < D; i += 4) mx = fmaxf(mx, n < heads ? fabsf(q[(int64_t)n * D + i]) : 0.0f);
-      mx = cross_max(mx);
-    }
-    const int e = mx > 0.0f && mx < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(mx) : 0;
-    s_scale = ldexpf(s_scale, -e);
-    for (int c = wave; c < kQC; c += kWaves) {
-      float x[kPer];
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int i = 4 * kPer * c + kPer * g + j;
-        x[j] = n < heads && i < D ? q[(int64_t)n * D + i] : 0.0f;
-        if constexpr (!kF && kType != kBF16) x[j] = ldexpf(x[j], e);
-      }
-      if constexpr (kF) {
-        q_lds[c * 64 + lane] = u32x4{as_u32(x[0]), as_u32(x[1]), as_u32(x[2]), as_u32(x[3])};
-      } else {
-        u32x4 limb[kL];
-        if constexpr (kType == kBF16) limbs_bf16(x, limb);
-        else limbs_f16(x, limb);
-#pragma unroll
-        for (int k = 0; k < kL; ++k) q_lds[(c * kL + k) * 64 + lane] = limb[k];
-      }
-    }
-  }
-  __syncthreads();
-
-  // ---- the chunk's tiles
-  const float to_log2 = a.softcap > 0.0f ? s_scale : s_scale * kLog2e;
-  f32x4 o[kVG * kVD];
-#pragma unroll
-  for (int t = 0; t < kVG * kVD; ++t) o[t] = f32x4{0, 0, 0, 0};
-  float m = -INFINITY, l = 0.0f;
-  int d_exp = -100;  // Q8_0: O is scaled so that scales of up to 2^d_exp keep P's limbs in range
+  // ---- loads of a tile: its rows' offsets (lane i the i-th token's) through
+  // LDS; K in the A operand's order, V in rows.  Dims past head_dim repeat dim
+  // 0 (their queries are zero, their outputs dropped).  A tile's page numbers
+  // are fetched two tiles ahead, its K when the products of the tile before
+  // have read theirs, its V likewise: the waits hide behind the other half.
   const int32_t *table = a.table + (int64_t)seq * a.table_width;
   const uint8_t *kb = a.cache.k + (int64_t)kvh * a.cache.head_stride, *vb = a.cache.v + (int64_t)kvh * a.cache.head_stride;
-  const int pt = a.cache.page_tokens;
+  const int pt = a.cache.page_tokens, mine = lane & (kTile - 1);
   auto page_of = [&](int t) { return (int)(__umulhi(2u * (uint32_t)t, ta.page_mul) >> ta.page_shift); };
-  int page = 0;
-  {
-    const int t = lo + wave * kTile + (lane & (kTile - 1));
-    if (t < hi) page = table[page_of(t)];
-  }
-  for (int t0 = lo + wave * kTile; t0 < hi; t0 += kWaves * kTile) {
-    // this tile's row offsets, lane i the i-th token's
-    const int t = t0 + (lane & (kTile - 1));
-    int64_t off = -1;
-    if (t < hi && (unsigned)page < (unsigned)a.cache.n_pages)
-      off = page * a.cache.page_stride + (int64_t)(t - page_of(t) * pt) * a.cache.token_stride;
-    const bool whole = __ballot(off < 0) == 0;
-    if (lane < kTile) offs[wave][lane] = off;
+  auto fetch_page = [&](int t0) { return t0 + mine < hi ? table[page_of(t0 + mine)] : -1; };
+  auto place = [&](int t0, int page, int buf) {  // the tile's offsets; a bit for each token that is not seen
+    const int t = t0 + mine;
+    const bool in = t < hi && (unsigned)page < (unsigned)a.cache.n_pages;
+    const int64_t off = page * a.cache.page_stride + (int64_t)(t - page_of(t) * pt) * a.cache.token_stride;
+    if (lane < kTile) offs[wave][buf][lane] = in ? off : 0;
     wave_sync();
-    const int tn = t + kWaves * kTile;
-    if (tn < hi) page = table[page_of(tn)];
-    int64_t ko[kSub], vo[kSlots];
-#pragma unroll
-    for (int s = 0; s < kSub; ++s) ko[s] = offs[wave][16 * s + n];
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) vo[j] = offs[wave][16 * (j >> 2) + 4 * g + (j & 3)];
-    float dk[(NC + 1) / 2], dv[(NC + 1) / 2];  // Q8_0: scale of token slot n & 7, block 2 i + (n >> 3)
+    return (uint32_t)__ballot(!in);  // lanes past kTile repeat
+  };
+  u32x4 kr[kSub][kQC], vr[kSlots][kVG];
+  float dk[kSB], dv[kSB];  // Q8_0: scale of token slot n & 7, block 2 i + (n >> 3)
+  auto load_k = [&](int buf) {
     if constexpr (kQ) {
-      const int64_t own = offs[wave][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
-      const int64_t row = own < 0 ? 0 : own;
+      const int64_t own = offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
 #pragma unroll
-      for (int i = 0; i < (NC + 1) / 2; ++i) {
-        const int b = 2 * i + (n >> 3), bb = 32 * b < D ? kQ8Bytes * b : 0;
-        dk[i] = f16_bits_hw(load_any<uint16_t>(kb + row + bb));
-        dv[i] = own < 0 ? 0.0f : f16_bits_hw(load_any<uint16_t>(vb + row + bb));
+      for (int i = 0; i < kSB; ++i) {
+        const int b = 2 * i + (n >> 3);
+        dk[i] = f16_bits_hw(load_any<uint16_t>(kb + own + (32 * b < D ? kQ8Bytes * b : 0)));
       }
     }
-    wave_sync();  // the next tile overwrites the offsets
-    unsigned seen = 0;
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
-      seen |= (vo[j] >= 0 ? 1u : 0u) << j;
-      vo[j] = vo[j] < 0 ? 0 : vo[j];
-    }
-    // rows: K in the A operand's order, V in rows; dims past head_dim repeat
-    // dim 0 (their queries are zero, their outputs dropped)
-    u32x4 kr[kSub][kQC];
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
-      const uint8_t *row = kb + (ko[s] < 0 ? 0 : ko[s]);
+      const uint8_t *row = kb + offs[wave][buf][16 * s + n];
 #pragma unroll
       for (int c = 0; c < kQC; ++c) {
         if constexpr (kQ) {
@@ -415,13 +366,22 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
         }
       }
     }
-    u32x4 vr[kSlots][kVG];
+  };
+  auto load_v = [&](int buf) {
+    if constexpr (kQ) {
+      const int64_t own = offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
+#pragma unroll
+      for (int i = 0; i < kSB; ++i) {
+        const int b = 2 * i + (n >> 3);
+        dv[i] = f16_bits_hw(load_any<uint16_t>(vb + own + (32 * b < D ? kQ8Bytes * b : 0)));
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
+      const uint8_t *row = vb + offs[wave][buf][16 * (j >> 2) + 4 * g + (j & 3)];
 #pragma unroll
       for (int v = 0; v < kVG; ++v) {
         const int i = 16 * kVD * v + kVD * n, ii = i < D ? i : 0;
-        const uint8_t *row = vb + vo[j];
         if constexpr (kQ) {
           vr[j][v] = u32x4{load_any<uint16_t>(row + (ii >> 5) * kQ8Bytes + 2 + (ii & 31)), 0, 0, 0};
         } else if constexpr (kF || kVD == 8) {
@@ -432,6 +392,84 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
         }
       }
     }
+  };
+  constexpr int kStep = kWaves * kTile;
+  int t0 = lo + wave * kTile, buf = 0;
+  int page = fetch_page(t0), page_next = fetch_page(t0 + kStep);
+  // the queries, requested before the first rows
+  constexpr int kPer = kF ? 4 : 8, kMy = (kQC + kWaves - 1) / kWaves;  // a lane's dims of a chunk, a wave's chunks
+  const float *q = a.q + (int64_t)seq * a.q_stride + (int64_t)h0 * D;
+  float x[kMy][kPer];
+#pragma unroll
+  for (int u = 0; u < kMy; ++u)
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const int i = 4 * kPer * (wave + u * kWaves) + kPer * g + j;
+      f32x4 v = {0, 0, 0, 0};  // head_dim is a multiple of four
+      if (n < heads && i < D) v = load_any<f32x4>(reinterpret_cast<const uint8_t *>(q + (int64_t)n * D + i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][j + e] = v[e];
+    }
+  uint32_t hidden = 0;
+  if (t0 < hi) {
+    hidden = place(t0, page, 0);
+    load_k(0);
+    load_v(0);
+  }
+
+  // ---- queries into LDS, as the product's B operand
+  float s_scale = a.scale;  // of this lane's head
+  if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
+#pragma unroll
+    for (int u = 0; u < kMy; ++u) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, fabsf(x[u][j]));
+      mx = cross_max(mx);
+      if (g == 0 && wave + u * kWaves < kQC) q_max[wave + u * kWaves][n] = mx;
+    }
+    __syncthreads();
+    float mx = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kQC; ++c) mx = fmaxf(mx, q_max[c][n]);
+    const int e = mx > 0.0f && mx < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(mx) : 0;
+    s_scale = ldexpf(s_scale, -e);
+#pragma unroll
+    for (int u = 0; u < kMy; ++u)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) x[u][j] = ldexpf(x[u][j], e);
+  }
+#pragma unroll
+  for (int u = 0; u < kMy; ++u) {
+    const int c = wave + u * kWaves;
+    if (c >= kQC) break;
+    if constexpr (kF) {
+      q_lds[c * 64 + lane] = u32x4{as_u32(x[u][0]), as_u32(x[u][1]), as_u32(x[u][2]), as_u32(x[u][3])};
+    } else {
+      u32x4 limb[kL];
+      if constexpr (kType == kBF16) limbs_bf16(x[u], limb);
+      else limbs_f16(x[u], limb);
+#pragma unroll
+      for (int k = 0; k < kL; ++k) q_lds[(c * kL + k) * 64 + lane] = limb[k];
+    }
+  }
+  __syncthreads();
+
+  // ---- the chunk's tiles
+  const float to_log2 = a.softcap > 0.0f ? s_scale : s_scale * kLog2e;
+  f32x4 o[kVG * kVD];
+#pragma unroll
+  for (int t = 0; t < kVG * kVD; ++t) o[t] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+  int d_exp = -100;  // Q8_0: O is scaled so that scales of up to 2^d_exp keep P's limbs in range
+  while (t0 < hi) {
+    const bool more = t0 + kStep < hi;
+    uint32_t hidden_next = 0;
+    if (more) {
+      page = page_next;
+      page_next = fetch_page(t0 + 2 * kStep);
+      hidden_next = place(t0 + kStep, page, buf ^ 1);
+    }
     // scores
     float p[kSlots];
     if constexpr (kQ) {  // a block's products, times its keys' scales
@@ -440,6 +478,9 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
 #pragma unroll
       for (int c = 0; c < kQC; ++c) {
         float b[8];
+        u32x4 qq[kL];
+#pragma unroll
+        for (int k = 0; k < kL; ++k) qq[k] = q_lds[(c * kL + k) * 64 + lane];
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
           u32x4 op;
@@ -450,55 +491,67 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
           }
           f32x4 t = {0, 0, 0, 0};
 #pragma unroll
-          for (int k = 0; k < kL; ++k) t = mfma<kType>(op, q_lds[(c * kL + k) * 64 + lane], t);
+          for (int k = 0; k < kL; ++k) t = mfma<kType>(op, qq[k], t);
 #pragma unroll
           for (int i = 0; i < 4; ++i) b[4 * s + i] = t[i];
         }
-        float x[8];
-        scale_slots(b, dk[c >> 1], c & 1, x);
+        float y[8];
+        scale_slots(b, dk[c >> 1], c & 1, y);
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j) p[j] += x[j];
+        for (int j = 0; j < kSlots; ++j) p[j] += y[j];
       }
+    } else {
+      constexpr int kAcc = kF ? 4 : kL;  // one sum a limb, or a quarter of the dims: products that do not wait for each other
+      f32x4 part[kSub][kAcc];
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
-    }
+      for (int s = 0; s < kSub; ++s)
 #pragma unroll
-    for (int s = 0; s < kSub && !kQ; ++s) {
-      f32x4 acc = {0, 0, 0, 0};
-      if constexpr (kF) {
+        for (int k = 0; k < kAcc; ++k) part[s][k] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < kQC; ++c) {
-          const u32x4 qq = q_lds[c * 64 + lane];
+      for (int c = 0; c < kQC; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc = mfma4(as_f32(kr[s][c][e]), as_f32(qq[e]), acc);
+        for (int k = 0; k < kQLimbs; ++k) {
+          const u32x4 qq = q_lds[(c * kQLimbs + k) * 64 + lane];
+#pragma unroll
+          for (int s = 0; s < kSub; ++s) {
+            if constexpr (kF) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) part[s][e] = mfma4(as_f32(kr[s][c][e]), as_f32(qq[e]), part[s][e]);
+            } else {
+              part[s][k] = mfma<kType>(kr[s][c], qq, part[s][k]);
+            }
+          }
         }
-      } else {
-        f32x4 part[kL];
 #pragma unroll
-        for (int k = 0; k < kL; ++k) part[k] = f32x4{0, 0, 0, 0};
+      for (int s = 0; s < kSub; ++s) {
+        f32x4 acc = part[s][kAcc - 1];
 #pragma unroll
-        for (int c = 0; c < kQC; ++c)
+        for (int k = kAcc - 2; k >= 0; --k) acc += part[s][k];
 #pragma unroll
-          for (int k = 0; k < kL; ++k) part[k] = mfma<kType>(kr[s][c], q_lds[(c * kL + k) * 64 + lane], part[k]);
-        acc = part[kL - 1];
-#pragma unroll
-        for (int k = kL - 2; k >= 0; --k) acc += part[k];
+        for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i];
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i] * to_log2;
     }
+    if (more) load_k(buf ^ 1);
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
     if (a.softcap > 0.0f) {
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) p[j] = a.softcap * tanhf(p[j] / a.softcap) * kLog2e;
     }
-    if (!whole) {
+    if (hidden) {  // no weight, and values that are zero whatever the memory holds
+      const uint32_t own = hidden >> (4 * g);
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
-        const bool in = seen >> j & 1u;
-        p[j] = in ? p[j] : -INFINITY;
+        const bool out = own >> (16 * (j >> 2) + (j & 3)) & 1u;
+        p[j] = out ? -INFINITY : p[j];
 #pragma unroll
         for (int v = 0; v < kVG; ++v)
-          if constexpr (!kQ) vr[j][v] = in ? vr[j][v] : u32x4{0, 0, 0, 0};
+          if constexpr (!kQ) vr[j][v] = out ? u32x4{0, 0, 0, 0} : vr[j][v];
+      }
+      if constexpr (kQ) {
+        const bool out = own >> (16 * ((n & 7) >> 2) + (n & 3)) & 1u;
+#pragma unroll
+        for (int i = 0; i < kSB; ++i) dv[i] = out ? 0.0f : dv[i];
       }
     }
     float top = p[0];
@@ -513,13 +566,13 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
       // the largest scale of the tile against what O's scaling allows for
       float dm = 0.0f;
 #pragma unroll
-      for (int i = 0; i < (NC + 1) / 2; ++i) dm = fmaxf(dm, fabsf(dv[i]));
+      for (int i = 0; i < kSB; ++i) dm = fmaxf(dm, fabsf(dv[i]));
       const int de = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) : -100;
       if (__ballot(de > d_exp) != 0) {
         int w = de;
         for (int d = 1; d < 64; d *= 2) {
-          const int x = __shfl_xor(w, d);
-          w = x > w ? x : w;
+          const int y = __shfl_xor(w, d);
+          w = y > w ? y : w;
         }
         d_new = __builtin_amdgcn_readfirstlane(w);
         grown = true;
@@ -554,10 +607,10 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
       for (int j = 0; j < kSlots; ++j) p[j] *= up;
 #pragma unroll
       for (int v = 0; v < kVG; ++v) {  // block v
-        float x[8];
-        scale_slots(p, dv[v >> 1], v & 1, x);
+        float y[8];
+        scale_slots(p, dv[v >> 1], v & 1, y);
         u32x4 limb[kL];
-        limbs_f16(x, limb);
+        limbs_f16(y, limb);
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           u32x4 op;
@@ -590,6 +643,10 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
           for (int k = 0; k < kL; ++k) o[v * kVD + d] = mfma<kType>(op, limb[k], o[v * kVD + d]);
         }
     }
+    buf ^= 1;
+    if (more) load_v(buf);
+    hidden = hidden_next;
+    t0 += kStep;
   }
 
   // ---- the waves' results into one
@@ -626,23 +683,33 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int dim = 16 * kVD * v + kVD * (4 * g + i);
+          if constexpr (kVD == 2) {
+            if (dim >= D) continue;
+            row[dim] = o[v * kVD][i] * f;
+            row[dim + 1] = o[v * kVD + 1][i] * f;
+          } else {
 #pragma unroll
-          for (int d = 0; d < kVD; d += 2)
-            if (dim + d < D) {
-              row[dim + d] = o[v * kVD + d][i] * f;
-              row[dim + d + 1] = o[v * kVD + d + 1][i] * f;
-            }
+            for (int d = 0; d < kVD; d += 4)
+              if (dim + d < D)
+                *reinterpret_cast<f32x4 *>(row + dim + d) = f32x4{o[v * kVD + d][i], o[v * kVD + d + 1][i],
+                                                                  o[v * kVD + d + 2][i], o[v * kVD + d + 3][i]} * f;
+          }
         }
     }
     __syncthreads();
-    for (int e = tid; e < count * D; e += 64 * kWaves) {
-      const int h = e / D, dim = e - h * D;
-      float v = 0.0f;
+    const int dq = D / 4;
+    for (int e = tid; e < count * dq; e += 64 * kWaves) {
+      const int h = (int)((unsigned)e / (unsigned)dq), dim = 4 * (e - h * dq);
+      f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += merge[(w * fit + h) * DS + dim];
+      for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(merge + (w * fit + h) * DS + dim);
       const float sum = l_lds[0][p0 + h];
-      if (chunks > 1) put(part + (p0 + h) * D + dim, v);
-      else out[(p0 + h) * D + dim] = sum == 0.0f ? 0.0f : v / sum;
+      float *to = (chunks > 1 ? part : out) + (p0 + h) * D + dim;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (chunks > 1) put(to + i, v[i]);
+        else to[i] = sum == 0.0f ? 0.0f : v[i] / sum;
+      }
     }
     __syncthreads();
   }
@@ -669,63 +736,85 @@ __global__ __launch_bounds__(64 * kWaves, NC <= 4 ? 2 : 1) void attention_tiles_
   __syncthreads();
   if (!last) return;
   if (tid == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const float *first = ta.part + ((int64_t)slot * heads_kv + head_at) * slot_floats;
+  // Teams of threads take every teams-th chunk, a thread four outputs of one
+  // head, with a running maximum and sum of their own; the teams then meet in LDS.
+  const float *origin = ta.part + ((int64_t)slot * heads_kv + head_at) * slot_floats;
   const int64_t step = (int64_t)heads_kv * slot_floats;
-  float *weight = merge;  // [heads][chunks] (the launch keeps chunks * kHeads within kMergeFloats)
-  for (int h = wave; h < heads; h += kWaves) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < chunks; i += 64) top = fmaxf(top, get(first + i * step + heads * D + h));
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int i = lane; i < chunks; i += 64) {
-      const float w = __builtin_amdgcn_exp2f(get(first + i * step + heads * D + h) - base);
-      weight[h * chunks + i] = w;
-      sum += w * get(first + i * step + heads * D + heads + h);
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) {
-      l_lds[0][h] = sum;
-      if (a.lse)
-        a.lse[(int64_t)seq * a.q_heads + h0 + h] =
-            top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-    }
-  }
-  __syncthreads();
   const int quads = heads * D / 4, teams = 64 * kWaves / quads > 1 ? 64 * kWaves / quads : 1;
-  const int team = tid / quads < teams ? tid / quads : 0;  // threads past the teams repeat the first's work
-  for (int q0 = teams > 1 ? tid % quads : tid; q0 < quads; q0 += teams > 1 ? quads : 64 * kWaves) {
-    const int h = 4 * q0 / D;
+  const int rounds = (quads + 64 * kWaves - 1) / (64 * kWaves);  // 1 where there are teams
+  for (int r = 0; r < rounds; ++r) {
+    const int team = teams > 1 ? (int)((unsigned)tid / (unsigned)quads) : 0;
+    const int quad = teams > 1 ? tid - team * quads : tid + r * 64 * kWaves;
+    const bool in = quad < quads && team < teams;
+    const int h = in ? (int)((unsigned)(4 * quad) / (unsigned)D) : 0;
     f32x4 v = {0, 0, 0, 0};
-#pragma unroll 8
-    for (int i = team; i < chunks; i += teams)
-      v += weight[h * chunks + i] * get4(first + i * step + 4 * q0);
+    float top = -INFINITY, sum = 0.0f;
+    constexpr int kAtOnce = 8;
+    for (int i0 = in ? team : chunks; i0 < chunks; i0 += kAtOnce * teams) {
+      float mi[kAtOnce], li[kAtOnce];
+      f32x4 vi[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = i0 + u * teams;
+        const float *from = origin + (i < chunks ? i : i0) * step;
+        mi[u] = get(from + heads * D + h);
+        li[u] = get(from + heads * D + heads + h);
+        vi[u] = get4(from + 4 * quad);
+      }
+      float most = top;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (i0 + u * teams >= chunks) mi[u] = -INFINITY;
+        most = fmaxf(most, mi[u]);
+      }
+      const float base = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(top - base);
+      v *= keep;
+      sum *= keep;
+      top = most;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (i0 + u * teams >= chunks) continue;
+        const float w = __builtin_amdgcn_exp2f(mi[u] - base);
+        sum += w * li[u];
+        v += w * vi[u];
+      }
+    }
     if (teams > 1) {
       joined[tid] = v;
-      continue;
+      merge[2 * tid] = top;
+      merge[2 * tid + 1] = sum;
+      __syncthreads();
+      if (team > 0) return;
+      float most = top;
+      for (int t = 1; t < teams; ++t) most = fmaxf(most, merge[2 * (t * quads + quad)]);
+      const float base = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(top - base);
+      v *= keep;
+      sum *= keep;
+      for (int t = 1; t < teams; ++t) {
+        const int from = t * quads + quad;
+        const float w = __builtin_amdgcn_exp2f(merge[2 * from] - base);
+        sum += w * merge[2 * from + 1];
+        v += w * joined[from];
+      }
+      top = most;
     }
-    const float sum = l_lds[0][h];
-    for (int i = 0; i < 4; ++i) out[4 * q0 + i] = sum == 0.0f ? 0.0f : v[i] / sum;
-  }
-  if (teams > 1) {
-    __syncthreads();
-    if (tid < quads) {
-      f32x4 v = joined[tid];
-      for (int t = 1; t < teams; ++t) v += joined[t * quads + tid];
-      const float sum = l_lds[0][4 * tid / D];
-      for (int i = 0; i < 4; ++i) out[4 * tid + i] = sum == 0.0f ? 0.0f : v[i] / sum;
-    }
+    if (!in) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[4 * quad + i] = sum == 0.0f ? 0.0f : v[i] / sum;
+    if (a.lse && 4 * quad == h * D)
+      a.lse[(int64_t)seq * a.q_heads + h0 + h] = top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 }
 
 namespace {
 
 template <int kType>
-void launch_tiles(const TileArgs &ta, unsigned grid, hipStream_t s) {
+void launch_tiles(const TileArgs &ta, dim3 grid, hipStream_t s) {
   const int D = ta.a.cache.head_dim;
-  if (D <= 64) launch_timed(attention_tiles_kernel<kType, 2>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
-  else if (D <= 96) launch_timed(attention_tiles_kernel<kType, 3>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
-  else if (D <= 128) launch_timed(attention_tiles_kernel<kType, 4>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
-  else launch_timed(attention_tiles_kernel<kType, 8>, dim3(grid), dim3(64 * kWaves), 0u, s, ta);
+  if (D <= 64) launch_timed(attention_tiles_kernel<kType, 2>, grid, dim3(64 * kWaves), 0u, s, ta);
+  else if (D <= 96) launch_timed(attention_tiles_kernel<kType, 3>, grid, dim3(64 * kWaves), 0u, s, ta);
+  else if (D <= 128) launch_timed(attention_tiles_kernel<kType, 4>, grid, dim3(64 * kWaves), 0u, s, ta);
+  else launch_timed(attention_tiles_kernel<kType, 8>, grid, dim3(64 * kWaves), 0u, s, ta);
 }
 
 }  // namespace
@@ -739,11 +828,11 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   if (!p.tiles) return p;
   const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
-  const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;  // workgroups that run at once
+  const int64_t aim = 2 * (int64_t)cu_count;  // workgroups that run at once
   p.min_tiles = kWaves;
-  p.units = (int)std::max<int64_t>(1, std::min<int64_t>(aim / pairs, kMergeFloats / kHeads));
+  p.units = (int)std::max<int64_t>(1, aim / pairs);
   const int64_t chunks = std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles);
-  p.grid = pairs * std::min<int64_t>(a.seqs + (chunks > 1 ? p.units : 0), a.seqs * chunks);
+  p.grid = std::min<int64_t>(a.seqs + (chunks > 1 ? p.units : 0), a.seqs * chunks);
   if (chunks > 1) {
     p.arrived_bytes = (size_t)(2 * p.units * pairs) * sizeof(uint32_t);
     p.part_bytes = (size_t)(2 * p.units * pairs) * (size_t)(std::min(a.group, kHeads) * (c.head_dim + 2)) * sizeof(float);
@@ -763,7 +852,8 @@ hipError_t launch_attention(const AttnArgs &a, const AttnPlan &p, void *part, vo
   while (((uint64_t)1 << n) < d) ++n;
   TileArgs ta{a, (uint32_t)(((uint64_t)1 << (31 + n)) / d + 1), n, (a.group + kHeads - 1) / kHeads, p.units, p.min_tiles,
               static_cast<float *>(part), static_cast<uint32_t *>(arrived)};
-  const unsigned grid = (unsigned)p.grid;
+  const unsigned y = (unsigned)std::min<int64_t>(p.grid, kGridY);
+  const dim3 grid((unsigned)(a.cache.kv_heads * ta.head_tiles), y, (unsigned)((p.grid + y - 1) / y));
   if (a.cache.type == kF32) launch_tiles<kF32>(ta, grid, s);
   else if (a.cache.type == kF16) launch_tiles<kF16>(ta, grid, s);
   else if (a.cache.type == kBF16) launch_tiles<kBF16>(ta, grid, s);

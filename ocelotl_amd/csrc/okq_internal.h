@@ -261,7 +261,7 @@ struct AttnArgs {
 struct AttnPlan {
   bool tiles;  // else one value at a time, without workspace
   int units, min_tiles;
-  int64_t grid;
+  int64_t grid;  // chunks, at most
   size_t part_bytes, arrived_bytes;
 };
 AttnPlan attention_plan(const AttnArgs &a, int cu_count);

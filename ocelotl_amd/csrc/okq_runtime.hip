@@ -1249,6 +1249,9 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > INT32_MAX - 65536)
     return fail(OKQ_E_SHAPE, "%s table_width=%lld max_length=%lld window=%lld must not be negative nor exceed 32 bits",
                 what, (long long)table_width, (long long)max_length, (long long)window);
+  if (seqs > 0 && max_length / 16 + 1 > INT32_MAX / seqs)
+    return fail(OKQ_E_SHAPE, "%s seqs=%lld of max_length=%lld exceed u32 launch limits", what, (long long)seqs,
+                (long long)max_length);
   if (!std::isfinite(scale) || !(softcap >= 0.0f) || softcap == INFINITY)
     return fail(OKQ_E_ARG, "%s scale must be finite and softcap finite and non-negative, got %g and %g", what, scale,
                 softcap);
