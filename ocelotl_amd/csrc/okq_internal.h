@@ -278,9 +278,9 @@ struct LogitsArgs {
   const uint32_t *mask;
   int32_t *best;
 };
-// The largest-value keys of a row's slices lie in the workspace until the row
-// is whole; none is needed without `best`.
-size_t logits_workspace(int64_t rows, int64_t vocab);
-hipError_t launch_logits(const LogitsArgs &a, void *workspace, hipStream_t s);
+// Each row's largest key and its finished slices, zero before and after every
+// call; not used without `best`.
+size_t logits_workspace(int64_t rows);
+hipError_t launch_logits(const LogitsArgs &a, void *workspace, int cu_count, hipStream_t s);
 
 }  // namespace okq

@@ -1304,10 +1304,10 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
   if (rows < 0 || vocab < 1 || vocab > INT32_MAX - 65536)
     return fail(OKQ_E_SHAPE, "%s rows=%lld vocab=%lld: vocab must be at least 1 and below 2^31 - 65536", what,
                 (long long)rows, (long long)vocab);
-  if (rows > (1 << 23) / (vocab / 4096 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
-  if (history_stride < 0 || bias_stride < 0 || mask_stride < 0 || history_stride > INT32_MAX || bias_stride > INT32_MAX)
+  if (rows > (1 << 22) / (vocab / 2048 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
+  if (history_stride < 0 || bias_stride < 0 || mask_stride < 0 || history_stride >= 1 << 30 || bias_stride >= 1 << 30)
     return fail(OKQ_E_SHAPE,
-                "%s history_stride=%lld bias_stride=%lld mask_stride=%lld must not be negative nor exceed 32 bits", what,
+                "%s history_stride=%lld bias_stride=%lld mask_stride=%lld must not be negative, the first two below 2^30", what,
                 (long long)history_stride, (long long)bias_stride, (long long)mask_stride);
   if (rows == 0) return ok();
   okq_status st = validate_rows(what, "logits", logits, rows, vocab, logits_stride);
@@ -1353,10 +1353,10 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
   std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
   void *ws = nullptr;
   if (best) {
-    st = get_workspace(dev, s, okq::logits_workspace(rows, vocab), &ws, 2);
+    st = get_zeroed_workspace(dev, s, okq::logits_workspace(rows), &ws, 2);
     if (st != OKQ_OK) return st;
   }
-  return hip_status(okq::launch_logits(a, ws, s), "logits_process launch");
+  return hip_status(okq::launch_logits(a, ws, info.cu_count, s), "logits_process launch");
 }
 
 okq_status okq_linear_out_by_in_q_noalloc(const float *x, int64_t rows, int64_t in_features, uint32_t w_type,
