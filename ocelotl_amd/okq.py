@@ -96,6 +96,8 @@ _lib = None
 def lib() -> ctypes.CDLL:
     """Load libokq.so once (raises LibraryMissing if it was not built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):
@@ -122,8 +124,9 @@ def check(status: int, call: str) -> None:
 
 def call(name: str, *args) -> int:
     """Call an entry point and raise OkqStatusError on a non-OK status."""
-    rc = getattr(lib(), name)(*args)
-    check(rc, name)
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc != OK:
+        check(rc, name)
     return rc
 
 
