@@ -325,7 +325,7 @@ okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, in
  * [seqs, table_width] int32: the page of tokens j * page_tokens on of sequence
  * s is block_table[s, j]; entries outside [0, n_pages) hide their tokens and
  * are never followed.  lengths [seqs] int32 (device), read as at most
- * max_length and table_width * page_tokens; max_length (below 2^31 - 65536)
+ * max_length and table_width * page_tokens; max_length (at most 2^30)
  * bounds the launch.  lse [seqs, q_heads] f32 or NULL: log of the sum of
  * exp(f(scale * q . K)).  A sequence with nothing to see (length 0, hidden pages)
  * gets zeros and lse -inf; tokens outside the length or the window may hold

@@ -122,21 +122,37 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 namespace {
 
 constexpr int kHeads = 16;            // query heads of a tile
-constexpr int kMergeFloats = 4096;    // LDS for the waves' outputs
 constexpr int kWaves = 4;             // of a workgroup
+constexpr int kThreads = 64 * kWaves;
+constexpr int kPages = 512;           // pages that a workgroup holds the places of
+constexpr float kGrowth = 8.0f;       // how far (in powers of two) weights may exceed 1 before O is rescaled
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct TileArgs {
   AttnArgs a;
   uint32_t page_mul, page_shift;  // token / page_tokens = umulhi(2 token, mul) >> shift
+  uint32_t token_stride;
   int head_tiles;                 // tiles of kHeads query heads in a group
-  int units;                      // at least total chunks of all sequences that the split aims at
+  float inv_units;
+  int units;                      // chunks of all sequences together that the split aims at
   int min_tiles;                  // of a chunk
+  int segment;                    // tokens, a multiple of the waves' tiles, of at most kPages pages
+  uint32_t part_bytes;
   float *part;                    // a slot for each chunk of a split sequence and head tile: O, maxima, sums
   uint32_t *arrived;              // at a sequence's first slot: chunks that are done; zero between calls
 };
 
 constexpr int kGridY = 32768;
+
+// ceil(a / b) with 1 / b at hand.  Exact while a < 2^22 or the quotient is
+// below 2^20; past both it is off by less than 2^-22 of itself, which leaves a
+// split uneven by that much, and the last chunk still ends with its sequence.
+__device__ __forceinline__ int ceil_div(int a, int b, float inv_b) {
+  int q = (int)(((float)a + (float)b - 0.5f) * inv_b);
+  q += (int64_t)q * b < a ? 1 : 0;
+  q -= (int64_t)(q - 1) * b >= a ? 1 : 0;
+  return q;
+}
 
 // Inclusive sum over the lanes: within 16 lanes by shifts, then each row's last
 // lane added to the rows after it.
@@ -223,58 +239,49 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 template <class T>
-__device__ __forceinline__ T load_any(const uint8_t *p) {  // any alignment
+__device__ __forceinline__ T load_any(const void *p) {  // any alignment
   T v;
   __builtin_memcpy(&v, p, sizeof v);
   return v;
 }
 
 // Chunks' results go between workgroups past the XCDs' own L2 caches, by stores
-// and loads of agent scope; the writer waits for its stores (results_stored)
-// before it counts itself done.  A release fence in their place writes the
-// XCD's whole L2 back, for every wave: 303 us instead of 64 on a ragged
-// batch of 64 sequences, 177 instead of 98 on one of 131072 tokens.
-__device__ __forceinline__ void put(float *p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float get(const float *p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x4 get4(const float *p) {  // p 8-byte aligned
-  const uint64_t *u = reinterpret_cast<const uint64_t *>(p);
-  const uint64_t a = __hip_atomic_load(u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const uint64_t b = __hip_atomic_load(u + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return f32x4{as_f32((uint32_t)a), as_f32((uint32_t)(a >> 32)), as_f32((uint32_t)b), as_f32((uint32_t)(b >> 32))};
-}
+// and loads of agent scope (kAgent); the writer waits for its stores
+// (results_stored) before it counts itself done.  A release fence in their
+// place writes the XCD's whole L2 back, for every wave: 303 us instead of 64 on
+// a ragged batch of 64 sequences, 177 instead of 98 on one of 131072 tokens.
+constexpr int kAgent = 16;  // sc1
 __device__ __forceinline__ void results_stored() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 }  // namespace
 
-template <int kType, int NC>  // head_dim <= 32 NC
-__global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArgs ta) {
+template <int kType, int NC, bool kFull>  // head_dim <= 32 NC; kFull: equal
+__global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_kernel(TileArgs ta) {
   constexpr bool kF = kType == kF32, kQ = kType == kQ8_0;
-  constexpr int kL = kType == kBF16 ? 3 : 2;                       // limbs
+  constexpr int kL = kType == kBF16 ? 3 : kF ? 1 : 2;              // limbs
   constexpr int kSub = kF ? 1 : 2;                                  // 16-token products of a tile
   constexpr int kTile = 16 * kSub, kSlots = 4 * kSub;               // tokens of a tile, of a lane
-  constexpr int kQC = kF ? 2 * NC : NC;                             // chunks of 16 (f32) or 32 dims
+  constexpr int kStep = kWaves * kTile;
+  constexpr int kQC = kF ? 2 * NC : NC, kPer = kF ? 4 : 8;          // chunks of 16 (f32) or 32 dims, a lane's dims of one
   // dims of a lane's load of V; Q8_0: two, so that a product's 16 rows (one
   // dim of each lane) lie in one block and its scales can go with P
   constexpr int kVD = kQ ? 2 : kF || NC <= 2 ? 4 : 8;
   constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such loads
-  constexpr int kQLimbs = kF ? 1 : kL;
   constexpr int kSB = (NC + 1) / 2;                                 // registers of Q8_0 scales
-  __shared__ u32x4 q_lds[kQC * kQLimbs * 64];
+  constexpr bool kRegQ = NC <= (kQ ? 3 : 4);  // the queries' limbs in registers, every wave its own; else one copy in LDS
+  constexpr int kQuads = NC <= 2 ? 16 : NC <= 4 ? 32 : 64;          // threads of a row of outputs, four values each
+  __shared__ u32x4 q_lds[kRegQ ? 1 : kQC * kL * 64];
+  constexpr int kMergeFloats = NC <= 4 ? 4096 : 8192;  // LDS for the waves' outputs
   __shared__ float merge[kMergeFloats];
   __shared__ int64_t offs[kWaves][2][kTile];
+  __shared__ int64_t page_at[kPages];
   __shared__ float m_lds[kWaves][kHeads], l_lds[kWaves][kHeads];
-  __shared__ float q_max[kQC][kHeads];
-  __shared__ f32x4 joined[64 * kWaves];
   __shared__ int last;
 
   const AttnArgs &a = ta.a;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int D = a.cache.head_dim, heads_kv = a.cache.kv_heads * ta.head_tiles;
+  const int D = kFull ? 32 * NC : a.cache.head_dim, heads_kv = a.cache.kv_heads * ta.head_tiles;
 
   // ---- which chunk: all tiles in order, a sequence's shared out evenly over
   // its chunks; every wave counts them by itself
@@ -293,12 +300,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
     look(s0);
     total += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   }
-  int chunk = (int)(((uint32_t)total + (uint32_t)ta.units - 1) / (uint32_t)ta.units);
+  int chunk = ceil_div(total, ta.units, ta.inv_units);
+  chunk = (chunk + kWaves - 1) / kWaves * kWaves;  // a tile more for one wave costs what it costs for all
   chunk = chunk < ta.min_tiles ? ta.min_tiles : chunk;
+  const float inv_chunk = __builtin_amdgcn_rcpf((float)chunk);
   int seq = -1, at = 0, chunks = 0, slot = 0, lo = 0, hi = 0, before = 0, alone = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     if (a.seqs > 64) look(s0);
-    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? (int)(((uint32_t)(tiles + chunk) - 1) / (uint32_t)chunk) : 1;
+    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? ceil_div(tiles, chunk, inv_chunk) : 1;
     const int sum = wave_scan(c);
     const uint64_t who = __ballot(unit >= before + sum - c && unit < before + sum), ones = __ballot(c == 1);
     if (who) {
@@ -308,11 +317,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
       slot = before + __builtin_amdgcn_readlane(sum - c, w);
       at = unit - slot;
       slot -= alone + __builtin_popcountll(ones & ((1ull << w) - 1));  // sequences of one chunk need no slot
-      const int per = chunks == 1 ? __builtin_amdgcn_readlane(tiles, w)
-                                  : (int)((uint32_t)(__builtin_amdgcn_readlane(tiles, w) + chunks - 1) / (uint32_t)chunks);
+      const int per = ceil_div(__builtin_amdgcn_readlane(tiles, w), chunks, __builtin_amdgcn_rcpf((float)chunks));
       const int begin = __builtin_amdgcn_readlane(first, w), end = begin + __builtin_amdgcn_readlane(tokens, w);
       lo = begin + at * per * kTile;
-      hi = lo + per * kTile < end ? lo + per * kTile : end;
+      hi = at == chunks - 1 || lo + per * kTile > end ? end : lo + per * kTile;
       break;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -325,65 +333,61 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
 
   // ---- loads of a tile: its rows' offsets (lane i the i-th token's) through
   // LDS; K in the A operand's order, V in rows.  Dims past head_dim repeat dim
-  // 0 (their queries are zero, their outputs dropped).  A tile's page numbers
-  // are fetched two tiles ahead, its K when the products of the tile before
-  // have read theirs, its V likewise: the waits hide behind the other half.
+  // 0 (their queries are zero, their outputs dropped).  A tile's K is requested
+  // when the products of the tile before have read theirs, its V likewise: each
+  // wait hides behind the other half.
   const int32_t *table = a.table + (int64_t)seq * a.table_width;
   const uint8_t *kb = a.cache.k + (int64_t)kvh * a.cache.head_stride, *vb = a.cache.v + (int64_t)kvh * a.cache.head_stride;
   const int pt = a.cache.page_tokens, mine = lane & (kTile - 1);
   auto page_of = [&](int t) { return (int)(__umulhi(2u * (uint32_t)t, ta.page_mul) >> ta.page_shift); };
-  auto fetch_page = [&](int t0) { return t0 + mine < hi ? table[page_of(t0 + mine)] : -1; };
-  auto place = [&](int t0, int page, int buf) {  // the tile's offsets; a bit for each token that is not seen
-    const int t = t0 + mine;
-    const bool in = t < hi && (unsigned)page < (unsigned)a.cache.n_pages;
-    const int64_t off = page * a.cache.page_stride + (int64_t)(t - page_of(t) * pt) * a.cache.token_stride;
-    if (lane < kTile) offs[wave][buf][lane] = in ? off : 0;
+  auto place = [&](int t0, int end, int page0, int buf) {  // the tile's offsets; a bit for each token that is not seen
+    const int t = t0 + mine, page = page_of(t);
+    const int64_t base = t < end ? page_at[page - page0] : -1;
+    const bool in = base >= 0;
+    const uint32_t within = (uint32_t)(t - page * pt) * ta.token_stride;
+    if (lane < kTile) offs[wave][buf][lane] = in ? base + within : 0;
     wave_sync();
     return (uint32_t)__ballot(!in);  // lanes past kTile repeat
   };
   u32x4 kr[kSub][kQC], vr[kSlots][kVG];
   float dk[kSB], dv[kSB];  // Q8_0: scale of token slot n & 7, block 2 i + (n >> 3)
-  auto load_k = [&](int buf) {
-    if constexpr (kQ) {
-      const int64_t own = offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
+  auto scales = [&](const uint8_t *base, int buf, float (&d)[kSB]) {
+    const uint8_t *row = base + offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
 #pragma unroll
-      for (int i = 0; i < kSB; ++i) {
-        const int b = 2 * i + (n >> 3);
-        dk[i] = f16_bits_hw(load_any<uint16_t>(kb + own + (32 * b < D ? kQ8Bytes * b : 0)));
-      }
+    for (int i = 0; i < kSB; ++i) {
+      const bool there = kFull ? 2 * i + 1 < NC || n < 8 : 32 * (2 * i + (n >> 3)) < D;
+      d[i] = f16_bits_hw(load_any<uint16_t>(row + (there ? kQ8Bytes * (2 * i + (n >> 3)) : 0)));
     }
+  };
+  auto load_k = [&](int buf) {
+    if constexpr (kQ) scales(kb, buf, dk);
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       const uint8_t *row = kb + offs[wave][buf][16 * s + n];
+      if constexpr (kQ) row += 2 + 8 * g;
 #pragma unroll
       for (int c = 0; c < kQC; ++c) {
         if constexpr (kQ) {
-          const u32x2 v = load_any<u32x2>(row + (32 * c < D ? kQ8Bytes * c + 8 * g + 2 : 2));
+          const u32x2 v = load_any<u32x2>(row + (kFull || 32 * c < D ? kQ8Bytes * c : 0));
           kr[s][c] = u32x4{v[0], v[1], 0, 0};
         } else {
-          const int i = kF ? 16 * c + 4 * g : 32 * c + 8 * g;
-          kr[s][c] = *reinterpret_cast<const u32x4 *>(row + (i < D ? i * (kF ? 4 : 2) : 0));
+          const int i = 4 * kPer * c + kPer * g;
+          kr[s][c] = *reinterpret_cast<const u32x4 *>(row + (kFull || i < D ? i * (kF ? 4 : 2) : 0));
         }
       }
     }
   };
   auto load_v = [&](int buf) {
-    if constexpr (kQ) {
-      const int64_t own = offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
-#pragma unroll
-      for (int i = 0; i < kSB; ++i) {
-        const int b = 2 * i + (n >> 3);
-        dv[i] = f16_bits_hw(load_any<uint16_t>(vb + own + (32 * b < D ? kQ8Bytes * b : 0)));
-      }
-    }
+    if constexpr (kQ) scales(vb, buf, dv);
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       const uint8_t *row = vb + offs[wave][buf][16 * (j >> 2) + 4 * g + (j & 3)];
+      if constexpr (kQ) row += 2 + 2 * n;
 #pragma unroll
       for (int v = 0; v < kVG; ++v) {
-        const int i = 16 * kVD * v + kVD * n, ii = i < D ? i : 0;
+        const int i = 16 * kVD * v + kVD * n, ii = (kFull && 32 * NC % (16 * kVD) == 0) || i < D ? i : 0;
         if constexpr (kQ) {
-          vr[j][v] = u32x4{load_any<uint16_t>(row + (ii >> 5) * kQ8Bytes + 2 + (ii & 31)), 0, 0, 0};
+          vr[j][v] = u32x4{load_any<uint16_t>(row + (kFull || 32 * v < D ? kQ8Bytes * v : 0)), 0, 0, 0};
         } else if constexpr (kF || kVD == 8) {
           vr[j][v] = *reinterpret_cast<const u32x4 *>(row + ii * (kF ? 4 : 2));
         } else {
@@ -393,260 +397,273 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
       }
     }
   };
-  constexpr int kStep = kWaves * kTile;
-  int t0 = lo + wave * kTile, buf = 0;
-  int page = fetch_page(t0), page_next = fetch_page(t0 + kStep);
-  // the queries, requested before the first rows
-  constexpr int kPer = kF ? 4 : 8, kMy = (kQC + kWaves - 1) / kWaves;  // a lane's dims of a chunk, a wave's chunks
+
+  // ---- queries, requested before the first rows: the product's B operand,
+  // lane (head n, dims kPer g on of every chunk)
+  constexpr int kMy = kRegQ ? kQC : (kQC + kWaves - 1) / kWaves;  // a wave's chunks
   const float *q = a.q + (int64_t)seq * a.q_stride + (int64_t)h0 * D;
   float x[kMy][kPer];
 #pragma unroll
   for (int u = 0; u < kMy; ++u)
 #pragma unroll
     for (int j = 0; j < kPer; j += 4) {
-      const int i = 4 * kPer * (wave + u * kWaves) + kPer * g + j;
+      const int i = 4 * kPer * (kRegQ ? u : wave + u * kWaves) + kPer * g + j;
       f32x4 v = {0, 0, 0, 0};  // head_dim is a multiple of four
-      if (n < heads && i < D) v = load_any<f32x4>(reinterpret_cast<const uint8_t *>(q + (int64_t)n * D + i));
+      if (n < heads && i < D) v = load_any<f32x4>(q + (int64_t)n * D + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[u][j + e] = v[e];
     }
-  uint32_t hidden = 0;
-  if (t0 < hi) {
-    hidden = place(t0, page, 0);
-    load_k(0);
-    load_v(0);
-  }
+  u32x4 ql[kRegQ ? kQC : 1][kL];
+  auto query = [&](int c, int k) { return kRegQ ? ql[c][k] : q_lds[(c * kL + k) * 64 + lane]; };
+  float to_log2 = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;  // of this lane's head
 
-  // ---- queries into LDS, as the product's B operand
-  float s_scale = a.scale;  // of this lane's head
-  if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
-#pragma unroll
-    for (int u = 0; u < kMy; ++u) {
-      float mx = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, fabsf(x[u][j]));
-      mx = cross_max(mx);
-      if (g == 0 && wave + u * kWaves < kQC) q_max[wave + u * kWaves][n] = mx;
-    }
-    __syncthreads();
-    float mx = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kQC; ++c) mx = fmaxf(mx, q_max[c][n]);
-    const int e = mx > 0.0f && mx < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(mx) : 0;
-    s_scale = ldexpf(s_scale, -e);
-#pragma unroll
-    for (int u = 0; u < kMy; ++u)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) x[u][j] = ldexpf(x[u][j], e);
-  }
-#pragma unroll
-  for (int u = 0; u < kMy; ++u) {
-    const int c = wave + u * kWaves;
-    if (c >= kQC) break;
-    if constexpr (kF) {
-      q_lds[c * 64 + lane] = u32x4{as_u32(x[u][0]), as_u32(x[u][1]), as_u32(x[u][2]), as_u32(x[u][3])};
-    } else {
-      u32x4 limb[kL];
-      if constexpr (kType == kBF16) limbs_bf16(x[u], limb);
-      else limbs_f16(x[u], limb);
-#pragma unroll
-      for (int k = 0; k < kL; ++k) q_lds[(c * kL + k) * 64 + lane] = limb[k];
-    }
-  }
-  __syncthreads();
-
-  // ---- the chunk's tiles
-  const float to_log2 = a.softcap > 0.0f ? s_scale : s_scale * kLog2e;
   f32x4 o[kVG * kVD];
 #pragma unroll
   for (int t = 0; t < kVG * kVD; ++t) o[t] = f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
   int d_exp = -100;  // Q8_0: O is scaled so that scales of up to 2^d_exp keep P's limbs in range
-  while (t0 < hi) {
-    const bool more = t0 + kStep < hi;
-    uint32_t hidden_next = 0;
-    if (more) {
-      page = page_next;
-      page_next = fetch_page(t0 + 2 * kStep);
-      hidden_next = place(t0 + kStep, page, buf ^ 1);
+  for (int seg = lo; seg < hi; seg += ta.segment) {
+    const int end = hi - seg < ta.segment ? hi : seg + ta.segment;
+    const int page0 = page_of(seg), pages = page_of(end - 1) - page0 + 1;
+    if (seg > lo) __syncthreads();
+    for (int i = tid; i < pages; i += kThreads) {
+      const int page = table[page0 + i];
+      page_at[i] = (unsigned)page < (unsigned)a.cache.n_pages ? page * a.cache.page_stride : -1;
     }
-    // scores
-    float p[kSlots];
-    if constexpr (kQ) {  // a block's products, times its keys' scales
+    __syncthreads();
+    int t0 = seg + wave * kTile, buf = 0;
+    uint32_t hidden = 0;
+    if (t0 < end) {
+      hidden = place(t0, end, page0, 0);
+      load_k(0);
+      load_v(0);
+    }
+    if (seg == lo) {
+      // not before the first rows are requested
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) p[j] = 0.0f;
+      for (int u = 0; u < kMy; ++u)
 #pragma unroll
-      for (int c = 0; c < kQC; ++c) {
-        float b[8];
-        u32x4 qq[kL];
+        for (int j = 0; j < kPer; ++j) asm volatile("" : "+v"(x[u][j]));
+      if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
+        float mx = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kL; ++k) qq[k] = q_lds[(c * kL + k) * 64 + lane];
+        for (int u = 0; u < kMy; ++u)
 #pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          u32x4 op;
+          for (int j = 0; j < kPer; ++j) mx = __builtin_fmaxf(mx, __builtin_fabsf(x[u][j]));
+        mx = cross_max(mx);
+        if constexpr (!kRegQ) {
+          if (g == 0) m_lds[wave][n] = mx;
+          __syncthreads();
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            op[2 * w] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c010c00u));
-            op[2 * w + 1] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c030c02u));
-          }
-          f32x4 t = {0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < kL; ++k) t = mfma<kType>(op, qq[k], t);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b[4 * s + i] = t[i];
+          for (int w = 0; w < kWaves; ++w) mx = __builtin_fmaxf(mx, m_lds[w][n]);
         }
-        float y[8];
-        scale_slots(b, dk[c >> 1], c & 1, y);
+        const int e = mx > 0.0f && mx < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        to_log2 = ldexpf(to_log2, -e);
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j) p[j] += y[j];
+        for (int u = 0; u < kMy; ++u)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) x[u][j] = ldexpf(x[u][j], e);
       }
-    } else {
-      constexpr int kAcc = kF ? 4 : kL;  // one sum a limb, or a quarter of the dims: products that do not wait for each other
-      f32x4 part[kSub][kAcc];
 #pragma unroll
-      for (int s = 0; s < kSub; ++s)
+      for (int u = 0; u < kMy; ++u) {
+        u32x4 limb[kL];
+        if constexpr (kF) limb[0] = u32x4{as_u32(x[u][0]), as_u32(x[u][1]), as_u32(x[u][2]), as_u32(x[u][3])};
+        else if constexpr (kType == kBF16) limbs_bf16(x[u], limb);
+        else limbs_f16(x[u], limb);
 #pragma unroll
-        for (int k = 0; k < kAcc; ++k) part[s][k] = f32x4{0, 0, 0, 0};
+        for (int k = 0; k < kL; ++k) {
+          if constexpr (kRegQ) ql[u][k] = limb[k];
+          else if (wave + u * kWaves < kQC) q_lds[((wave + u * kWaves) * kL + k) * 64 + lane] = limb[k];
+        }
+      }
+      if constexpr (!kRegQ) __syncthreads();
+    }
+    while (t0 < end) {
+      const bool more = t0 + kStep < end;
+      uint32_t hidden_next = 0;
+      if (more) hidden_next = place(t0 + kStep, end, page0, buf ^ 1);
+      // scores
+      float p[kSlots];
+      if constexpr (kQ) {  // a block's products, times its keys' scales
 #pragma unroll
-      for (int c = 0; c < kQC; ++c)
+        for (int j = 0; j < kSlots; ++j) p[j] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kQLimbs; ++k) {
-          const u32x4 qq = q_lds[(c * kQLimbs + k) * 64 + lane];
+        for (int c = 0; c < kQC; ++c) {
+          float b[8];
 #pragma unroll
           for (int s = 0; s < kSub; ++s) {
-            if constexpr (kF) {
+            u32x4 op;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) part[s][e] = mfma4(as_f32(kr[s][c][e]), as_f32(qq[e]), part[s][e]);
-            } else {
-              part[s][k] = mfma<kType>(kr[s][c], qq, part[s][k]);
+            for (int w = 0; w < 2; ++w) {
+              op[2 * w] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c010c00u));
+              op[2 * w + 1] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c030c02u));
+            }
+            f32x4 t = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < kL; ++k) t = mfma<kType>(op, query(c, k), t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[4 * s + i] = t[i];
+          }
+          float y[8];
+          scale_slots(b, dk[c >> 1], c & 1, y);
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) p[j] += y[j];
+        }
+      } else {
+        constexpr int kAcc = kF ? 4 : kL;  // one sum a limb, or a quarter of the dims: products that do not wait for each other
+        f32x4 part[kSub][kAcc];
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+          for (int k = 0; k < kAcc; ++k) part[s][k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kQC; ++c)
+#pragma unroll
+          for (int k = 0; k < kL; ++k) {
+            const u32x4 qq = query(c, k);
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) {
+              if constexpr (kF) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[s][e] = mfma4(as_f32(kr[s][c][e]), as_f32(qq[e]), part[s][e]);
+              } else {
+                part[s][k] = mfma<kType>(kr[s][c], qq, part[s][k]);
+              }
             }
           }
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) {
+          f32x4 acc = part[s][kAcc - 1];
+#pragma unroll
+          for (int k = kAcc - 2; k >= 0; --k) acc += part[s][k];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i];
         }
-#pragma unroll
-      for (int s = 0; s < kSub; ++s) {
-        f32x4 acc = part[s][kAcc - 1];
-#pragma unroll
-        for (int k = kAcc - 2; k >= 0; --k) acc += part[s][k];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i];
       }
-    }
-    if (more) load_k(buf ^ 1);
+      if (more) load_k(buf ^ 1);
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
-    if (a.softcap > 0.0f) {
+      for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
+      if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) p[j] = a.softcap * tanhf(p[j] / a.softcap) * kLog2e;
-    }
-    if (hidden) {  // no weight, and values that are zero whatever the memory holds
-      const uint32_t own = hidden >> (4 * g);
+        for (int j = 0; j < kSlots; ++j) p[j] = a.softcap * tanhf(p[j] / a.softcap) * kLog2e;
+      }
+      if (hidden) {  // no weight, and values that are zero whatever the memory holds
+        const uint32_t own = hidden >> (4 * g);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+          const bool out = own >> (16 * (j >> 2) + (j & 3)) & 1u;
+          p[j] = out ? -INFINITY : p[j];
+#pragma unroll
+          for (int v = 0; v < kVG; ++v)
+            if constexpr (!kQ) vr[j][v] = out ? u32x4{0, 0, 0, 0} : vr[j][v];
+        }
+        if constexpr (kQ) {
+          const bool out = own >> (16 * ((n & 7) >> 2) + (n & 3)) & 1u;
+#pragma unroll
+          for (int i = 0; i < kSB; ++i) dv[i] = out ? 0.0f : dv[i];
+        }
+      }
+      float top = p[0];
+#pragma unroll
+      for (int j = 1; j < kSlots; ++j) top = __builtin_fmaxf(top, p[j]);
+      top = cross_max(top);
+      bool grown = __ballot(top > m + kGrowth) != 0;
+      int d_new = d_exp;
+      if constexpr (kQ) {
+        // the largest scale of the tile against what O's scaling allows for
+        float dm = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSB; ++i) dm = __builtin_fmaxf(dm, __builtin_fabsf(dv[i]));
+        const int de = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) : -100;
+        if (__ballot(de > d_exp) != 0) {
+          int w = de;
+          for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_xor(w, d);
+            w = y > w ? y : w;
+          }
+          d_new = __builtin_amdgcn_readfirstlane(w);
+          grown = true;
+        }
+      }
+      if (grown) {
+        top = __builtin_fmaxf(m, top);
+        float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        m = top;
+        l *= f;
+        if constexpr (kQ) f = ldexpf(f, d_exp - d_new);
+        d_exp = d_new;
+#pragma unroll
+        for (int t = 0; t < kVG * kVD; ++t) o[t] *= f;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
-        const bool out = own >> (16 * (j >> 2) + (j & 3)) & 1u;
-        p[j] = out ? -INFINITY : p[j];
+        p[j] = __builtin_amdgcn_exp2f(p[j] - base);
+        l += p[j];
+      }
+      // outputs
+      if constexpr (kF) {
 #pragma unroll
         for (int v = 0; v < kVG; ++v)
-          if constexpr (!kQ) vr[j][v] = out ? u32x4{0, 0, 0, 0} : vr[j][v];
-      }
-      if constexpr (kQ) {
-        const bool out = own >> (16 * ((n & 7) >> 2) + (n & 3)) & 1u;
-#pragma unroll
-        for (int i = 0; i < kSB; ++i) dv[i] = out ? 0.0f : dv[i];
-      }
-    }
-    float top = p[0];
-#pragma unroll
-    for (int j = 1; j < kSlots; ++j) top = fmaxf(top, p[j]);
-    top = fmaxf(m, cross_max(top));
-    float keep = 1.0f;
-    bool grown = __ballot(top > m) != 0;
-    if (grown) keep = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-    int d_new = d_exp;
-    if constexpr (kQ) {
-      // the largest scale of the tile against what O's scaling allows for
-      float dm = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSB; ++i) dm = fmaxf(dm, fabsf(dv[i]));
-      const int de = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) : -100;
-      if (__ballot(de > d_exp) != 0) {
-        int w = de;
-        for (int d = 1; d < 64; d *= 2) {
-          const int y = __shfl_xor(w, d);
-          w = y > w ? y : w;
-        }
-        d_new = __builtin_amdgcn_readfirstlane(w);
-        grown = true;
-      }
-    }
-    if (grown) {
-      l *= keep;
-      float f = keep;
-      if constexpr (kQ) f = ldexpf(keep, d_exp - d_new);
-      d_exp = d_new;
-#pragma unroll
-      for (int t = 0; t < kVG * kVD; ++t) o[t] *= f;
-    }
-    m = top;
-    const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(p[j] - base);
-      l += p[j];
-    }
-    // outputs
-    if constexpr (kF) {
-#pragma unroll
-      for (int v = 0; v < kVG; ++v)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[4 * v + e] = mfma4(as_f32(vr[j][v][e]), p[j], o[4 * v + e]);
-    } else if constexpr (kQ) {
-      const float up = ldexpf(1.0f, 14 - d_exp);
-#pragma unroll
-      for (int j = 0; j < kSlots; ++j) p[j] *= up;
-#pragma unroll
-      for (int v = 0; v < kVG; ++v) {  // block v
-        float y[8];
-        scale_slots(p, dv[v >> 1], v & 1, y);
-        u32x4 limb[kL];
-        limbs_f16(y, limb);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          u32x4 op;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            op[j] = codes_f16(__builtin_amdgcn_perm(vr[2 * j + 1][v][0], vr[2 * j][v][0], d ? 0x0c050c01u : 0x0c040c00u));
 #pragma unroll
-          for (int k = 0; k < kL; ++k) o[2 * v + d] = mfma<kType>(op, limb[k], o[2 * v + d]);
+            for (int e = 0; e < 4; ++e) o[4 * v + e] = mfma4(as_f32(vr[j][v][e]), p[j], o[4 * v + e]);
+      } else if constexpr (kQ) {
+        const float up = ldexpf(1.0f, 6 - d_exp);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) p[j] *= up;
+#pragma unroll
+        for (int v = 0; v < kVG; ++v) {  // block v
+          float y[8];
+          scale_slots(p, dv[v >> 1], v & 1, y);
+          u32x4 limb[kL];
+          limbs_f16(y, limb);
+          u32x4 op[2];
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              op[d][j] = codes_f16(__builtin_amdgcn_perm(vr[2 * j + 1][v][0], vr[2 * j][v][0], d ? 0x0c050c01u : 0x0c040c00u));
+#pragma unroll
+          for (int k = 0; k < kL; ++k)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) o[2 * v + d] = mfma<kType>(op[d], limb[k], o[2 * v + d]);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
-    } else {
-      u32x4 limb[kL];
-      if constexpr (kType == kBF16) {
-        limbs_bf16(p, limb);
       } else {
+        u32x4 limb[kL];
+        if constexpr (kType == kBF16) {
+          limbs_bf16(p, limb);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] *= 16384.0f;
-        limbs_f16(p, limb);
-      }
-#pragma unroll
-      for (int v = 0; v < kVG; ++v)
-#pragma unroll
-        for (int d = 0; d < kVD; ++d) {
-          u32x4 op;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            op[j] = d & 1 ? hi16s(vr[2 * j][v][d / 2], vr[2 * j + 1][v][d / 2])
-                          : lo16s(vr[2 * j][v][d / 2], vr[2 * j + 1][v][d / 2]);
-#pragma unroll
-          for (int k = 0; k < kL; ++k) o[v * kVD + d] = mfma<kType>(op, limb[k], o[v * kVD + d]);
+          for (int j = 0; j < 8; ++j) p[j] *= 64.0f;
+          limbs_f16(p, limb);
         }
+#pragma unroll
+        for (int v = 0; v < kVG; ++v)
+#pragma unroll
+          for (int d0 = 0; d0 < kVD; d0 += 4) {
+            u32x4 op[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t lower = vr[2 * j][v][(d0 + d) / 2], upper = vr[2 * j + 1][v][(d0 + d) / 2];
+                op[d][j] = d & 1 ? hi16s(lower, upper) : lo16s(lower, upper);
+              }
+#pragma unroll
+            for (int k = 0; k < kL; ++k)
+#pragma unroll
+              for (int d = 0; d < 4; ++d) o[v * kVD + d0 + d] = mfma<kType>(op[d], limb[k], o[v * kVD + d0 + d]);
+          }
+      }
+      if (!more) break;
+      buf ^= 1;
+      load_v(buf);
+      hidden = hidden_next;
+      t0 += kStep;
     }
-    buf ^= 1;
-    if (more) load_v(buf);
-    hidden = hidden_next;
-    t0 += kStep;
   }
 
   // ---- the waves' results into one
@@ -655,79 +672,76 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
     m_lds[wave][n] = m;
     l_lds[wave][n] = l;
   }
-  __syncthreads();
-  float M = -INFINITY, L = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m_lds[w][n]);
-  const float M0 = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) L += l_lds[w][n] * __builtin_amdgcn_exp2f(m_lds[w][n] - M0);
-  float f = __builtin_amdgcn_exp2f(m - M0);
-  if constexpr (kQ) f = ldexpf(f, d_exp - 14);
-  else if constexpr (kType == kF16) f *= 1.0f / 16384.0f;
+  float f = 1.0f;
+  if constexpr (kQ) f = ldexpf(1.0f, d_exp - 6);
+  else if constexpr (kType == kF16) f = 1.0f / 64.0f;
   const int DS = D + 4, fit = kMergeFloats / (kWaves * DS);  // heads that fit at once
-  const int slot_floats = (a.group < kHeads ? a.group : kHeads) * (D + 2);
-  float *part = ta.part + ((int64_t)(slot + at) * heads_kv + head_at) * slot_floats;
+  const int slot_floats = ((a.group < kHeads ? a.group : kHeads) * (D + 2) + 3) / 4 * 4;
+  const auto part = __builtin_amdgcn_make_buffer_rsrc(ta.part, 0, (int)ta.part_bytes, 0x00020000);
+  const uint32_t origin = 4u * ((uint32_t)slot * heads_kv + head_at) * slot_floats, step = 4u * heads_kv * slot_floats;
   float *out = a.out + (int64_t)seq * a.out_stride + (int64_t)h0 * D;
-  __syncthreads();
-  if (wave == 0 && g == 0) {
-    m_lds[0][n] = M;
-    l_lds[0][n] = L;
-  }
+  float *lse = a.lse ? a.lse + (int64_t)seq * a.q_heads + h0 : nullptr;
+  constexpr int kRows = kThreads / kQuads;  // rows of outputs that the threads hold at once
+  const int row = tid / kQuads, quad = tid % kQuads;
+  auto finish = [&](int h, f32x4 v, float top, float sum) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] / sum;
+    __builtin_memcpy(out + h * D + 4 * quad, &v, sizeof v);
+    if (lse && quad == 0) lse[h] = top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  };
   for (int p0 = 0; p0 < heads; p0 += fit) {
     const int count = heads - p0 < fit ? heads - p0 : fit;
+    if (p0 > 0) __syncthreads();
     if (n >= p0 && n < p0 + count) {
-      float *row = merge + (wave * fit + n - p0) * DS;
+      float *to = merge + (wave * fit + n - p0) * DS;
 #pragma unroll
       for (int v = 0; v < kVG; ++v)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int dim = 16 * kVD * v + kVD * (4 * g + i);
           if constexpr (kVD == 2) {
-            if (dim >= D) continue;
-            row[dim] = o[v * kVD][i] * f;
-            row[dim + 1] = o[v * kVD + 1][i] * f;
+            if (!kFull && dim >= D) continue;
+            to[dim] = o[v * kVD][i] * f;
+            to[dim + 1] = o[v * kVD + 1][i] * f;
           } else {
 #pragma unroll
             for (int d = 0; d < kVD; d += 4)
-              if (dim + d < D)
-                *reinterpret_cast<f32x4 *>(row + dim + d) = f32x4{o[v * kVD + d][i], o[v * kVD + d + 1][i],
-                                                                  o[v * kVD + d + 2][i], o[v * kVD + d + 3][i]} * f;
+              if ((kFull && 32 * NC % (16 * kVD) == 0) || dim + d < D)
+                *reinterpret_cast<f32x4 *>(to + dim + d) = f32x4{o[v * kVD + d][i], o[v * kVD + d + 1][i],
+                                                                 o[v * kVD + d + 2][i], o[v * kVD + d + 3][i]} * f;
           }
         }
     }
     __syncthreads();
-    const int dq = D / 4;
-    for (int e = tid; e < count * dq; e += 64 * kWaves) {
-      const int h = (int)((unsigned)e / (unsigned)dq), dim = 4 * (e - h * dq);
+    for (int h = p0 + row; h < p0 + count; h += kRows) {
+      if (4 * quad >= D) break;
+      float top = m_lds[0][h], sum = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, m_lds[w][h]);
+      const float base = top == -INFINITY ? 0.0f : top;
       f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(merge + (w * fit + h) * DS + dim);
-      const float sum = l_lds[0][p0 + h];
-      float *to = (chunks > 1 ? part : out) + (p0 + h) * D + dim;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (chunks > 1) put(to + i, v[i]);
-        else to[i] = sum == 0.0f ? 0.0f : v[i] / sum;
+      for (int w = 0; w < kWaves; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(m_lds[w][h] - base);
+        sum += weight * l_lds[w][h];
+        v += weight * *reinterpret_cast<const f32x4 *>(merge + (w * fit + h - p0) * DS + 4 * quad);
+      }
+      if (chunks == 1) {
+        finish(h, v, top, sum);
+      } else {
+        const uint32_t mine_at = origin + (uint32_t)at * step;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, mine_at + 4 * (h * D + 4 * quad), 0, kAgent);
+        if (quad == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(as_u32(top), part, mine_at + 4 * (heads * D + h), 0, kAgent);
+          __builtin_amdgcn_raw_buffer_store_b32(as_u32(sum), part, mine_at + 4 * (heads * D + heads + h), 0, kAgent);
+        }
       }
     }
-    __syncthreads();
   }
-  if (chunks == 1) {
-    if (a.lse && tid < heads) {
-      const float top = m_lds[0][tid];
-      a.lse[(int64_t)seq * a.q_heads + h0 + tid] =
-          top == -INFINITY ? top : (top + __builtin_amdgcn_logf(l_lds[0][tid])) * kLn2;
-    }
-    return;
-  }
+  if (chunks == 1) return;
 
   // ---- the chunks' results into one, by the workgroup that finishes last, in
   // the chunks' order
-  if (tid < heads) {
-    put(part + heads * D + tid, m_lds[0][tid]);
-    put(part + heads * D + heads + tid, l_lds[0][tid]);
-  }
   results_stored();
   __syncthreads();
   uint32_t *arrived = ta.arrived + (int64_t)slot * heads_kv + head_at;
@@ -736,36 +750,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
   __syncthreads();
   if (!last) return;
   if (tid == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Teams of threads take every teams-th chunk, a thread four outputs of one
-  // head, with a running maximum and sum of their own; the teams then meet in LDS.
-  const float *origin = ta.part + ((int64_t)slot * heads_kv + head_at) * slot_floats;
-  const int64_t step = (int64_t)heads_kv * slot_floats;
-  const int quads = heads * D / 4, teams = 64 * kWaves / quads > 1 ? 64 * kWaves / quads : 1;
-  const int rounds = (quads + 64 * kWaves - 1) / (64 * kWaves);  // 1 where there are teams
-  for (int r = 0; r < rounds; ++r) {
-    const int team = teams > 1 ? (int)((unsigned)tid / (unsigned)quads) : 0;
-    const int quad = teams > 1 ? tid - team * quads : tid + r * 64 * kWaves;
-    const bool in = quad < quads && team < teams;
-    const int h = in ? (int)((unsigned)(4 * quad) / (unsigned)D) : 0;
+  // Where the rows are fewer than the threads hold, teams of rows take every
+  // teams-th chunk, with a running maximum and sum of their own, and meet in LDS.
+  const int teams = heads >= kRows ? 1 : kRows / heads, team = heads >= kRows ? 0 : row * (256 / heads + 1) >> 8;
+  for (int h = row - team * heads; h < heads; h += kRows) {
     f32x4 v = {0, 0, 0, 0};
     float top = -INFINITY, sum = 0.0f;
-    constexpr int kAtOnce = 8;
-    for (int i0 = in ? team : chunks; i0 < chunks; i0 += kAtOnce * teams) {
+    constexpr int kAtOnce = 4;
+    for (int i0 = team; i0 < chunks && team < teams && 4 * quad < D; i0 += kAtOnce * teams) {
       float mi[kAtOnce], li[kAtOnce];
       f32x4 vi[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         const int i = i0 + u * teams;
-        const float *from = origin + (i < chunks ? i : i0) * step;
-        mi[u] = get(from + heads * D + h);
-        li[u] = get(from + heads * D + heads + h);
-        vi[u] = get4(from + 4 * quad);
+        const uint32_t from = origin + (uint32_t)(i < chunks ? i : i0) * step;
+        mi[u] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(part, from + 4 * (heads * D + h), 0, kAgent));
+        li[u] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(part, from + 4 * (heads * D + heads + h), 0, kAgent));
+        vi[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, from + 4 * (h * D + 4 * quad), 0, kAgent));
       }
       float most = top;
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        if (i0 + u * teams >= chunks) mi[u] = -INFINITY;
-        most = fmaxf(most, mi[u]);
+        if (i0 + u * teams >= chunks) mi[u] = -INFINITY, li[u] = 0.0f, vi[u] = f32x4{0, 0, 0, 0};
+        most = __builtin_fmaxf(most, mi[u]);
       }
       const float base = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(top - base);
       v *= keep;
@@ -773,48 +780,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_tiles_kernel(TileArg
       top = most;
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        if (i0 + u * teams >= chunks) continue;
         const float w = __builtin_amdgcn_exp2f(mi[u] - base);
         sum += w * li[u];
         v += w * vi[u];
       }
     }
-    if (teams > 1) {
+    if (teams > 1) {  // every row here once
+      f32x4 *joined = reinterpret_cast<f32x4 *>(merge);
       joined[tid] = v;
-      merge[2 * tid] = top;
-      merge[2 * tid + 1] = sum;
+      merge[4 * kThreads + 2 * tid] = top;
+      merge[4 * kThreads + 2 * tid + 1] = sum;
       __syncthreads();
       if (team > 0) return;
       float most = top;
-      for (int t = 1; t < teams; ++t) most = fmaxf(most, merge[2 * (t * quads + quad)]);
+      for (int t = 1; t < teams; ++t) most = __builtin_fmaxf(most, merge[4 * kThreads + 2 * (tid + t * heads * kQuads)]);
       const float base = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(top - base);
       v *= keep;
       sum *= keep;
       for (int t = 1; t < teams; ++t) {
-        const int from = t * quads + quad;
-        const float w = __builtin_amdgcn_exp2f(merge[2 * from] - base);
-        sum += w * merge[2 * from + 1];
+        const int from = tid + t * heads * kQuads;
+        const float w = __builtin_amdgcn_exp2f(merge[4 * kThreads + 2 * from] - base);
+        sum += w * merge[4 * kThreads + 2 * from + 1];
         v += w * joined[from];
       }
       top = most;
     }
-    if (!in) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[4 * quad + i] = sum == 0.0f ? 0.0f : v[i] / sum;
-    if (a.lse && 4 * quad == h * D)
-      a.lse[(int64_t)seq * a.q_heads + h0 + h] = top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (team == 0 && 4 * quad < D) finish(h, v, top, sum);
   }
 }
 
 namespace {
 
+template <int kType, int NC>
+void launch_tiles(const TileArgs &ta, dim3 grid, hipStream_t s) {
+  if (ta.a.cache.head_dim == 32 * NC) launch_timed(attention_tiles_kernel<kType, NC, true>, grid, dim3(kThreads), 0u, s, ta);
+  else launch_timed(attention_tiles_kernel<kType, NC, false>, grid, dim3(kThreads), 0u, s, ta);
+}
 template <int kType>
 void launch_tiles(const TileArgs &ta, dim3 grid, hipStream_t s) {
   const int D = ta.a.cache.head_dim;
-  if (D <= 64) launch_timed(attention_tiles_kernel<kType, 2>, grid, dim3(64 * kWaves), 0u, s, ta);
-  else if (D <= 96) launch_timed(attention_tiles_kernel<kType, 3>, grid, dim3(64 * kWaves), 0u, s, ta);
-  else if (D <= 128) launch_timed(attention_tiles_kernel<kType, 4>, grid, dim3(64 * kWaves), 0u, s, ta);
-  else launch_timed(attention_tiles_kernel<kType, 8>, grid, dim3(64 * kWaves), 0u, s, ta);
+  if (D <= 64) launch_tiles<kType, 2>(ta, grid, s);
+  else if (D <= 96) launch_tiles<kType, 3>(ta, grid, s);
+  else if (D <= 128) launch_tiles<kType, 4>(ta, grid, s);
+  else launch_tiles<kType, 8>(ta, grid, s);
 }
 
 }  // namespace
@@ -824,18 +832,24 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   const KvPages &c = a.cache;
   const uint64_t strides = (uint64_t)(c.page_stride | c.head_stride | c.token_stride);
   const bool aligned = ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | strides) & 15u) == 0;
-  p.tiles = c.head_dim <= 256 && (c.type == kQ8_0 || (aligned && c.head_dim % (c.type == kF32 ? 4 : 8) == 0));
+  const uint64_t page = (uint64_t)c.token_stride * (uint64_t)c.page_tokens;  // 32-bit offsets within a page
+  p.tiles = c.head_dim <= 256 && c.token_stride < (1ll << 32) && page < (1ull << 32) &&
+            (c.type == kQ8_0 || (aligned && c.head_dim % (c.type == kF32 ? 4 : 8) == 0));
   if (!p.tiles) return p;
   const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
-  const int64_t aim = 2 * (int64_t)cu_count;  // workgroups that run at once
+  const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;  // workgroups that run at once
   p.min_tiles = kWaves;
-  p.units = (int)std::max<int64_t>(1, aim / pairs);
+  // All chunks (units + seqs a head at most) at once where the sequences leave
+  // room for that; where they do not, twice as many, for an even end.
+  const int64_t units = aim / pairs;
+  p.units = (int)std::max<int64_t>(1, a.seqs <= units / 2 ? units - a.seqs : 2 * units);
   const int64_t chunks = std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles);
-  p.grid = std::min<int64_t>(a.seqs + (chunks > 1 ? p.units : 0), a.seqs * chunks);
-  if (chunks > 1) {
-    p.arrived_bytes = (size_t)(2 * p.units * pairs) * sizeof(uint32_t);
-    p.part_bytes = (size_t)(2 * p.units * pairs) * (size_t)(std::min(a.group, kHeads) * (c.head_dim + 2)) * sizeof(float);
+  const bool splits = chunks > 1 && p.units > 1;  // one unit: every sequence is one chunk
+  p.grid = splits ? std::min<int64_t>(a.seqs + p.units + 1, a.seqs * chunks) : a.seqs;
+  if (splits) {
+    p.arrived_bytes = (size_t)(2 * (p.units + 1) * pairs) * sizeof(uint32_t);
+    p.part_bytes = (size_t)(2 * (p.units + 1) * pairs) * (size_t)((std::min(a.group, kHeads) * (c.head_dim + 2) + 3) / 4 * 4) * sizeof(float);
   }
   return p;
 }
@@ -850,8 +864,20 @@ hipError_t launch_attention(const AttnArgs &a, const AttnPlan &p, void *part, vo
   const uint32_t d = (uint32_t)a.cache.page_tokens;
   uint32_t n = 0;
   while (((uint64_t)1 << n) < d) ++n;
-  TileArgs ta{a, (uint32_t)(((uint64_t)1 << (31 + n)) / d + 1), n, (a.group + kHeads - 1) / kHeads, p.units, p.min_tiles,
-              static_cast<float *>(part), static_cast<uint32_t *>(arrived)};
+  const int tile = a.cache.type == kF32 ? 16 : 32, step = kWaves * tile;
+  TileArgs ta{};
+  ta.a = a;
+  ta.page_mul = (uint32_t)(((uint64_t)1 << (31 + n)) / d + 1);
+  ta.page_shift = n;
+  ta.token_stride = (uint32_t)a.cache.token_stride;
+  ta.head_tiles = (a.group + kHeads - 1) / kHeads;
+  ta.units = p.units;
+  ta.inv_units = 1.0f / (float)p.units;
+  ta.min_tiles = p.min_tiles;
+  ta.segment = (int)(std::min<int64_t>((int64_t)(kPages - 2) * d, 1 << 30) / step * step);
+  ta.part_bytes = (uint32_t)p.part_bytes;
+  ta.part = static_cast<float *>(part);
+  ta.arrived = static_cast<uint32_t *>(arrived);
   const unsigned y = (unsigned)std::min<int64_t>(p.grid, kGridY);
   const dim3 grid((unsigned)(a.cache.kv_heads * ta.head_tiles), y, (unsigned)((p.grid + y - 1) / y));
   if (a.cache.type == kF32) launch_tiles<kF32>(ta, grid, s);
