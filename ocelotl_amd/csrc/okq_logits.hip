@@ -13,12 +13,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kVB = 4, kVH = 4;
-constexpr int kAhead = 8;  // history entries that a thread requests before it needs them
-// A token's word: its count in the answer so far, or kPrompt where only the
-// prompt holds it; kBiased where a bias is listed.
-constexpr uint32_t kBiased = 0x80000000u, kPrompt = 0x40000000u, kCount = 0x3fffffffu;
+constexpr int kThreads = 1024;
+constexpr int kAhead = 4;  // history entries that a thread requests before it needs them
+// A token's word: how often the answer so far holds it, kPrompt if the prompt
+// does, kBiased if a bias is listed, and (for lists of at most kThreads) the
+// bias's place in its list, which leaves the count kShortBits bits.
+constexpr uint32_t kBiased = 0x80000000u, kPrompt = 0x40000000u;
+constexpr int kShortBits = 20;
+static_assert(kThreads <= 1 << (30 - kShortBits), "a place fits beside the count");
 
 // A result's place in the order of results: larger values first, then lower
 // indexes; all ones is for NaN, before everything.  Zeros of both signs are
@@ -32,15 +34,12 @@ __device__ __forceinline__ int32_t best_of(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return o == 0xffffffffu || o <= 0x007fffffu ? -1 : (int32_t)(0xffffffffu - (uint32_t)key);
 }
-template <class T>
-__device__ __forceinline__ T load_any(const void *p) {  // any alignment
-  T v;
-  __builtin_memcpy(&v, p, sizeof v);
-  return v;
+// Any alignment; past the caches, where nothing of a row is read twice.
+typedef f32x4 f32x4_4 __attribute__((aligned(4)));
+__device__ __forceinline__ f32x4 load_past(const float *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const f32x4_4 *>(p));
 }
-// Any alignment, and past the caches, which the logits of the rows to come fill.
 __device__ __forceinline__ void store_past(float *p, f32x4 v) {
-  typedef f32x4 f32x4_4 __attribute__((aligned(4)));
   __builtin_nontemporal_store(v, reinterpret_cast<f32x4_4 *>(p));
 }
 __device__ __forceinline__ uint64_t wave_max(uint64_t k) {
@@ -51,9 +50,25 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t k) {
   return k;
 }
 
+// A slice's best key joins its row's; the last slice's workgroup names the
+// token.  Atomics of agent scope; the wait between them is the order that the
+// last one relies on.  Both words are zero again afterwards.
+__device__ __forceinline__ void choose(const LogitsArgs &a, int row, int slices, uint64_t best, uint64_t *keys,
+                                       uint32_t *arrived) {
+  if (slices > 1) {
+    __hip_atomic_fetch_max(&keys[row], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (__hip_atomic_fetch_add(&arrived[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (uint32_t)slices - 1)
+      return;
+    best = __hip_atomic_exchange(&keys[row], (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&arrived[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  a.best[row] = best_of(best);
+}
+
 }  // namespace
 
-// A workgroup per row and slice of 2048 V entries of the vocabulary, four
+// A workgroup per row and slice of 4096 V entries of the vocabulary, four
 // consecutive ones a thread and step.  The slice's logits are requested first;
 // while they come, the row's whole history and bias list are read (they stay
 // in the caches for the row's other slices) and what falls into the slice is
@@ -61,14 +76,16 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t k) {
 // biases by the thread that holds a token's first entry, in list order.  The
 // workgroup that ends last on a row turns the largest key into the token.
 // Memory bounds it: the logits are read and written once.
-template <int V, bool kMarks, bool kBias>  // a history; biases (with marks)
+template <int V, bool kMarks, int kBias>  // a history; biases (with marks): 1 a list of kThreads at most, 2 a longer one
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slices, uint64_t *keys, uint32_t *arrived) {
   constexpr int kSlice = 4 * kThreads * V, kWaves = kThreads / 64;
+  constexpr uint32_t kCount = kBias == 1 ? (1u << kShortBits) - 1 : 0x3fffffffu;
   __shared__ uint32_t marks[kMarks ? kSlice : 1];
-  __shared__ float bsum[kBias ? kSlice : 1];
+  __shared__ float bsum[kBias == 2 ? kSlice : 1];
   __shared__ int list_at[kBias ? kThreads : 1];
   __shared__ float list_value[kBias ? kThreads : 1];
   __shared__ int wave_count[kWaves];
+  __shared__ int twice;  // a token is listed twice
   __shared__ uint64_t red[kWaves];
   const int row = (int)(blockIdx.x / (unsigned)slices), slice = (int)(blockIdx.x - (unsigned)row * (unsigned)slices);
   const int base = slice * kSlice, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -81,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
   for (int j = 0; j < V; ++j) {
     const int i = 4 * (tid + j * kThreads);
     if (i + 4 <= n) {
-      v[j] = load_any<f32x4>(x + i);
+      v[j] = load_past(x + i);
     } else {
       v[j] = f32x4{0, 0, 0, 0};
       for (int e = 0; e < 4; ++e)
@@ -101,6 +118,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
   const float *bias = a.bias + row * a.bias_stride;
   int id[kMarks ? kAhead : 1], bid = -1;
   float bvalue = 0.0f;
+  int entries = 0;  // of the list in LDS
   if (hist) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) id[j] = tid + j * kThreads < a.hist_stride ? ids[tid + j * kThreads] : -1;
@@ -125,55 +143,72 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
   blen = !biased ? 0 : blen < a.bias_stride ? blen : (int)a.bias_stride;
   if constexpr (kMarks) {
     for (int i = tid; i < kSlice / 4; i += kThreads) reinterpret_cast<u32x4 *>(marks)[i] = u32x4{0, 0, 0, 0};
+    // the slice's entries of the list's next kThreads, in list order: where
+    // each goes, then the entry itself
+    uint32_t at = 0;
+    uint64_t who = 0;
+    auto find = [&](int i) {
+      at = (uint32_t)bid - (uint32_t)base;
+      who = __ballot(i < blen && at < (uint32_t)n);
+      if (lane == 0) wave_count[wave] = __builtin_popcountll(who);
+    };
+    auto list = [&](int &place) {  // false: not this slice's
+      entries = 0;
+      place = __builtin_popcountll(who & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = wave_count[w];
+        place += w < wave ? c : 0;
+        entries += c;
+      }
+      if (!(who >> lane & 1)) return false;
+      list_at[place] = (int)at;
+      list_value[place] = bvalue;
+      return true;
+    };
+    if (kBias == 2 && biased) find(tid);
+    if (kBias == 1 && tid == 0) twice = 0;
     __syncthreads();
     auto count = [&](int i, int token) {
-      const uint32_t at = (uint32_t)token - (uint32_t)base;
-      if (i >= len || at >= (uint32_t)n) return;
-      if (i >= start) atomicAdd(&marks[at], 1u);
-      else atomicOr(&marks[at], kPrompt);
+      const uint32_t where = (uint32_t)token - (uint32_t)base;
+      if (i >= len || where >= (uint32_t)n) return;
+      if (i >= start) atomicAdd(&marks[where], 1u);
+      else atomicOr(&marks[where], kPrompt);
     };
     if (hist) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) count(tid + j * kThreads, id[j]);
       for (int i = tid + kAhead * kThreads; i < len; i += kThreads) count(i, ids[i]);
     }
-    if constexpr (kBias) {
+    if constexpr (kBias == 1) {
+      at = (uint32_t)bid - (uint32_t)base;
+      const bool in = tid < blen && at < (uint32_t)n;
+      list_at[tid] = in ? (int)at : -1;
+      list_value[tid] = bvalue;
+      if (in && (atomicOr(&marks[at], kBiased | (uint32_t)tid << kShortBits) & kBiased)) twice = 1;
+    }
+    if constexpr (kBias == 2) {
       for (int i0 = 0; i0 < blen; i0 += kThreads) {
-        // the slice's entries among the next kThreads, in list order
-        const int i = i0 + tid;
-        if (i0 > 0 && i < blen) {
-          bid = bids[i];
-          bvalue = bias[i];
-        }
-        const uint32_t at = (uint32_t)bid - (uint32_t)base;
-        const bool in = i < blen && at < (uint32_t)n;
-        const uint64_t who = __ballot(in);
-        if (lane == 0) wave_count[wave] = __builtin_popcountll(who);
-        __syncthreads();
-        int place = 0, entries = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const int c = wave_count[w];
-          place += w < wave ? c : 0;
-          entries += c;
-        }
-        place += __builtin_popcountll(who & ((1ull << lane) - 1));
-        if (in) {
-          list_at[place] = (int)at;
-          list_value[place] = bvalue;
-        }
-        __syncthreads();
-        if (in) {
-          bool first = true;
-          for (int e = 0; e < place; ++e) first = first && list_at[e] != (int)at;
-          if (first) {
-            const bool old = marks[at] & kBiased;
-            float sum = old ? __fadd_rn(bsum[at], bvalue) : bvalue;
-            for (int e = place + 1; e < entries; ++e)
-              if (list_at[e] == (int)at) sum = __fadd_rn(sum, list_value[e]);
-            bsum[at] = sum;
-            if (!old) atomicOr(&marks[at], kBiased);
+        if (i0 > 0) {
+          if (i0 + tid < blen) {
+            bid = bids[i0 + tid];
+            bvalue = bias[i0 + tid];
           }
+          find(i0 + tid);
+          __syncthreads();
+        }
+        int place;
+        const bool in = list(place);
+        __syncthreads();
+        bool first = in;
+        for (int e = 0; e < place && first; ++e) first = list_at[e] != (int)at;
+        if (first) {  // a token's first entry here adds them all
+          const bool old = marks[at] & kBiased;
+          float sum = old ? __fadd_rn(bsum[at], bvalue) : bvalue;
+          for (int e = place + 1; e < entries; ++e)
+            if (list_at[e] == (int)at) sum = __fadd_rn(sum, list_value[e]);
+          bsum[at] = sum;
+          if (!old) atomicOr(&marks[at], kBiased);
         }
         __syncthreads();
       }
@@ -183,6 +218,11 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
   float top = -INFINITY;  // the thread's largest, its lowest place, and whether one is NaN
   int where = 0;
   bool nan = false;
+  auto rank = [&](float value, int i) {
+    nan = nan || value != value;
+    where = value > top ? i : where;
+    top = value > top ? value : top;
+  };
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int i = 4 * (tid + j * kThreads);
@@ -192,10 +232,23 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t k = c[e] & kCount;
-          if (c[e] & ~kBiased) v[j][e] = v[j][e] > 0.0f ? __fdiv_rn(v[j][e], rep) : __fmul_rn(v[j][e], rep);
+          if (c[e] & (kPrompt | kCount)) v[j][e] = v[j][e] > 0.0f ? __fdiv_rn(v[j][e], rep) : __fmul_rn(v[j][e], rep);
           if (k) v[j][e] = __fsub_rn(__fsub_rn(v[j][e], __fmul_rn(freq, (float)k)), pres);
-          if constexpr (kBias)
+          if constexpr (kBias == 2)
             if (c[e] & kBiased) v[j][e] = __fadd_rn(v[j][e], bsum[i + e]);
+          if constexpr (kBias == 1)
+            if (c[e] & kBiased) {
+              float sum = list_value[c[e] >> kShortBits & (kThreads - 1)];
+              if (twice) {  // some token is: the places of a word may be mixed
+                bool any = false;
+                for (int b = 0; b < blen; ++b)
+                  if (list_at[b] == i + e) {
+                    sum = any ? __fadd_rn(sum, list_value[b]) : list_value[b];
+                    any = true;
+                  }
+              }
+              v[j][e] = __fadd_rn(v[j][e], sum);
+            }
         }
       }
     }
@@ -206,40 +259,25 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slic
     if (i + 4 <= n) {
       store_past(out + i, v[j]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        nan = nan || v[j][e] != v[j][e];
-        where = v[j][e] > top ? i + e : where;
-        top = v[j][e] > top ? v[j][e] : top;
-      }
+      for (int e = 0; e < 4; ++e) rank(v[j][e], i + e);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < n) {
           out[i + e] = v[j][e];
-          nan = nan || v[j][e] != v[j][e];
-          where = v[j][e] > top ? i + e : where;
-          top = v[j][e] > top ? v[j][e] : top;
+          rank(v[j][e], i + e);
         }
     }
   }
-  uint64_t best = nan ? ~0ull : key_of(top, base + where);
-  if (!a.best) return;
-  best = wave_max(best);
-  if (lane == 0) red[wave] = best;
-  __syncthreads();
-  if (tid != 0) return;
-  for (int w = 1; w < kWaves; ++w) best = red[w] > best ? red[w] : best;
-  if (slices == 1) {
-    a.best[row] = best_of(best);
-    return;
+  if (a.best) {
+    uint64_t best = wave_max(nan ? ~0ull : key_of(top, base + where));
+    if (lane == 0) red[wave] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kWaves; ++w) best = red[w] > best ? red[w] : best;
+      choose(a, row, slices, best, keys, arrived);
+    }
   }
-  // Atomics of agent scope; the wait between them is the order that the last
-  // workgroup relies on.  Both words are zero again afterwards.
-  __hip_atomic_fetch_max(&keys[row], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if (__hip_atomic_fetch_add(&arrived[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (uint32_t)slices - 1) return;
-  a.best[row] = best_of(__hip_atomic_exchange(&keys[row], (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  __hip_atomic_store(&arrived[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 size_t logits_workspace(int64_t rows) { return (size_t)rows * (sizeof(uint64_t) + sizeof(uint32_t)); }
@@ -254,15 +292,18 @@ hipError_t launch_logits(const LogitsArgs &a, void *workspace, int cu_count, hip
   // small slices until there is a workgroup for every CU: a call of few rows is
   // a wait for memory, which more CUs share
   const bool few = (int64_t)a.rows * a.vocab <= (int64_t)cu_count * 8192;
-  if (a.bias_ids) {
-    if (few) run(logits_kernel<1, true, true>, 4 * kThreads);
-    else run(logits_kernel<kVB, true, true>, 4 * kVB * kThreads);
+  if (a.bias_ids && (a.bias_stride > kThreads || a.hist_stride >= 1 << kShortBits)) {
+    if (few) run(logits_kernel<1, true, 2>, 4 * kThreads);
+    else run(logits_kernel<2, true, 2>, 8 * kThreads);
+  } else if (a.bias_ids) {
+    if (few) run(logits_kernel<1, true, 1>, 4 * kThreads);
+    else run(logits_kernel<4, true, 1>, 16 * kThreads);
   } else if (a.hist) {
-    if (few) run(logits_kernel<1, true, false>, 4 * kThreads);
-    else run(logits_kernel<kVH, true, false>, 4 * kVH * kThreads);
+    if (few) run(logits_kernel<1, true, 0>, 4 * kThreads);
+    else run(logits_kernel<4, true, 0>, 16 * kThreads);
   } else {
-    if (few) run(logits_kernel<1, false, false>, 4 * kThreads);
-    else run(logits_kernel<4, false, false>, 16 * kThreads);
+    if (few) run(logits_kernel<1, false, 0>, 4 * kThreads);
+    else run(logits_kernel<4, false, 0>, 16 * kThreads);
   }
   return hipGetLastError();
 }
