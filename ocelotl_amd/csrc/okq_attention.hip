@@ -203,7 +203,11 @@ __device__ __forceinline__ void limbs_bf16(const float (&x)[8], u32x4 (&limb)[3]
 __device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+    f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+    // one rounding for both uses: where x is a product, the compiler may round
+    // it to f16 in one step here and in two there, and a tie apart is a whole
+    // step of f16 that neither limb holds
+    asm("" : "+v"(hi));
     const f16x2 lo = {(_Float16)(x[2 * j] - (float)hi[0]), (_Float16)(x[2 * j + 1] - (float)hi[1])};
     limb[0][j] = __builtin_bit_cast(uint32_t, hi);
     limb[1][j] = __builtin_bit_cast(uint32_t, lo);

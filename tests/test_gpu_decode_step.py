@@ -382,6 +382,21 @@ def test_attention_of_odd_places(torch, okq, tn, d, offset, pad):
     assert wide[1].isnan().sum() == 16  # nothing written between the rows
 
 
+@pytest.mark.parametrize("tn", ["Q8_0", "F16", "BF16", "F32"])
+def test_attention_weights_keep_f32_precision(torch, okq, tn):
+    """Hundreds of short sequences with scores near zero: the bound is a few
+    steps of f32, so no weight of the 10^5 (tokens, heads, blocks) may lose
+    bits, a step of f16 apart (2^-11 of an eighth) least of all."""
+    lengths, d, kv, group = [8] * 256, 128, 4, 8
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], d, kv, group, 8, lengths)
+    q = q * 0.1
+    got = _attention(torch, okq, cache, table, q, lengths, 8, d ** -0.5)
+    torch.cuda.synchronize()
+    want = _attn_want(torch, cache, table, q, lengths, d ** -0.5, 0.0, 0, group)
+    assert want[2].max() < 2.0 ** -16
+    _attn_check(torch, got, want)
+
+
 def test_attention_hides_pages_outside_the_cache_and_clamps_lengths(torch, okq):
     """Table entries of -1, n_pages and far off; a length over max_length and
     over the table; a negative one; every page hidden."""
