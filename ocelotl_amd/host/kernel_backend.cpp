@@ -515,6 +515,84 @@ Result<void> HipKernelBackend::mlp_gated_silu_q(const DeviceTensor &x, size_t ro
                                     gate_buf.device_ptr(), up_buf.device_ptr(), out.device_ptr(), stream_));
 }
 
+namespace {
+
+Result<void> tensor_len(const char *call, const char *name, const DeviceTensor &t, size_t want) {
+  if (t.len() == want) return {};
+  return kernel_err(std::string(call) + " " + name + " length " + std::to_string(t.len()) + " does not match " +
+                    std::to_string(want));
+}
+
+const float *ptr_or_null(const DeviceTensor *t) { return t ? t->device_ptr() : nullptr; }
+
+Result<void> cache_status(okq_status st, uint32_t type) {
+  if (st == OKQ_E_TYPE)
+    return OcelotlError::unsupported("kv_cache_type", std::to_string(type), {"F32", "F16", "BF16", "Q8_0"});
+  return check(st);
+}
+
+}  // namespace
+
+Result<void> HipKernelBackend::qk_norm_rope_d(const DeviceTensor &q, const DeviceTensor &k, const DeviceTensor &v,
+                                              size_t tokens, size_t q_heads, const DeviceTensor *q_norm,
+                                              const DeviceTensor *k_norm, float epsilon, const int32_t *positions,
+                                              const DeviceTensor &inv_freq, bool interleaved,
+                                              const DeviceTensor &q_out, const okq_kv_pages &cache,
+                                              const int64_t *slots) const {
+  const char *call = "qk_norm_rope";
+  const size_t d = (size_t)cache.head_dim, qw = q_heads * d, kw = (size_t)cache.kv_heads * d;
+  for (const auto &[name, t, want] : {std::tuple<const char *, const DeviceTensor *, size_t>{"q", &q, tokens * qw},
+                                      {"k", &k, tokens * kw},
+                                      {"v", &v, tokens * kw},
+                                      {"q_out", &q_out, tokens * qw},
+                                      {"q_norm", q_norm, d},
+                                      {"k_norm", k_norm, d}}) {
+    if (!t) continue;
+    Result<void> r = tensor_len(call, name, *t, want);
+    if (r.is_err()) return r;
+  }
+  return cache_status(
+      okq_qk_norm_rope(q.device_ptr(), (int64_t)qw, k.device_ptr(), (int64_t)kw, v.device_ptr(), (int64_t)kw,
+                       (int64_t)tokens, (int64_t)q_heads, cache.kv_heads, cache.head_dim, ptr_or_null(q_norm),
+                       ptr_or_null(k_norm), epsilon, positions, inv_freq.device_ptr(), 2 * (int64_t)inv_freq.len(),
+                       interleaved ? 1 : 0, q_out.device_ptr(), (int64_t)qw, nullptr, 0, &cache, slots, stream_),
+      cache.type);
+}
+
+Result<void> HipKernelBackend::paged_attention_d(const DeviceTensor &q, size_t seqs, size_t q_heads,
+                                                 const okq_kv_pages &cache, const int32_t *block_table,
+                                                 size_t table_width, const int32_t *lengths, size_t max_length,
+                                                 float scale, float softcap, size_t window, const DeviceTensor &out,
+                                                 const DeviceTensor *lse) const {
+  const char *call = "paged_attention";
+  const size_t width = q_heads * (size_t)cache.head_dim;
+  Result<void> r = tensor_len(call, "q", q, seqs * width);
+  if (!r.is_err()) r = tensor_len(call, "out", out, seqs * width);
+  if (!r.is_err() && lse) r = tensor_len(call, "lse", *lse, seqs * q_heads);
+  if (r.is_err()) return r;
+  return cache_status(okq_paged_attention(q.device_ptr(), (int64_t)width, (int64_t)seqs, (int64_t)q_heads, &cache,
+                                          block_table, (int64_t)table_width, lengths, (int64_t)max_length, scale,
+                                          softcap, (int64_t)window, out.device_ptr(), (int64_t)width,
+                                          lse ? lse->device_ptr() : nullptr, stream_),
+                      cache.type);
+}
+
+Result<void> HipKernelBackend::logits_process_d(const DeviceTensor &logits, size_t rows, size_t vocab,
+                                                const LogitsOptions &o, const DeviceTensor &out, int32_t *best) const {
+  const char *call = "logits_process";
+  Result<void> r = tensor_len(call, "logits", logits, rows * vocab);
+  if (!r.is_err()) r = tensor_len(call, "out", out, rows * vocab);
+  for (const DeviceTensor *t : {o.repetition, o.frequency, o.presence})
+    if (!r.is_err() && t) r = tensor_len(call, "penalty", *t, rows);
+  if (!r.is_err() && o.bias) r = tensor_len(call, "bias", *o.bias, rows * o.bias_stride);
+  if (r.is_err()) return r;
+  return check(okq_logits_process(logits.device_ptr(), (int64_t)vocab, (int64_t)rows, (int64_t)vocab, o.history,
+                                  (int64_t)o.history_stride, o.history_len, o.history_start, ptr_or_null(o.repetition),
+                                  ptr_or_null(o.frequency), ptr_or_null(o.presence), o.bias_ids, ptr_or_null(o.bias),
+                                  (int64_t)o.bias_stride, o.bias_len, o.mask, (int64_t)o.mask_stride, out.device_ptr(),
+                                  (int64_t)vocab, best, stream_));
+}
+
 Result<DeviceTensor> HipKernelBackend::embedding_rows(const QuantizedWeight &table, const uint32_t *ids,
                                                       size_t n) const {
   auto a = device_alloc(n * table.ne0() * sizeof(float));

@@ -27,6 +27,8 @@
 #include <variant>
 #include <vector>
 
+struct okq_kv_pages;  // okq.h
+
 namespace ocelotl {
 
 // ---- errors (crates/core/src/lib.rs) -------------------------------------
@@ -278,6 +280,19 @@ class KernelBackend {
                                 size_t out_features, const DeviceTensor *bias, const DeviceTensor &out) const;
 };
 
+// The parts of logits_process_d that a call has (null or zero: none); device
+// pointers, as okq_logits_process documents them.
+struct LogitsOptions {
+  const int32_t *history = nullptr, *history_len = nullptr, *history_start = nullptr;
+  size_t history_stride = 0;
+  const DeviceTensor *repetition = nullptr, *frequency = nullptr, *presence = nullptr;  // [rows]
+  const int32_t *bias_ids = nullptr, *bias_len = nullptr;
+  const DeviceTensor *bias = nullptr;  // [rows, bias_stride]
+  size_t bias_stride = 0;
+  const uint32_t *mask = nullptr;
+  size_t mask_stride = 0;
+};
+
 // The gfx950 backend: name() == "hip-gfx950" (the backend_id convention of
 // crates/kernels/src/cubecl_backend.rs:2268-2272).
 class HipKernelBackend final : public KernelBackend {
@@ -335,6 +350,23 @@ class HipKernelBackend final : public KernelBackend {
   // dequantized into row j of the result (the f32 row copy of
   // qwen2_5/prefill.rs:95-105 for a GGUF table).
   Result<DeviceTensor> embedding_rows(const QuantizedWeight &table, const uint32_t *ids, size_t n) const;
+  // The decode step around the projections (okq.h: okq_qk_norm_rope,
+  // okq_paged_attention, okq_logits_process) on device tensors of contiguous
+  // rows; integer arrays are device pointers.  No counterparts in the trait.
+  // Norm of query and key heads (null: none), rotation of the first 2 *
+  // inv_freq.len() values, and the store of k and v at `slots` of the cache.
+  Result<void> qk_norm_rope_d(const DeviceTensor &q, const DeviceTensor &k, const DeviceTensor &v, size_t tokens,
+                              size_t q_heads, const DeviceTensor *q_norm, const DeviceTensor *k_norm, float epsilon,
+                              const int32_t *positions, const DeviceTensor &inv_freq, bool interleaved,
+                              const DeviceTensor &q_out, const okq_kv_pages &cache, const int64_t *slots) const;
+  // One new token of each sequence over its pages; lse may be null.
+  Result<void> paged_attention_d(const DeviceTensor &q, size_t seqs, size_t q_heads, const okq_kv_pages &cache,
+                                 const int32_t *block_table, size_t table_width, const int32_t *lengths,
+                                 size_t max_length, float scale, float softcap, size_t window, const DeviceTensor &out,
+                                 const DeviceTensor *lse) const;
+  // Penalties, biases and grammar mask, and the greedy token (best may be null).
+  Result<void> logits_process_d(const DeviceTensor &logits, size_t rows, size_t vocab, const LogitsOptions &options,
+                                const DeviceTensor &out, int32_t *best) const;
   // Waits for the backend's stream.
   Result<void> synchronize() const;
 
