@@ -213,11 +213,20 @@ __device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2])
     limb[1][j] = __builtin_bit_cast(uint32_t, lo);
   }
 }
-// Two codes, in bytes 0 and 2 (the others zero), as f16: with its top bit
-// flipped a code is code + 128, and 0x6400 | b is the f16 1024 + b.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
+// Codes as f16: with its top bit flipped a code's byte is code + 128, and the
+// f16 whose bytes are that and 0x64 is 1024 + 128 + code.
+__device__ __forceinline__ uint32_t less_1152(uint32_t v) {
   const f16x2 c = {(_Float16)1152.0f, (_Float16)1152.0f};
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, two ^ 0x64806480u) - c);
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - c);
+}
+__device__ __forceinline__ uint32_t codes_f16(uint32_t two) {  // in bytes 0 and 2, the others zero
+  return less_1152(two ^ 0x64806480u);
+}
+// A register whose upper half nothing reads (so that nothing clears it).
+__device__ __forceinline__ uint32_t low_half(uint16_t v) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 w = {v, 0};
+  return __builtin_bit_cast(uint32_t, __builtin_shufflevector(w, w, 0, -1));
 }
 // x[j] = p[j] * (lane j, or 8 + j, of the own row's d): a block's scales of the
 // lane's eight token slots.
@@ -391,7 +400,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       for (int v = 0; v < kVG; ++v) {
         const int i = 16 * kVD * v + kVD * n, ii = (kFull && 32 * NC % (16 * kVD) == 0) || i < D ? i : 0;
         if constexpr (kQ) {
-          vr[j][v] = u32x4{load_any<uint16_t>(row + (kFull || 32 * v < D ? kQ8Bytes * v : 0)), 0, 0, 0};
+          vr[j][v] = u32x4{low_half(load_any<uint16_t>(row + (kFull || 32 * v < D ? kQ8Bytes * v : 0))), 0, 0, 0};
         } else if constexpr (kF || kVD == 8) {
           vr[j][v] = *reinterpret_cast<const u32x4 *>(row + ii * (kF ? 4 : 2));
         } else {
@@ -412,8 +421,8 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
     for (int j = 0; j < kPer; j += 4) {
       const int i = 4 * kPer * (kRegQ ? u : wave + u * kWaves) + kPer * g + j;
-      f32x4 v = {0, 0, 0, 0};  // head_dim is a multiple of four
-      if (n < heads && i < D) v = load_any<f32x4>(q + (int64_t)n * D + i);
+      // heads and dims that are not there read others, and become zero below
+      const f32x4 v = load_any<f32x4>(q + (int64_t)(n < heads ? n : 0) * D + (i < D ? i : 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[u][j + e] = v[e];
     }
@@ -437,17 +446,29 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
     __syncthreads();
     int t0 = seg + wave * kTile, buf = 0;
     uint32_t hidden = 0;
+    // the queries are here (they were asked for before the pages): said so
+    // that their use after the next loads waits for nothing
+    auto settled = [&]() {
+#pragma unroll
+      for (int u = 0; u < kMy; ++u)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) asm volatile("" : "+v"(x[u][j]));
+    };
+    settled();
     if (t0 < end) {
       hidden = place(t0, end, page0, 0);
       load_k(0);
       load_v(0);
     }
     if (seg == lo) {
-      // not before the first rows are requested
+      settled();  // and not used before the first rows are requested
 #pragma unroll
       for (int u = 0; u < kMy; ++u)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) asm volatile("" : "+v"(x[u][j]));
+        for (int j = 0; j < kPer; ++j) {
+          const bool there = n < heads && (kFull || 4 * kPer * (kRegQ ? u : wave + u * kWaves) + kPer * g + j < D);
+          x[u][j] = there ? x[u][j] : 0.0f;
+        }
       if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
         float mx = 0.0f;
 #pragma unroll
@@ -499,8 +520,9 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
             u32x4 op;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-              op[2 * w] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c010c00u));
-              op[2 * w + 1] = codes_f16(__builtin_amdgcn_perm(0u, kr[s][c][w], 0x0c030c02u));
+              const uint32_t x = kr[s][c][w] ^ 0x80808080u;
+              op[2 * w] = less_1152(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u));
+              op[2 * w + 1] = less_1152(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u));
             }
             f32x4 t = {0, 0, 0, 0};
 #pragma unroll
@@ -512,6 +534,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           scale_slots(b, dk[c >> 1], c & 1, y);
 #pragma unroll
           for (int j = 0; j < kSlots; ++j) p[j] += y[j];
+          __builtin_amdgcn_sched_barrier(0);  // a block at a time: all at once spill
         }
       } else {
         constexpr int kAcc = kF ? 4 : kL;  // one sum a limb, or a quarter of the dims: products that do not wait for each other
@@ -851,9 +874,10 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   const int64_t chunks = std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles);
   const bool splits = chunks > 1 && p.units > 1;  // one unit: every sequence is one chunk
   p.grid = splits ? std::min<int64_t>(a.seqs + p.units + 1, a.seqs * chunks) : a.seqs;
-  if (splits) {
-    p.arrived_bytes = (size_t)(2 * (p.units + 1) * pairs) * sizeof(uint32_t);
-    p.part_bytes = (size_t)(2 * (p.units + 1) * pairs) * (size_t)((std::min(a.group, kHeads) * (c.head_dim + 2) + 3) / 4 * 4) * sizeof(float);
+  if (splits) {  // the same for every call of these heads: slots for the most units
+    const size_t slots = (size_t)(2 * (2 * units + 1) * pairs);
+    p.arrived_bytes = slots * sizeof(uint32_t);
+    p.part_bytes = slots * (size_t)((std::min(a.group, kHeads) * (c.head_dim + 2) + 3) / 4 * 4) * sizeof(float);
   }
   return p;
 }
