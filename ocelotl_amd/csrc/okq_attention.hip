@@ -10,6 +10,7 @@
 // (head_dim or addresses that are no multiple of 16 bytes, head_dim above
 // 256), one value at a time.
 #include <algorithm>
+#include <type_traits>
 
 #include "okq_device.h"
 #include "okq_internal.h"
@@ -345,11 +346,15 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
   int chunk = ceil_div(total, ta.units, ta.inv_units);
   chunk = (chunk + kWaves - 1) / kWaves * kWaves;  // a tile more for one wave costs what it costs for all
   chunk = chunk < ta.min_tiles ? ta.min_tiles : chunk;
-  const float inv_chunk = __builtin_amdgcn_rcpf((float)chunk);
   int seq = -1, at = 0, chunks = 0, slot = 0, lo = 0, hi = 0, before = 0, alone = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     if (a.seqs > 64) look(s0);
-    const int c = s0 + lane >= a.seqs ? 0 : tiles > chunk ? ceil_div(tiles, chunk, inv_chunk) : 1;
+    // A sequence's own chunks are not below half the root of its tiles: what
+    // fewer tiles save each of them, the join of more chunks takes back (60000
+    // tokens of one head: 17.6 us in 117 chunks, 32.6 in 469).
+    int own = (int)(0.5f * __builtin_amdgcn_sqrtf((float)tiles));
+    own = own > chunk ? (own + kWaves - 1) / kWaves * kWaves : chunk;
+    const int c = s0 + lane >= a.seqs ? 0 : tiles > own ? ceil_div(tiles, own, __builtin_amdgcn_rcpf((float)own)) : 1;
     const int sum = wave_scan(c);
     const uint64_t who = __ballot(unit >= before + sum - c && unit < before + sum), ones = __ballot(c == 1);
     if (who) {
@@ -815,22 +820,27 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
   for (int h = row - team * heads; h < heads; h += kRows) {
     f32x4 v = {0, 0, 0, 0};
     float top = -INFINITY, sum = 0.0f;
-    constexpr int kAtOnce = 4;
-    for (int i0 = team; i0 < chunks && team < teams && 4 * quad < D; i0 += kAtOnce * teams) {
-      float mi[kAtOnce], li[kAtOnce];
-      f32x4 vi[kAtOnce];
+    // n chunks requested together: with four a wait each, a join of 123 takes
+    // 8 us more than with sixteen, one of five 0.5 us less
+    auto gather = [&](auto count, int i0) {
+      constexpr int kN = decltype(count)::value;
+      float mi[kN], li[kN];
+      f32x4 vi[kN];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int i = i0 + u * teams;
-        const uint32_t from = origin + (uint32_t)(i < chunks ? i : i0) * step;
+      for (int u = 0; u < kN; ++u) {
+        int i = i0 + u * teams;
+        mi[u] = -INFINITY, li[u] = 0.0f, vi[u] = f32x4{0, 0, 0, 0};
+        if (kN > 4 && i >= chunks) continue;
+        i = i < chunks ? i : i0;
+        const uint32_t from = origin + (uint32_t)i * step;
         mi[u] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(part, from + 4 * (heads * D + h), 0, kAgent));
         li[u] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(part, from + 4 * (heads * D + heads + h), 0, kAgent));
         vi[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, from + 4 * (h * D + 4 * quad), 0, kAgent));
       }
       float most = top;
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (i0 + u * teams >= chunks) mi[u] = -INFINITY, li[u] = 0.0f, vi[u] = f32x4{0, 0, 0, 0};
+      for (int u = 0; u < kN; ++u) {
+        if (kN <= 4 && i0 + u * teams >= chunks) mi[u] = -INFINITY, li[u] = 0.0f, vi[u] = f32x4{0, 0, 0, 0};
         most = __builtin_fmaxf(most, mi[u]);
       }
       const float base = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(top - base);
@@ -838,10 +848,17 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       sum *= keep;
       top = most;
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
+      for (int u = 0; u < kN; ++u) {
         const float w = __builtin_amdgcn_exp2f(mi[u] - base);
         sum += w * li[u];
         v += w * vi[u];
+      }
+    };
+    if (team < teams && 4 * quad < D) {
+      if (chunks <= 4 * teams) {
+        if (team < chunks) gather(std::integral_constant<int, 4>{}, team);
+      } else {
+        for (int i0 = team; i0 < chunks; i0 += 16 * teams) gather(std::integral_constant<int, 16>{}, i0);
       }
     }
     if (teams > 1) {  // every row here once
