@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeArgs a) {
 // heads of one token a pass of the wave.  The angles, 64-bit arithmetic, are
 // formed once for all of a wave's passes.  What bounds it is memory: a row is
 // read and written once, in 16-byte pieces, kAhead passes requested at a time
-// (4096 tokens of 32 + 8 heads of 128, 184 MB: 34.3 us, 5.4 TB/s, with two;
+// (4096 tokens of 32 + 8 heads of 128, 184 MB: 35 us, 5.3 TB/s, with two;
 // four, and outputs through the caches, 46).
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -332,9 +332,9 @@ hipError_t launch_rope(const RopeArgs &a, int cu_count, hipStream_t s) {
     const int lanes = D <= 64 ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : 64, at_once = 64 / lanes;
     const int all = (heads + at_once - 1) / at_once;  // a token's passes
     // A wave takes several passes of a token, sharing its angles, once there
-    // are waves enough: 64 a CU (4096 tokens of 32 + 8 heads of 128: 34.3 us
-    // so, 35.7 with 32, 37.1 with 16)
-    const int64_t want = (int64_t)a.tokens * all / (64 * (int64_t)cu_count);
+    // are waves enough: 32 a CU, rounded down (2048 tokens of 32 + 8 heads of
+    // 128: 16.8 us so, 18.4 with 64; 2598 of 28 + 7 of 96: 17.3, 19.2)
+    const int64_t some = 32 * (int64_t)cu_count, want = ((int64_t)a.tokens * all + some - 1) / some;
     const int passes = (int)(want < 1 ? 1 : want > all ? all : want), shares = (all + passes - 1) / passes;
     const dim3 grid((unsigned)(((int64_t)a.tokens * shares + 3) / 4));
     if (lanes == 8) launch_timed(rope_kernel<8>, grid, dim3(256), 0u, s, a, shares, passes);
