@@ -167,3 +167,13 @@ def test_valid_calls_without_a_device_are_refused_as_such(okqlib):
     assert logits() == okq.E_NODEV
     assert logits(hist=None, hs=0, hlen=None, hstart=None, rep=None, freq=None, pres=None, bids=None, bias=None,
                   blen=None, mask=None, ms=0, best=None) == okq.E_NODEV
+
+
+@pytest.mark.parametrize("call,kw,text", [
+    (attention, dict(longest=(1 << 30) + 1), "max_length"),
+    (logits, dict(hs=1 << 30), "history_stride"),
+    (logits, dict(bs=1 << 30), "bias_stride"),
+])
+def test_sizes_past_what_the_kernels_index(okqlib, call, kw, text):
+    assert call(**kw) == okq.E_SHAPE
+    assert text in okq.last_error()

@@ -692,3 +692,51 @@ def test_logits_in_a_graph(torch, okq):
         step(None)
         torch.cuda.synchronize()
         _logits_check(out.cpu().numpy(), best.cpu().numpy(), d, True, True)
+
+
+# ---- wider heads, larger groups, pages of one token, longer lists ---------------------
+
+@pytest.mark.parametrize("tn", ["BF16", "F16", "F32", "Q8_0"])
+@pytest.mark.parametrize("d", [160, 192, 320])
+def test_attention_of_heads_between_the_common_sizes(torch, okq, tn, d):
+    print(f"[gpu] attention {tn} head_dim {d}", flush=True)
+    lengths = [700, 0, 33]
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], d, 2, 3, 16, lengths)
+    got = _attention(torch, okq, cache, table, q, lengths, 700, d ** -0.5)
+    torch.cuda.synchronize()
+    _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, d ** -0.5, 0.0, 0, 3))
+
+
+@pytest.mark.parametrize("tn,kv,group,page", [("BF16", 520, 1, 1), ("F32", 520, 2, 1), ("F16", 130, 17, 2), ("Q8_0", 520, 1, 1)])
+def test_attention_of_one_chunk_with_more_pages_than_are_held_at_once(torch, okq, tn, kv, group, page):
+    """So many heads that nothing is split: one workgroup walks all pages, some of them hidden."""
+    print(f"[gpu] attention pages {tn} {kv} {page}", flush=True)
+    lengths = [1200 * page, 509 * page, 511 * page, 0]
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], 32, kv, group, page, lengths)
+    table[0, 505:540], table[0, 1021], table[2, 510] = -1, cache.n_pages, -7
+    got = _attention(torch, okq, cache, table, q, lengths, 1300 * page, 0.2)
+    torch.cuda.synchronize()
+    _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 0.2, 0.0, 0, group))
+
+
+@pytest.mark.parametrize("tn,group", [("BF16", 17), ("F16", 40), ("F32", 33), ("Q8_0", 24)])
+def test_attention_of_large_groups_split_over_a_long_cache(torch, okq, tn, group):
+    print(f"[gpu] attention group {tn} {group}", flush=True)
+    lengths = [9000, 5]
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], 64, 1, group, 32, lengths)
+    got = [_attention(torch, okq, cache, table, q, lengths, 9000, 0.125, 40.0, 6001) for _ in range(2)]
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+    _attn_check(torch, got[0], _attn_want(torch, cache, table, q, lengths, 0.125, 40.0, 6001, group))
+
+
+@pytest.mark.parametrize("rows,vocab,hist,biases,masked,duplicates", [
+    (3, 50001, 9000, 1025, True, False), (2, 6000, 5000, 3000, False, True), (40, 33000, 4500, 2000, True, True),
+    (1, 70000, 4097, 1024, False, True), (3, 900, 6000, 1500, True, True)])
+def test_logits_of_long_lists(torch, okq, rows, vocab, hist, biases, masked, duplicates):
+    """Histories and biases longer than a workgroup reads at once."""
+    print(f"[gpu] logits {rows}x{vocab} h{hist} b{biases}", flush=True)
+    d = _logits_inputs(torch, rows, vocab, hist, biases, masked, 11 + vocab, duplicates)
+    got, best = _logits(torch, okq, d, hist, biases, masked, inplace=rows == 2)
+    _logits_check(got, best, d, True, masked)
