@@ -548,9 +548,18 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       if constexpr (kQ) {  // a block's products, times its keys' scales
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) p[j] = 0.0f;
+        // A block's products are folded in behind the next block's.  pinned()
+        // keeps the folding there: left to itself it moves behind all blocks,
+        // whose products and scales then need more registers than there are.
+        float b[2][8];
+        auto fold = [&](int c) {
+          float y[8];
+          scale_slots(b[c & 1], dk[c >> 1], c & 1, y);
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) p[j] += y[j];
+        };
 #pragma unroll
         for (int c = 0; c < kQC; ++c) {
-          float b[8];
 #pragma unroll
           for (int s = 0; s < kSub; ++s) {
             u32x4 op;
@@ -564,14 +573,14 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
             for (int k = 0; k < kL; ++k) t = mfma<kType>(op, query(c, k), t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[4 * s + i] = t[i];
+            for (int i = 0; i < 4; ++i) b[c & 1][4 * s + i] = t[i];
           }
-          float y[8];
-          scale_slots(b, dk[c >> 1], c & 1, y);
+          if (c > 0) fold(c - 1);
 #pragma unroll
-          for (int j = 0; j < kSlots; ++j) p[j] += y[j];
+          for (int j = 0; j < kSlots; ++j) asm volatile("" : "+v"(p[j]));
           __builtin_amdgcn_sched_barrier(0);  // a block at a time: all at once spill
         }
+        fold(kQC - 1);
       } else {
         constexpr int kAcc = kF ? 4 : kL;  // one sum a limb, or a quarter of the dims: products that do not wait for each other
         f32x4 part[kSub][kAcc];
