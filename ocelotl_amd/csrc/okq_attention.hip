@@ -309,7 +309,14 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
   // dims of a lane's load of V; Q8_0: two, so that a product's 16 rows (one
   // dim of each lane) lie in one block and its scales can go with P
   constexpr int kVD = kQ ? 2 : kF || NC <= 2 ? 4 : 8;
-  constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such loads
+  constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such groups
+  // Wide Q8_0 rows: loads of four dims, a 16-lane row's upper eight lanes those
+  // of the next block, so a register holds two blocks.  Loads of two dims take
+  // 64 registers of a tile there, more than are left (4 sequences of 14563,
+  // head_dim 256: 36.9 us); at head_dim 128 they are the faster ones, as most
+  // of the four-byte loads lie across two words (131072 tokens: 68.5 us, 73.9).
+  constexpr bool kPaired = kQ && NC > 4;
+  constexpr int kVL = kPaired ? (NC + 1) / 2 : kVG;                 // a token's loads of V
   constexpr int kSB = (NC + 1) / 2;                                 // registers of Q8_0 scales
   constexpr bool kRegQ = NC <= (kQ ? 3 : 4);  // the queries' limbs in registers, every wave its own; else one copy in LDS
   constexpr int kQuads = NC <= 2 ? 16 : NC <= 4 ? 32 : 64;          // threads of a row of outputs, four values each
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
     wave_sync();
     return (uint32_t)__ballot(!in);  // lanes past kTile repeat
   };
-  u32x4 kr[kSub][kQC], vr[kSlots][kVG];
+  u32x4 kr[kSub][kQC], vr[kSlots][kVL];
   float dk[kSB], dv[kSB];  // Q8_0: scale of token slot n & 7, block 2 i + (n >> 3)
   auto scales = [&](const uint8_t *base, int buf, float (&d)[kSB]) {
     const uint8_t *row = base + offs[wave][buf][16 * ((n & 7) >> 2) + 4 * g + (n & 3)];
@@ -429,12 +436,15 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       const uint8_t *row = vb + offs[wave][buf][16 * (j >> 2) + 4 * g + (j & 3)];
-      if constexpr (kQ) row += 2 + 2 * n;
+      if constexpr (kQ) row += 2 + (kPaired ? 4 * (n & 7) : 2 * n);
 #pragma unroll
-      for (int v = 0; v < kVG; ++v) {
+      for (int v = 0; v < kVL; ++v) {
         const int i = 16 * kVD * v + kVD * n, ii = (kFull && 32 * NC % (16 * kVD) == 0) || i < D ? i : 0;
-        if constexpr (kQ) {
+        if constexpr (kQ && !kPaired) {
           vr[j][v] = u32x4{low_half(load_any<uint16_t>(row + (kFull || 32 * v < D ? kQ8Bytes * v : 0))), 0, 0, 0};
+        } else if constexpr (kPaired) {
+          const bool there = kFull ? 2 * v + 1 < NC || n < 8 : 32 * (2 * v + (n >> 3)) < D;
+          vr[j][v] = u32x4{load_any<uint32_t>(row + (there ? kQ8Bytes * (2 * v + (n >> 3)) : 0)), 0, 0, 0};
         } else if constexpr (kF || kVD == 8) {
           vr[j][v] = *reinterpret_cast<const u32x4 *>(row + ii * (kF ? 4 : 2));
         } else {
@@ -627,7 +637,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           const bool out = own >> (16 * (j >> 2) + (j & 3)) & 1u;
           p[j] = out ? -INFINITY : p[j];
 #pragma unroll
-          for (int v = 0; v < kVG; ++v)
+          for (int v = 0; v < kVL; ++v)
             if constexpr (!kQ) vr[j][v] = out ? u32x4{0, 0, 0, 0} : vr[j][v];
         }
         if constexpr (kQ) {
@@ -686,8 +696,21 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
         const float up = ldexpf(1.0f, 6 - d_exp);
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) p[j] *= up;
+        // of a pair of blocks, lanes below 8 keep the lower two dims, those above
+        // the upper: the rest is swapped between them
+        const uint32_t halves = n < 8 ? 0x05040100u : 0x03020706u;
+        uint32_t codes[kSlots];  // two dims' codes of block v in bytes 0 and 1, of a pair's second in bytes 2 and 3
 #pragma unroll
         for (int v = 0; v < kVG; ++v) {  // block v
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            if constexpr (!kPaired) {
+              codes[j] = vr[j][v][0];
+            } else if (v % 2 == 0) {
+              const uint32_t x = vr[j][v / 2][0];
+              codes[j] = __builtin_amdgcn_perm((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true), x, halves);
+            }
+          }
           float y[8];
           scale_slots(p, dv[v >> 1], v & 1, y);
           u32x4 limb[kL];
@@ -697,7 +720,8 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           for (int d = 0; d < 2; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              op[d][j] = codes_f16(__builtin_amdgcn_perm(vr[2 * j + 1][v][0], vr[2 * j][v][0], d ? 0x0c050c01u : 0x0c040c00u));
+              op[d][j] = codes_f16(__builtin_amdgcn_perm(codes[2 * j + 1], codes[2 * j],
+                                                         0x0c040c00u + 0x00010001u * ((kPaired ? 2 * (v % 2) : 0) + d)));
 #pragma unroll
           for (int k = 0; k < kL; ++k)
 #pragma unroll
@@ -771,8 +795,8 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       for (int v = 0; v < kVG; ++v)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int dim = 16 * kVD * v + kVD * (4 * g + i);
-          if constexpr (kVD == 2) {
+          const int r = 4 * g + i, dim = 16 * kVD * v + (kPaired ? 4 * (r & 7) + 2 * (r >> 3) : kVD * r);
+          if constexpr (kQ) {
             if (!kFull && dim >= D) continue;
             to[dim] = o[v * kVD][i] * f;
             to[dim + 1] = o[v * kVD + 1][i] * f;
