@@ -22,72 +22,127 @@ namespace {
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
 
 // Value i of a cached row.
-__device__ __forceinline__ float cached(int type, const uint8_t *row, int i) {
-  if (type == kF32) return reinterpret_cast<const float *>(row)[i];
-  if (type == kQ8_0) return deq_elem(kQ8_0, row, (uint32_t)i);
+template <int kType>
+__device__ __forceinline__ float cached(const uint8_t *row, int i) {
+  if constexpr (kType == kF32) return reinterpret_cast<const float *>(row)[i];
+  if constexpr (kType == kQ8_0) return deq_elem(kQ8_0, row, (uint32_t)i);
   const uint16_t b = reinterpret_cast<const uint16_t *>(row)[i];
-  return type == kF16 ? f16_bits_hw(b) : as_f32((uint32_t)b << 16);
+  return kType == kF16 ? f16_bits_hw(b) : as_f32((uint32_t)b << 16);
 }
+
+constexpr int kRowHeads = 4, kRowTokens = 4;
+// As many waves as the registers of a row allow: one workgroup has all tokens.
+constexpr int row_waves(int kV) { return kV <= 4 ? 16 : 8; }
 
 }  // namespace
 
-// One workgroup per sequence and query head; its four waves take the tokens
-// in turn, a wave's lanes the row's values.  Any head_dim up to kMaxHeadDim,
-// any alignment, every cache type.
-__global__ __launch_bounds__(256) void attention_rows_kernel(AttnArgs a) {
-  constexpr int kV = kMaxHeadDim / 64;
-  __shared__ float lds[4][kMaxHeadDim + 2];
-  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+// One workgroup per sequence and kRowHeads query heads of a key/value head,
+// which share its rows; its waves take kRowTokens tokens each in turn, a wave's
+// lanes the row's values.  Any head_dim up to 64 kV, any alignment.  The waits
+// for pages and rows bound it, so a wave asks for all its tokens' rows at once
+// (16 sequences of 2000 tokens, 32 heads over 8, bf16: head_dim 512 282 us,
+// 100 170; token by token, four waves and a workgroup a head, 3986 and 928).
+template <int kType, int kV>
+__global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(AttnArgs a, int sets) {
+  constexpr int kRowWaves = row_waves(kV);
+  __shared__ float lds[kRowWaves][kRowHeads][64 * kV + 2];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
   const int D = a.cache.head_dim, pt = a.cache.page_tokens;
-  const int seq = (int)(blockIdx.x / (unsigned)a.q_heads), h = (int)(blockIdx.x % (unsigned)a.q_heads);
-  const int64_t kv_at = (int64_t)(h / a.group) * a.cache.head_stride;
-  float q[kV], o[kV];
-  for (int j = 0; j < kV; ++j) {
-    const int i = lane + 64 * j;
-    q[j] = i < D ? a.q[seq * a.q_stride + (int64_t)h * D + i] : 0.0f;
-    o[j] = 0.0f;
+  const int set = (int)(blockIdx.x % (unsigned)sets), pair = (int)(blockIdx.x / (unsigned)sets);
+  const int seq = pair / a.cache.kv_heads, kvh = pair - seq * a.cache.kv_heads;
+  const int heads = a.group - set * kRowHeads < kRowHeads ? a.group - set * kRowHeads : kRowHeads;
+  const int64_t h0 = (int64_t)kvh * a.group + set * kRowHeads;
+  const uint8_t *kb = a.cache.k + (int64_t)kvh * a.cache.head_stride, *vb = a.cache.v + (int64_t)kvh * a.cache.head_stride;
+  const int32_t *table = a.table + (int64_t)seq * a.table_width;
+  float q[kRowHeads][kV], o[kRowHeads][kV], m[kRowHeads], l[kRowHeads];
+#pragma unroll
+  for (int h = 0; h < kRowHeads; ++h) {
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const int i = lane + 64 * j;
+      q[h][j] = h < heads && i < D ? a.q[seq * a.q_stride + (h0 + h) * D + i] : 0.0f;
+      o[h][j] = 0.0f;
+    }
+    m[h] = -INFINITY;
+    l[h] = 0.0f;
   }
   int len = a.lengths[seq];
   len = len < a.max_len ? len : a.max_len;
   const int lo = a.window && len > a.window ? len - a.window : 0;
-  float m = -INFINITY, l = 0.0f;
-  for (int t = lo + wave; t < len; t += 4) {
-    const int page = a.table[(int64_t)seq * a.table_width + t / pt];
-    if ((unsigned)page >= (unsigned)a.cache.n_pages) continue;
-    const int64_t at = page * a.cache.page_stride + kv_at + t % pt * a.cache.token_stride;
-    float dot = 0.0f;
-    for (int j = 0; j < kV; ++j) {
-      const int i = lane + 64 * j;
-      if (i < D) dot += q[j] * cached(a.cache.type, a.cache.k + at, i);
+  for (int t0 = lo + wave * kRowTokens; t0 < len; t0 += kRowWaves * kRowTokens) {
+    bool seen[kRowTokens];
+    float k[kRowTokens][kV], v[kRowTokens][kV];
+    int64_t at[kRowTokens];
+#pragma unroll
+    for (int u = 0; u < kRowTokens; ++u) {  // tokens that are not seen read the cache's first row
+      const int t = t0 + u < len ? t0 + u : len - 1, page = table[t / pt];
+      seen[u] = t0 + u < len && (unsigned)page < (unsigned)a.cache.n_pages;
+      at[u] = seen[u] ? page * a.cache.page_stride + t % pt * a.cache.token_stride : 0;
     }
-    float s = wave_sum(dot) * a.scale;
-    if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
-    const float keep = expf(m - base), p = expf(s - base);
-    m = top;
-    l = l * keep + p;
-    for (int j = 0; j < kV; ++j) {
-      const int i = lane + 64 * j;
-      if (i < D) o[j] = o[j] * keep + p * cached(a.cache.type, a.cache.v + at, i);
+#pragma unroll
+    for (int u = 0; u < kRowTokens; ++u)
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        const int i = lane + 64 * j;
+        const float kx = cached<kType>(kb + at[u], i < D ? i : 0), vx = cached<kType>(vb + at[u], i < D ? i : 0);
+        k[u][j] = i < D ? kx : 0.0f;
+        v[u][j] = i < D && seen[u] ? vx : 0.0f;
+      }
+#pragma unroll
+    for (int h = 0; h < kRowHeads; ++h) {
+      float s[kRowTokens], top = m[h];
+#pragma unroll
+      for (int u = 0; u < kRowTokens; ++u) {
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) dot += q[h][j] * k[u][j];
+        s[u] = wave_sum(dot) * a.scale;
+        if (a.softcap > 0.0f) s[u] = a.softcap * tanhf(s[u] / a.softcap);
+        s[u] = seen[u] ? s[u] : -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      const float base = top == -INFINITY ? 0.0f : top, keep = expf(m[h] - base);
+      m[h] = top;
+      l[h] *= keep;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) o[h][j] *= keep;
+#pragma unroll
+      for (int u = 0; u < kRowTokens; ++u) {
+        const float p = expf(s[u] - base);
+        l[h] += p;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) o[h][j] += p * v[u][j];
+      }
     }
   }
-  for (int j = 0; j < kV; ++j)
-    if (lane + 64 * j < D) lds[wave][lane + 64 * j] = o[j];
-  if (lane == 0) {
-    lds[wave][kMaxHeadDim] = m;
-    lds[wave][kMaxHeadDim + 1] = l;
+#pragma unroll
+  for (int h = 0; h < kRowHeads; ++h) {
+#pragma unroll
+    for (int j = 0; j < kV; ++j) lds[wave][h][lane + 64 * j] = o[h][j];
+    if (lane == 0) {
+      lds[wave][h][64 * kV] = m[h];
+      lds[wave][h][64 * kV + 1] = l[h];
+    }
   }
   __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, lds[w][kMaxHeadDim]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  for (int w = 0; w < 4; ++w) sum += lds[w][kMaxHeadDim + 1] * expf(lds[w][kMaxHeadDim] - base);
-  for (int i = (int)threadIdx.x; i < D; i += 256) {
-    float v = 0.0f;
-    for (int w = 0; w < 4; ++w) v += lds[w][i] * expf(lds[w][kMaxHeadDim] - base);
-    a.out[seq * a.out_stride + (int64_t)h * D + i] = sum == 0.0f ? 0.0f : v / sum;
+  for (int h = 0; h < heads; ++h) {
+    float top = -INFINITY, sum = 0.0f, weight[kRowWaves];
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) top = fmaxf(top, lds[w][h][64 * kV]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) {
+      weight[w] = expf(lds[w][h][64 * kV] - base);
+      sum += lds[w][h][64 * kV + 1] * weight[w];
+    }
+    for (int i = (int)threadIdx.x; i < D; i += 64 * kRowWaves) {
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kRowWaves; ++w) x += lds[w][h][i] * weight[w];
+      a.out[seq * a.out_stride + (h0 + h) * D + i] = sum == 0.0f ? 0.0f : x / sum;
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[(int64_t)seq * a.q_heads + h0 + h] = top == INFINITY ? top : base + logf(sum);
   }
-  if (a.lse && threadIdx.x == 0) a.lse[(int64_t)seq * a.q_heads + h] = top == INFINITY ? top : base + logf(sum);
 }
 
 
@@ -111,7 +166,18 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(AttnArgs a) {
 // (exactly), two f16 (to 2^-23, scaled by a power of two into f16's range) --
 // and each limb gets its product.  The cached values are exact operands as they
 // are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
-// against the 16 KB that a SIMD's share of the memory takes 5000 cycles for.
+// against the 16 KB that a SIMD's share of the memory takes 7400 cycles for.
+//
+// Q8_0 codes become f16 exactly; a block's scale goes with its partial scores
+// (they leave the matrix unit per block) and, for V, with P before the limbs.
+//
+// What bounds it: memory, once the cache is long (131072 tokens of 8 key/value
+// heads of 128, bf16, 537 MB: 97 us, 5.5 TB/s; 64 ragged sequences of at most
+// 8192, 268 MB: 54 us, 5.0 TB/s); Q8_0 the vector instructions of its decoding
+// and the first-level cache, which serves its rows in pieces of 2 and 8 bytes
+// (131072 tokens, 285 MB: 68 us, 4.2 TB/s); a short cache the chain length ->
+// page -> row -> result -> count -> join, each a trip to memory (517 tokens,
+// 2 MB: 8.2 us).
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -934,6 +1000,17 @@ void launch_tiles(const TileArgs &ta, dim3 grid, hipStream_t s) {
   else launch_tiles<kType, 8>(ta, grid, s);
 }
 
+template <int kType>
+void launch_rows(const AttnArgs &a, hipStream_t s) {
+  const int sets = (a.group + kRowHeads - 1) / kRowHeads;
+  auto run = [&](auto kernel, int waves) {
+    launch_timed(kernel, dim3((unsigned)(a.seqs * a.cache.kv_heads * sets)), dim3(64 * waves), 0u, s, a, sets);
+  };
+  if (a.cache.head_dim <= 128) run(attention_rows_kernel<kType, 2>, row_waves(2));
+  else if (a.cache.head_dim <= 256) run(attention_rows_kernel<kType, 4>, row_waves(4));
+  else run(attention_rows_kernel<kType, 8>, row_waves(8));
+}
+
 }  // namespace
 
 AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
@@ -947,7 +1024,10 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   if (!p.tiles) return p;
   const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
-  const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;  // workgroups that run at once
+  // workgroups that run at once: above head_dim 128 a wave takes more than half
+  // of a SIMD's registers (held to half, 4 sequences of 14563 tokens of Q8_0 and
+  // head_dim 256 take 49.8 us for 33.8)
+  const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;
   // All chunks (units + seqs a head at most) at once where the sequences leave
   // room for that.  Where they do not, the card is full without a split, which
   // then only evens its end: twice as many units, but none of fewer than four
@@ -969,7 +1049,10 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
 
 hipError_t launch_attention(const AttnArgs &a, const AttnPlan &p, void *part, void *arrived, hipStream_t s) {
   if (!p.tiles) {
-    launch_timed(attention_rows_kernel, dim3((unsigned)(a.seqs * a.q_heads)), dim3(256), 0u, s, a);
+    if (a.cache.type == kF32) launch_rows<kF32>(a, s);
+    else if (a.cache.type == kF16) launch_rows<kF16>(a, s);
+    else if (a.cache.type == kBF16) launch_rows<kBF16>(a, s);
+    else launch_rows<kQ8_0>(a, s);
     return hipGetLastError();
   }
   // token / page_tokens for tokens below 2^31: floor(2^(31 + n) / d) + 1 with

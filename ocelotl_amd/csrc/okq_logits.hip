@@ -81,7 +81,9 @@ __device__ __forceinline__ void choose(const LogitsArgs &a, int row, int slices,
 // gathered in LDS: counts, whose order does not matter, by integer atomics;
 // biases by the thread that holds a token's first entry, in list order.  The
 // workgroup that ends last on a row turns the largest key into the token.
-// Memory bounds it: the logits are read and written once.
+// Memory bounds it: the logits are read and written once (200 rows of 262144
+// with a mask, 426 MB: 85 us, 5.0 TB/s); a single row the chain logits or lists
+// -> LDS -> result -> meeting place (128256 entries, 1 MB: 5.7 us).
 template <int V, bool kMarks, int kBias>  // a history; biases (with marks): 1 a list of kThreads at most, 2 a longer one
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slices, Meeting *meet) {
   constexpr int kSlice = 4 * kThreads * V, kWaves = kThreads / 64;

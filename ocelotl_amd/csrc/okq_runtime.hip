@@ -1244,7 +1244,7 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   if (seqs < 0 || q_heads < 1 || q_heads % cache->kv_heads != 0)
     return fail(OKQ_E_SHAPE, "%s seqs=%lld q_heads=%lld: q_heads must be a positive multiple of kv_heads=%lld", what,
                 (long long)seqs, (long long)q_heads, (long long)cache->kv_heads);
-  if (!mul_ok(seqs, q_heads, rows) || rows > (1 << 22))  // workgroups of up to 512 threads
+  if (!mul_ok(seqs, q_heads, rows) || rows >= (1 << 22))  // workgroups of up to 1024 threads
     return fail(OKQ_E_SHAPE, "%s seqs*q_heads exceeds u32 launch limits", what);
   if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > 1 << 30)
     return fail(OKQ_E_SHAPE, "%s table_width=%lld max_length=%lld window=%lld must not be negative nor exceed 32 bits",
