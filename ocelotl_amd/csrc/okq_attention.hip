@@ -8,7 +8,7 @@
 // long cache split over workgroups and joined by the last of them.
 // attention_rows_kernel: rows that the tiles' vector loads do not reach
 // (head_dim or addresses that are no multiple of 16 bytes, head_dim above
-// 256), one value at a time.
+// 256), one value at a time; a split sequence is joined by a launch of its own.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,17 +33,24 @@ __device__ __forceinline__ float cached(const uint8_t *row, int i) {
 constexpr int kRowHeads = 4, kRowTokens = 4;
 // As many waves as the registers of a row allow: one workgroup has all tokens.
 constexpr int row_waves(int kV) { return kV <= 4 ? 16 : 8; }
+// Where a chunk's results for a head begin: outputs, maximum, sum.
+__device__ __forceinline__ int64_t row_part(unsigned block, int chunks, unsigned chunk, int h, int D) {
+  return (((int64_t)block * chunks + chunk) * kRowHeads + h) * (D + 2);
+}
 
 }  // namespace
 
-// One workgroup per sequence and kRowHeads query heads of a key/value head,
-// which share its rows; its waves take kRowTokens tokens each in turn, a wave's
-// lanes the row's values.  Any head_dim up to 64 kV, any alignment.  The waits
-// for pages and rows bound it, so a wave asks for all its tokens' rows at once
-// (16 sequences of 2000 tokens, 32 heads over 8, bf16: head_dim 512 282 us,
-// 100 170; token by token, four waves and a workgroup a head, 3986 and 928).
+// A workgroup per sequence, kRowHeads query heads of a key/value head, which
+// share its rows, and chunk of the sequence; its waves take kRowTokens tokens
+// each in turn, a wave's lanes the row's values.  Any head_dim up to 64 kV, any
+// alignment.  The waits for pages and rows bound it, so a wave asks for all its
+// tokens' rows at once, and sequences are split, each into the same number of
+// equal chunks, until there are two workgroups a CU (16 sequences of 2000
+// tokens, 32 heads over 8, bf16: head_dim 512 170 us, 100 109; unsplit 282 and
+// 170; token by token, a workgroup of four waves a head, 3986 and 928).  A
+// chunk's outputs, maxima and sums go to `part`.
 template <int kType, int kV>
-__global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(AttnArgs a, int sets) {
+__global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(AttnArgs a, int sets, float *part) {
   constexpr int kRowWaves = row_waves(kV);
   __shared__ float lds[kRowWaves][kRowHeads][64 * kV + 2];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
@@ -68,7 +75,14 @@ __global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(Attn
   }
   int len = a.lengths[seq];
   len = len < a.max_len ? len : a.max_len;
-  const int lo = a.window && len > a.window ? len - a.window : 0;
+  int lo = a.window && len > a.window ? len - a.window : 0;
+  const int chunks = (int)gridDim.y;
+  if (len > lo) {
+    constexpr int kTurn = kRowWaves * kRowTokens;
+    const int per = ((len - lo + kTurn - 1) / kTurn + chunks - 1) / chunks * kTurn;
+    lo += per * (int)blockIdx.y;
+    len = len - lo < per ? len : lo + per;  // may leave nothing
+  }
   for (int t0 = lo + wave * kRowTokens; t0 < len; t0 += kRowWaves * kRowTokens) {
     bool seen[kRowTokens];
     float k[kRowTokens][kV], v[kRowTokens][kV];
@@ -139,10 +153,47 @@ __global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(Attn
       float x = 0.0f;
 #pragma unroll
       for (int w = 0; w < kRowWaves; ++w) x += lds[w][h][i] * weight[w];
-      a.out[seq * a.out_stride + (h0 + h) * D + i] = sum == 0.0f ? 0.0f : x / sum;
+      if (chunks == 1) a.out[seq * a.out_stride + (h0 + h) * D + i] = sum == 0.0f ? 0.0f : x / sum;
+      else part[row_part(blockIdx.x, chunks, blockIdx.y, h, D) + i] = x;
     }
-    if (a.lse && threadIdx.x == 0) a.lse[(int64_t)seq * a.q_heads + h0 + h] = top == INFINITY ? top : base + logf(sum);
+    if (threadIdx.x == 0) {
+      if (chunks > 1) {
+        part[row_part(blockIdx.x, chunks, blockIdx.y, h, D) + D] = top;
+        part[row_part(blockIdx.x, chunks, blockIdx.y, h, D) + D + 1] = sum;
+      } else if (a.lse) {
+        a.lse[(int64_t)seq * a.q_heads + h0 + h] = top == INFINITY ? top : base + logf(sum);
+      }
+    }
   }
+}
+
+// The chunks' results into one, in their order: a workgroup per first kernel's
+// workgroup of a sequence and head.
+__global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, int sets, int chunks, const float *part) {
+  const int set = (int)(blockIdx.x % (unsigned)sets), pair = (int)(blockIdx.x / (unsigned)sets), h = (int)blockIdx.y;
+  const int seq = pair / a.cache.kv_heads, kvh = pair - seq * a.cache.kv_heads, D = a.cache.head_dim;
+  if (set * kRowHeads + h >= a.group) return;
+  const int64_t head = (int64_t)kvh * a.group + set * kRowHeads + h;
+  part += row_part(blockIdx.x, chunks, 0, h, D);
+  const int64_t step = (int64_t)kRowHeads * (D + 2);
+  float top = -INFINITY, sum = 0.0f, x[kMaxHeadDim / 256] = {};
+  for (int c = 0; c < chunks; ++c) top = fmaxf(top, part[c * step + D]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  for (int c = 0; c < chunks; ++c) {
+    const float weight = expf(part[c * step + D] - base);
+    sum += part[c * step + D + 1] * weight;
+#pragma unroll
+    for (int j = 0; j < kMaxHeadDim / 256; ++j) {
+      const int i = (int)threadIdx.x + 256 * j;
+      if (i < D) x[j] += part[c * step + i] * weight;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kMaxHeadDim / 256; ++j) {
+    const int i = (int)threadIdx.x + 256 * j;
+    if (i < D) a.out[seq * a.out_stride + head * D + i] = sum == 0.0f ? 0.0f : x[j] / sum;
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[(int64_t)seq * a.q_heads + head] = top == INFINITY ? top : base + logf(sum);
 }
 
 
@@ -1001,14 +1052,16 @@ void launch_tiles(const TileArgs &ta, dim3 grid, hipStream_t s) {
 }
 
 template <int kType>
-void launch_rows(const AttnArgs &a, hipStream_t s) {
+void launch_rows(const AttnArgs &a, int chunks, float *part, hipStream_t s) {
   const int sets = (a.group + kRowHeads - 1) / kRowHeads;
+  const unsigned pairs = (unsigned)(a.seqs * a.cache.kv_heads * sets);
   auto run = [&](auto kernel, int waves) {
-    launch_timed(kernel, dim3((unsigned)(a.seqs * a.cache.kv_heads * sets)), dim3(64 * waves), 0u, s, a, sets);
+    launch_timed(kernel, dim3(pairs, (unsigned)chunks), dim3(64 * waves), 0u, s, a, sets, part);
   };
   if (a.cache.head_dim <= 128) run(attention_rows_kernel<kType, 2>, row_waves(2));
   else if (a.cache.head_dim <= 256) run(attention_rows_kernel<kType, 4>, row_waves(4));
   else run(attention_rows_kernel<kType, 8>, row_waves(8));
+  if (chunks > 1) launch_timed(attention_rows_join_kernel, dim3(pairs, kRowHeads), dim3(256), 0u, s, a, sets, chunks, (const float *)part);
 }
 
 }  // namespace
@@ -1021,7 +1074,14 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   const uint64_t page = (uint64_t)c.token_stride * (uint64_t)c.page_tokens;  // 32-bit offsets within a page
   p.tiles = c.head_dim <= 256 && c.token_stride < (1ll << 32) && page < (1ull << 32) &&
             (c.type == kQ8_0 || (aligned && c.head_dim % (c.type == kF32 ? 4 : 8) == 0));
-  if (!p.tiles) return p;
+  if (!p.tiles) {
+    // chunks of four turns of a workgroup's waves at least
+    const int64_t pairs = (int64_t)a.seqs * c.kv_heads * ((a.group + kRowHeads - 1) / kRowHeads), most = 2 * (int64_t)cu_count;
+    const int64_t turn = row_waves(c.head_dim <= 256 ? 4 : 8) * kRowTokens;
+    p.units = (int)std::max<int64_t>(1, std::min(most / pairs, a.max_len / (4 * turn)));
+    if (p.units > 1) p.part_bytes = (size_t)(most * kRowHeads * (c.head_dim + 2)) * sizeof(float);
+    return p;
+  }
   const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
   const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
   // workgroups that run at once: above head_dim 128 a wave takes more than half
@@ -1049,10 +1109,11 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
 
 hipError_t launch_attention(const AttnArgs &a, const AttnPlan &p, void *part, void *arrived, hipStream_t s) {
   if (!p.tiles) {
-    if (a.cache.type == kF32) launch_rows<kF32>(a, s);
-    else if (a.cache.type == kF16) launch_rows<kF16>(a, s);
-    else if (a.cache.type == kBF16) launch_rows<kBF16>(a, s);
-    else launch_rows<kQ8_0>(a, s);
+    float *rows = static_cast<float *>(part);
+    if (a.cache.type == kF32) launch_rows<kF32>(a, p.units, rows, s);
+    else if (a.cache.type == kF16) launch_rows<kF16>(a, p.units, rows, s);
+    else if (a.cache.type == kBF16) launch_rows<kBF16>(a, p.units, rows, s);
+    else launch_rows<kQ8_0>(a, p.units, rows, s);
     return hipGetLastError();
   }
   // token / page_tokens for tokens below 2^31: floor(2^(31 + n) / d) + 1 with

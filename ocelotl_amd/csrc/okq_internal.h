@@ -259,8 +259,8 @@ struct AttnArgs {
 // How a call runs, and the workspace that it takes: chunks' results, and
 // counters that are zero before and after every call.
 struct AttnPlan {
-  bool tiles;  // else one value at a time, without workspace
-  int units, min_tiles;
+  bool tiles;  // else one value at a time
+  int units, min_tiles;  // one value at a time: units chunks a sequence
   int64_t grid;  // chunks, at most
   size_t part_bytes, arrived_bytes;
 };

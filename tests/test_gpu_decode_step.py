@@ -740,3 +740,19 @@ def test_logits_of_long_lists(torch, okq, rows, vocab, hist, biases, masked, dup
     d = _logits_inputs(torch, rows, vocab, hist, biases, masked, 11 + vocab, duplicates)
     got, best = _logits(torch, okq, d, hist, biases, masked, inplace=rows == 2)
     _logits_check(got, best, d, True, masked)
+
+
+@pytest.mark.parametrize("tn,d,kv,group,page,lengths,window,softcap", [
+    ("BF16", 512, 1, 5, 16, [9001, 0, 40], 0, 0.0), ("F16", 100, 2, 1, 24, [12000], 5000, 30.0),
+    ("F32", 33, 1, 3, 7, [7001, 1, 256, 257, 4000], 0, 0.0), ("Q8_0", 288, 2, 4, 32, [3000, 129], 0, 0.0),
+    ("BF16", 260, 8, 9, 16, [300, 700], 0, 0.0), ("F32", 1, 1, 1, 64, [50000], 0, 0.0)])
+def test_attention_of_odd_heads_over_long_caches(torch, okq, tn, d, kv, group, page, lengths, window, softcap):
+    """Rows that are read one value at a time, split; two calls agree bit for bit."""
+    print(f"[gpu] attention odd long {tn} {d} {lengths[:3]}", flush=True)
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], d, kv, group, page, lengths)
+    table[0, 3] = -1
+    got = [_attention(torch, okq, cache, table, q, lengths, max(lengths), d ** -0.5, softcap, window) for _ in range(2)]
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+    _attn_check(torch, got[0], _attn_want(torch, cache, table, q, lengths, d ** -0.5, softcap, window, group))
