@@ -1079,7 +1079,8 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
     const int64_t pairs = (int64_t)a.seqs * c.kv_heads * ((a.group + kRowHeads - 1) / kRowHeads), most = 2 * (int64_t)cu_count;
     const int64_t turn = row_waves(c.head_dim <= 256 ? 4 : 8) * kRowTokens;
     p.units = (int)std::max<int64_t>(1, std::min(most / pairs, a.max_len / (4 * turn)));
-    if (p.units > 1) p.part_bytes = (size_t)(most * kRowHeads * (c.head_dim + 2)) * sizeof(float);
+    p.splits = p.units > 1;
+    p.part_bytes = (size_t)(most * kRowHeads * (c.head_dim + 2)) * sizeof(float);
     return p;
   }
   const int tile = c.type == kF32 ? 16 : 32, head_tiles = (a.group + kHeads - 1) / kHeads;
@@ -1097,9 +1098,9 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   p.units = (int)std::max<int64_t>(1, room ? units - a.seqs : 2 * units);
   p.min_tiles = room ? kWaves : 4 * kWaves;
   const int64_t chunks = std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles);
-  const bool splits = chunks > 1 && p.units > 1;  // one unit: every sequence is one chunk
-  p.grid = splits ? std::min<int64_t>(a.seqs + p.units + 1, a.seqs * chunks) : a.seqs;
-  if (splits) {  // the same for every call of these heads: slots for the most units
+  p.splits = chunks > 1 && p.units > 1;  // one unit: every sequence is one chunk
+  p.grid = p.splits ? std::min<int64_t>(a.seqs + p.units + 1, a.seqs * chunks) : a.seqs;
+  if (units >= 1) {  // the same for every call of these heads: slots for the most units
     const size_t slots = (size_t)(2 * (2 * units + 1) * pairs);
     p.arrived_bytes = slots * sizeof(uint32_t);
     p.part_bytes = slots * (size_t)((std::min(a.group, kHeads) * (c.head_dim + 2) + 3) / 4 * 4) * sizeof(float);

@@ -256,10 +256,13 @@ struct AttnArgs {
   float *out, *lse;
   KvPages cache;
 };
-// How a call runs, and the workspace that it takes: chunks' results, and
-// counters that are zero before and after every call.
+// How a call runs, and the workspace: chunks' results, and counters that are
+// zero before and after every call.  It is the same for all calls of the same
+// heads, and a call that splits nothing asks for it too (and goes on without),
+// so that any first call makes room for a captured one.
 struct AttnPlan {
-  bool tiles;  // else one value at a time
+  bool tiles;   // else one value at a time
+  bool splits;
   int units, min_tiles;  // one value at a time: units chunks a sequence
   int64_t grid;  // chunks, at most
   size_t part_bytes, arrived_bytes;

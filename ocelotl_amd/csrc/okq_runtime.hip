@@ -1289,7 +1289,7 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   if (plan.part_bytes) {
     st = get_workspace(dev, s, plan.part_bytes, &part, 3);
     if (st == OKQ_OK && plan.arrived_bytes) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 4);
-    if (st != OKQ_OK) return st;
+    if (st != OKQ_OK && plan.splits) return st;
   }
   return hip_status(okq::launch_attention(a, plan, part, arrived, s), "paged_attention launch");
 }

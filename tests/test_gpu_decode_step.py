@@ -756,3 +756,30 @@ def test_attention_of_odd_heads_over_long_caches(torch, okq, tn, d, kv, group, p
     for a, b in zip(*got):
         assert torch.equal(a.view(torch.int32), b.view(torch.int32))
     _attn_check(torch, got[0], _attn_want(torch, cache, table, q, lengths, d ** -0.5, softcap, window, group))
+
+
+@pytest.mark.parametrize("tn,d", [("BF16", 64), ("F32", 50)])
+def test_attention_captured_after_a_call_of_other_sequences(torch, okq, tn, d):
+    """Many short sequences, which nothing splits, then one long one in a graph
+    on the same stream."""
+    s = torch.cuda.Stream()
+    short, st, sq = _attn_inputs(torch, okq, TYPES[tn], d, 2, 2, 16, [9] * 700)
+    long, lt, lq = _attn_inputs(torch, okq, TYPES[tn], d, 2, 2, 16, [4000])
+    td, ld = lt.cuda(), torch.tensor([4000], dtype=torch.int32, device="cuda")
+    out, lse = torch.empty_like(lq), torch.empty(1, 4, device="cuda")
+    torch.cuda.synchronize()
+    got = _attention(torch, okq, short, st, sq, [9] * 700, 16, 0.125, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    _attn_check(torch, got, _attn_want(torch, short, st, sq, [9] * 700, 0.125, 0.0, 0, 2))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        okq.call("okq_paged_attention", lq.data_ptr(), 4 * d, 1, 4, long.ref(), td.data_ptr(), td.shape[1],
+                 ld.data_ptr(), 4000, 0.125, 0.0, 0, out.data_ptr(), 4 * d, lse.data_ptr(),
+                 torch.cuda.current_stream().cuda_stream)
+    want = _attn_want(torch, long, lt, lq, [4000], 0.125, 0.0, 0, 2)
+    for _ in range(3):
+        out.fill_(math.nan)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        _attn_check(torch, (out, lse), want)
