@@ -305,7 +305,7 @@ typedef struct okq_kv_pages {
  * rows at slots[token] (int64; a slot outside the cache, -1 say, stores
  * nothing), or cache NULL (then v and slots are not read).  Keys and values
  * are rounded to the cache's type, to nearest even; Q8_0 blocks are
- * okq_quantize's bytes.  Tokens that share a slot leave either one's row.
+ * okq_quantize's bytes.  Tokens that share a slot race: its row may mix theirs.
  * tokens == 0 is a no-op.  The rotation follows crates/kernels/src/rope.rs
  * (its pairs are the halves); no counterpart in the reference fuses the three. */
 okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
@@ -330,8 +330,9 @@ okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, in
  * exp(f(scale * q . K)).  A sequence with nothing to see (length 0, hidden pages)
  * gets zeros and lse -inf; tokens outside the length or the window may hold
  * anything, NaN too; a visible infinity or NaN leaves no finite number in what
- * it reaches (a key: its heads' lse; a value: its column of out).  Products and sums are f32 on the cached values; a row's
- * result depends on the call's shape and lengths only, not on timing.
+ * it reaches (a key: its heads' lse; a value: its column of out).  Products and
+ * sums are f32 on the cached values; a row's result depends on the call's shape
+ * and lengths only, not on timing.
  * seqs == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
  * reference, whose attention is on contiguous host rows
  * (crates/kernels/src/attention.rs). */
