@@ -224,9 +224,9 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 //
 // What bounds it: memory, once the cache is long (131072 tokens of 8 key/value
 // heads of 128, bf16, 537 MB: 97 us, 5.5 TB/s; 64 ragged sequences of at most
-// 8192, 268 MB: 54 us, 5.0 TB/s); Q8_0 the vector instructions of its decoding
-// and the first-level cache, which serves its rows in pieces of 2 and 8 bytes
-// (131072 tokens, 285 MB: 68 us, 4.2 TB/s); a short cache the chain length ->
+// 8192, 268 MB: 54 us, 5.0 TB/s); Q8_0 what two waves a SIMD have in flight, as
+// its rows come in pieces of 2 and 8 bytes, beside the instructions that decode
+// them (131072 tokens, 285 MB: 68 us, 4.2 TB/s); a short cache the chain length ->
 // page -> row -> result -> count -> join, each a trip to memory (517 tokens,
 // 2 MB: 8.2 us).
 
