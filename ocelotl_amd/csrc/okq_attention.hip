@@ -215,8 +215,13 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 // The queries and probabilities are f32, the matrix instructions' operands 16
 // bits: each is split into limbs whose sum is the f32 value -- three bf16
 // (exactly), two f16 (to 2^-23, scaled by a power of two into f16's range) --
-// and each limb gets its product.  The cached values are exact operands as they
-// are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
+// and each limb gets its product.  Over F16 caches the second limb has a scale
+// of its own, so do the weights of a tile and head, and those too small for it
+// go in by themselves: a weight keeps its precision however far it lies below
+// the largest (a token whose value is near zero may have that one).  The price
+// is a sum per limb, added to O in f32: 24 sequences, window 1024, head_dim
+// 256, 14.6 us (13.8 with limbs of one scale), 517 tokens 8.3 (7.8), 131072
+// tokens 99.2 (98.6).  The cached values are exact operands as they are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
 // against the 16 KB that a SIMD's share of the memory takes 7400 cycles for.
 //
 // Q8_0 codes become f16 exactly; a block's scale goes with its partial scores
@@ -327,6 +332,21 @@ __device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2])
     // step of f16 that neither limb holds
     asm("" : "+v"(hi));
     const f16x2 lo = {(_Float16)(x[2 * j] - (float)hi[0]), (_Float16)(x[2 * j + 1] - (float)hi[1])};
+    limb[0][j] = __builtin_bit_cast(uint32_t, hi);
+    limb[1][j] = __builtin_bit_cast(uint32_t, lo);
+  }
+}
+// Eight f32 values below 2^14 as two f16 limbs, the second 2^11 times its
+// worth, so that it has a range of its own: off by at most 2^-23 of the value
+// from kLeast on, by 2^-36 below.  (A query's largest element is 2^13 to 2^14
+// here: what is 2^26 times smaller is off by 2^-49 of the largest.)
+constexpr float kApart = 2048.0f, kLeast = 0x1p-13f;
+__device__ __forceinline__ void limbs_f16_apart(const float (&x)[8], u32x4 (&limb)[2]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
+    asm("" : "+v"(hi));  // one rounding for both uses
+    const f16x2 lo = {(_Float16)((x[2 * j] - (float)hi[0]) * kApart), (_Float16)((x[2 * j + 1] - (float)hi[1]) * kApart)};
     limb[0][j] = __builtin_bit_cast(uint32_t, hi);
     limb[1][j] = __builtin_bit_cast(uint32_t, lo);
   }
@@ -657,6 +677,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
         u32x4 limb[kL];
         if constexpr (kF) limb[0] = u32x4{as_u32(x[u][0]), as_u32(x[u][1]), as_u32(x[u][2]), as_u32(x[u][3])};
         else if constexpr (kType == kBF16) limbs_bf16(x[u], limb);
+        else if constexpr (kType == kF16) limbs_f16_apart(x[u], limb);
         else limbs_f16(x[u], limb);
 #pragma unroll
         for (int k = 0; k < kL; ++k) {
@@ -734,7 +755,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
         for (int s = 0; s < kSub; ++s) {
           f32x4 acc = part[s][kAcc - 1];
 #pragma unroll
-          for (int k = kAcc - 2; k >= 0; --k) acc += part[s][k];
+          for (int k = kAcc - 2; k >= 0; --k) acc = kType == kF16 ? acc * (1.0f / kApart) + part[s][k] : acc + part[s][k];
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[4 * s + i] = acc[i];
         }
@@ -767,6 +788,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
       for (int j = 1; j < kSlots; ++j) top = __builtin_fmaxf(top, p[j]);
       top = cross_max(top);
+      const float tile_top = top;
       bool grown = __ballot(top > m + kGrowth) != 0;
       int d_new = d_exp;
       if constexpr (kQ) {
@@ -846,31 +868,85 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
-        u32x4 limb[kL];
-        if constexpr (kType == kBF16) {
-          limbs_bf16(p, limb);
-        } else {
+        // Two f16 limbs hold a weight that is at least kLeast, so F16's weights
+        // go in scaled by a power of two, their tile's and head's own (the
+        // largest is 2^13 to 2^14), and what is still smaller, 26 powers of two
+        // below its tile's largest, waits for another turn: a weight is off by
+        // 2^-23 of itself, however far below the largest it is.
+        float x[kSlots], down = 1.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) p[j] *= 64.0f;
-          limbs_f16(p, limb);
+        for (int j = 0; j < kSlots; ++j) x[j] = p[j];
+        if constexpr (kType == kF16) {
+          const int e = 13 - (int)__builtin_floorf(__builtin_fmaxf(tile_top - base, -100.0f));
+          const float up = ldexpf(1.0f, e);
+          down = ldexpf(1.0f, -e);
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) x[j] *= up;
         }
+        for (;;) {
+          float later[kSlots];
+          bool again = false;
+          if constexpr (kType == kF16) {
+            uint32_t least = ~0u;  // zeros and NaN do not count
 #pragma unroll
-        for (int v = 0; v < kVG; ++v)
+            for (int j = 0; j < kSlots; ++j) least = min(least, as_u32(x[j]) - 1u);
+            again = __ballot(least < as_u32(kLeast) - 1u) != 0;
+            if (again) {
 #pragma unroll
-          for (int d0 = 0; d0 < kVD; d0 += 4) {
-            u32x4 op[4];
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t lower = vr[2 * j][v][(d0 + d) / 2], upper = vr[2 * j + 1][v][(d0 + d) / 2];
-                op[d][j] = d & 1 ? hi16s(lower, upper) : lo16s(lower, upper);
+              for (int j = 0; j < kSlots; ++j) {
+                const bool small = x[j] < kLeast;
+                later[j] = small ? x[j] * 0x1p26f : 0.0f;
+                x[j] = small ? 0.0f : x[j];
               }
-#pragma unroll
-            for (int k = 0; k < kL; ++k)
-#pragma unroll
-              for (int d = 0; d < 4; ++d) o[v * kVD + d0 + d] = mfma<kType>(op[d], limb[k], o[v * kVD + d0 + d]);
+            }
           }
+          u32x4 limb[kL];
+          if constexpr (kType == kBF16) limbs_bf16(x, limb);
+          else limbs_f16_apart(x, limb);
+#pragma unroll
+          for (int v = 0; v < kVG; ++v)
+#pragma unroll
+            for (int d0 = 0; d0 < kVD; d0 += 4) {
+              // not turned for all turns at once, before the loop: too many registers
+              if constexpr (kType == kF16) {
+#pragma unroll
+                for (int j = 0; j < kSlots; ++j) {
+                  asm volatile("" : "+v"(vr[j][v][d0 / 2]));
+                  asm volatile("" : "+v"(vr[j][v][d0 / 2 + 1]));
+                }
+              }
+              u32x4 op[4];
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const uint32_t lower = vr[2 * j][v][(d0 + d) / 2], upper = vr[2 * j + 1][v][(d0 + d) / 2];
+                  op[d][j] = d & 1 ? hi16s(lower, upper) : lo16s(lower, upper);
+                }
+              f32x4 *acc = o + v * kVD + d0;
+              if constexpr (kType == kBF16) {
+#pragma unroll
+                for (int k = 0; k < kL; ++k)
+#pragma unroll
+                  for (int d = 0; d < 4; ++d) acc[d] = mfma<kType>(op[d], limb[k], acc[d]);
+              } else {
+                f32x4 t[kL][4];
+#pragma unroll
+                for (int k = 0; k < kL; ++k)
+#pragma unroll
+                  for (int d = 0; d < 4; ++d) t[k][d] = mfma<kType>(op[d], limb[k], f32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    acc[d][i] = __builtin_fmaf(t[0][d][i], down, __builtin_fmaf(t[1][d][i], down * (1.0f / kApart), acc[d][i]));
+              }
+            }
+          if (!again) break;
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) x[j] = later[j];
+          down *= 0x1p-26f;
+        }
       }
       if (!more) break;
       buf ^= 1;
@@ -888,7 +964,6 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
   }
   float f = 1.0f;
   if constexpr (kQ) f = ldexpf(1.0f, d_exp - 6);
-  else if constexpr (kType == kF16) f = 1.0f / 64.0f;
   const int DS = D + 4, fit = kMergeFloats / (kWaves * DS);  // heads that fit at once
   const int slot_floats = ((a.group < kHeads ? a.group : kHeads) * (D + 2) + 3) / 4 * 4;
   const auto part = __builtin_amdgcn_make_buffer_rsrc(ta.part, 0, (int)ta.part_bytes, 0x00020000);

@@ -783,3 +783,66 @@ def test_attention_captured_after_a_call_of_other_sequences(torch, okq, tn, d):
         g.replay()
         torch.cuda.synchronize()
         _attn_check(torch, (out, lse), want)
+
+
+# ---- weights, queries and scales of very different sizes --------------------------------
+
+def _written_cache(torch, okq, tn, d, kv, page, K, V):
+    """A cache whose sequences hold the rows of K and V: lists of f32 [tokens, kv, d]."""
+    lengths = [k.shape[0] for k in K]
+    cache, table, _ = _attn_inputs(torch, okq, TYPES[tn], d, kv, 1, page, lengths)
+    for i, rows in enumerate(zip(K, V)):
+        for t in range(0, lengths[i], page):
+            p = int(table[i, t // page])
+            for view, r in zip(cache.views, rows):
+                r = r[t:t + page].transpose(0, 1).contiguous().cuda()
+                view[p, :, :r.shape[1]] = _encode(torch, okq, TYPES[tn], r)
+    return cache, table, lengths
+
+
+def _parked(torch, d, kv, n, gap, seed):
+    """n tokens of which the first is `gap` nats above all others (a query of
+    8 in dim 0 and 1 in dim 1) and has a value of zeros."""
+    g = torch.Generator().manual_seed(seed)
+    k, v = torch.zeros(n, kv, d), torch.randn(n, kv, d, generator=g)
+    k[:, :, 1] = torch.rand(n, kv, generator=g) - 0.5
+    k[0, :, 0], k[0, :, 1], v[0] = gap / 8, 0.0, 0.0
+    return k, v
+
+
+@pytest.mark.parametrize("gap", [8, 13, 17, 22, 40])
+@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("F16", 80), ("BF16", 128), ("F32", 128),
+                                  ("F16", 100)])
+def test_attention_keeps_the_weights_below_a_token_whose_value_is_zero(torch, okq, tn, d, gap):
+    """The output is what the small weights make it, and each of them is off by
+    2e + 8u of itself, however far below the largest: tokens of the heavy one's
+    tile, of its wave's later tiles and of other chunks."""
+    print(f"[gpu] parked {tn} {d} {gap}", flush=True)
+    for kv, sizes in ((2, [20, 128, 2000]), (1, [5000]), (4, [400] * 70)):
+        kvs = [_parked(torch, d, kv, n, gap, 3 + n + i) for i, n in enumerate(sizes)]
+        cache, table, lengths = _written_cache(torch, okq, tn, d, kv, 16, [k for k, _ in kvs], [v for _, v in kvs])
+        q = torch.zeros(len(sizes), kv, d, device="cuda")
+        q[:, :, 0], q[:, :, 1] = 8.0, 1.0
+        got = _attention(torch, okq, cache, table, q, lengths, max(lengths), 1.0)
+        torch.cuda.synchronize()
+        _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 1))
+
+
+@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("BF16", 128), ("F32", 128)])
+def test_attention_keeps_the_small_elements_of_a_query(torch, okq, tn, d):
+    """A query whose first element is 2^26 times the others, which meet large
+    keys: scores of about 1 that the large element has no part in."""
+    print(f"[gpu] small query elements {tn} {d}", flush=True)
+    g = torch.Generator().manual_seed(17)
+    K, V = [], []
+    for n in (3, 50):
+        k = torch.randn(n, 2, d, generator=g) * 2.0 ** 13
+        k[:, :, 0:32] = 0.0
+        K.append(k.clamp(-60000, 60000))
+        V.append(torch.randn(n, 2, d, generator=g))
+    cache, table, lengths = _written_cache(torch, okq, tn, d, 2, 16, K, V)
+    q = torch.randn(2, 2, d, generator=g).cuda() * 2.0 ** -16
+    q[:, :, 0] = 2.0 ** 10
+    got = _attention(torch, okq, cache, table, q, lengths, 50, 1.0)
+    torch.cuda.synchronize()
+    _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 1))
