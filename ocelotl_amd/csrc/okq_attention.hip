@@ -214,7 +214,8 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 //
 // The queries and probabilities are f32, the matrix instructions' operands 16
 // bits: each is split into limbs whose sum is the f32 value -- three bf16
-// (exactly), two f16 (to 2^-23, scaled by a power of two into f16's range) --
+// (exactly; BF16 and Q8_0 caches), two f16 (to 2^-23, scaled by a power of two
+// into f16's range; F16 caches) --
 // and each limb gets its product.  Over F16 caches the second limb has a scale
 // of its own, so do the weights of a tile and head, and those too small for it
 // go in by themselves: a weight keeps its precision however far it lies below
@@ -224,14 +225,17 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 // tokens 99.2 (98.6).  The cached values are exact operands as they are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
 // against the 16 KB that a SIMD's share of the memory takes 7400 cycles for.
 //
-// Q8_0 codes become f16 exactly; a block's scale goes with its partial scores
-// (they leave the matrix unit per block) and, for V, with P before the limbs.
+// Q8_0 codes become bf16 exactly; a block's scale goes with its partial scores
+// (they leave the matrix unit per block) and, for V, with P before the limbs:
+// bf16 limbs have f32's range, so neither weights nor scales far below others
+// lose bits.
 //
 // What bounds it: memory, once the cache is long (131072 tokens of 8 key/value
 // heads of 128, bf16, 537 MB: 97 us, 5.5 TB/s; 64 ragged sequences of at most
 // 8192, 268 MB: 54 us, 5.0 TB/s); Q8_0 what two waves a SIMD have in flight, as
 // its rows come in pieces of 2 and 8 bytes, beside the instructions that decode
-// them (131072 tokens, 285 MB: 68 us, 4.2 TB/s); a short cache the chain length ->
+// them and split the weights block by block (131072 tokens, 285 MB: 75 us, 3.8
+// TB/s; 68 with two f16 limbs, which lose small weights); a short cache the chain length ->
 // page -> row -> result -> count -> join, each a trip to memory (517 tokens,
 // 2 MB: 8.2 us).
 
@@ -321,27 +325,12 @@ __device__ __forceinline__ void limbs_bf16(const float (&x)[8], u32x4 (&limb)[3]
     }
   }
 }
-// Eight f32 values below 2^15 as two f16 limbs, off by at most 2^-23 of the
-// value (2^-25 for what lies below f16's normal range).
-__device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
-    // one rounding for both uses: where x is a product, the compiler may round
-    // it to f16 in one step here and in two there, and a tie apart is a whole
-    // step of f16 that neither limb holds
-    asm("" : "+v"(hi));
-    const f16x2 lo = {(_Float16)(x[2 * j] - (float)hi[0]), (_Float16)(x[2 * j + 1] - (float)hi[1])};
-    limb[0][j] = __builtin_bit_cast(uint32_t, hi);
-    limb[1][j] = __builtin_bit_cast(uint32_t, lo);
-  }
-}
 // Eight f32 values below 2^14 as two f16 limbs, the second 2^11 times its
 // worth, so that it has a range of its own: off by at most 2^-23 of the value
 // from kLeast on, by 2^-36 below.  (A query's largest element is 2^13 to 2^14
 // here: what is 2^26 times smaller is off by 2^-49 of the largest.)
 constexpr float kApart = 2048.0f, kLeast = 0x1p-13f;
-__device__ __forceinline__ void limbs_f16_apart(const float (&x)[8], u32x4 (&limb)[2]) {
+__device__ __forceinline__ void limbs_f16(const float (&x)[8], u32x4 (&limb)[2]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     f16x2 hi = {(_Float16)x[2 * j], (_Float16)x[2 * j + 1]};
@@ -351,14 +340,14 @@ __device__ __forceinline__ void limbs_f16_apart(const float (&x)[8], u32x4 (&lim
     limb[1][j] = __builtin_bit_cast(uint32_t, lo);
   }
 }
-// Codes as f16: with its top bit flipped a code's byte is code + 128, and the
-// f16 whose bytes are that and 0x64 is 1024 + 128 + code.
-__device__ __forceinline__ uint32_t less_1152(uint32_t v) {
-  const f16x2 c = {(_Float16)1152.0f, (_Float16)1152.0f};
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - c);
+// Two codes (byte kByte of each register) as bf16, which holds them exactly.
+template <int kByte>
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t a, uint32_t b) {
+  return hi16s(as_u32((float)(int8_t)(a >> (8 * kByte))), as_u32((float)(int8_t)(b >> (8 * kByte))));
 }
-__device__ __forceinline__ uint32_t codes_f16(uint32_t two) {  // in bytes 0 and 2, the others zero
-  return less_1152(two ^ 0x64806480u);
+template <int kFrom>  // of one register, bytes kFrom and kFrom + 1
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t v) {
+  return hi16s(as_u32((float)(int8_t)(v >> (8 * kFrom))), as_u32((float)(int8_t)(v >> (8 * kFrom + 8))));
 }
 // A register whose upper half nothing reads (so that nothing clears it).
 __device__ __forceinline__ uint32_t low_half(uint16_t v) {
@@ -381,7 +370,7 @@ __device__ __forceinline__ void scale_slots(const float (&p)[8], float d, int up
 }
 template <int kType>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (kType == kBF16)
+  if constexpr (kType != kF16)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -438,7 +427,7 @@ __device__ __forceinline__ void results_stored() { asm volatile("s_waitcnt vmcnt
 template <int kType, int NC, bool kFull>  // head_dim <= 32 NC; kFull: equal
 __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_kernel(TileArgs ta) {
   constexpr bool kF = kType == kF32, kQ = kType == kQ8_0;
-  constexpr int kL = kType == kBF16 ? 3 : kF ? 1 : 2;              // limbs
+  constexpr int kL = kF ? 1 : kType == kF16 ? 2 : 3;             // limbs
   constexpr int kSub = kF ? 1 : 2;                                  // 16-token products of a tile
   constexpr int kTile = 16 * kSub, kSlots = 4 * kSub;               // tokens of a tile, of a lane
   constexpr int kStep = kWaves * kTile;
@@ -448,10 +437,10 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
   constexpr int kVD = kQ ? 2 : kF || NC <= 2 ? 4 : 8;
   constexpr int kVG = (32 * NC + 16 * kVD - 1) / (16 * kVD);        // such groups
   // Wide Q8_0 rows: loads of four dims, a 16-lane row's upper eight lanes those
-  // of the next block, so a register holds two blocks.  Loads of two dims take
-  // 64 registers of a tile there, more than are left (4 sequences of 14563,
-  // head_dim 256: 36.9 us); at head_dim 128 they are the faster ones, as most
-  // of the four-byte loads lie across two words (131072 tokens: 68.5 us, 73.9).
+  // of the next block, so a register holds two blocks: half the loads and
+  // registers (4 sequences of 14563, 4 heads of 256: 47.4 us, in loads of two
+  // dims 47.7).  At head_dim 128 loads of two dims are the faster ones, as most
+  // of the four-byte loads lie across two words (131072 tokens: 74.7 us, 77.7).
   constexpr bool kPaired = kQ && NC > 4;
   constexpr int kVL = kPaired ? (NC + 1) / 2 : kVG;                 // a token's loads of V
   constexpr int kSB = (NC + 1) / 2;                                 // registers of Q8_0 scales
@@ -617,7 +606,6 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
   for (int t = 0; t < kVG * kVD; ++t) o[t] = f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
-  int d_exp = -100;  // Q8_0: O is scaled so that scales of up to 2^d_exp keep P's limbs in range
   for (int seg = lo; seg < hi; seg += ta.segment) {
     const int end = hi - seg < ta.segment ? hi : seg + ta.segment;
     const int page0 = page_of(seg), pages = page_of(end - 1) - page0 + 1;
@@ -652,7 +640,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           const bool there = n < heads && (kFull || 4 * kPer * (kRegQ ? u : wave + u * kWaves) + kPer * g + j < D);
           x[u][j] = there ? x[u][j] : 0.0f;
         }
-      if constexpr (!kF && kType != kBF16) {  // f16 limbs: every head's largest value just below 2^14
+      if constexpr (kType == kF16) {  // f16 limbs: every head's largest value just below 2^14
         float mx = 0.0f;
 #pragma unroll
         for (int u = 0; u < kMy; ++u)
@@ -676,9 +664,8 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       for (int u = 0; u < kMy; ++u) {
         u32x4 limb[kL];
         if constexpr (kF) limb[0] = u32x4{as_u32(x[u][0]), as_u32(x[u][1]), as_u32(x[u][2]), as_u32(x[u][3])};
-        else if constexpr (kType == kBF16) limbs_bf16(x[u], limb);
-        else if constexpr (kType == kF16) limbs_f16_apart(x[u], limb);
-        else limbs_f16(x[u], limb);
+        else if constexpr (kType == kF16) limbs_f16(x[u], limb);
+        else limbs_bf16(x[u], limb);
 #pragma unroll
         for (int k = 0; k < kL; ++k) {
           if constexpr (kRegQ) ql[u][k] = limb[k];
@@ -713,9 +700,8 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
             u32x4 op;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-              const uint32_t x = kr[s][c][w] ^ 0x80808080u;
-              op[2 * w] = less_1152(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u));
-              op[2 * w + 1] = less_1152(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u));
+              op[2 * w] = pair_bf16<0>(kr[s][c][w]);
+              op[2 * w + 1] = pair_bf16<2>(kr[s][c][w]);
             }
             f32x4 t = {0, 0, 0, 0};
 #pragma unroll
@@ -789,31 +775,11 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       for (int j = 1; j < kSlots; ++j) top = __builtin_fmaxf(top, p[j]);
       top = cross_max(top);
       const float tile_top = top;
-      bool grown = __ballot(top > m + kGrowth) != 0;
-      int d_new = d_exp;
-      if constexpr (kQ) {
-        // the largest scale of the tile against what O's scaling allows for
-        float dm = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kSB; ++i) dm = __builtin_fmaxf(dm, __builtin_fabsf(dv[i]));
-        const int de = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) : -100;
-        if (__ballot(de > d_exp) != 0) {
-          int w = de;
-          for (int d = 1; d < 64; d *= 2) {
-            const int y = __shfl_xor(w, d);
-            w = y > w ? y : w;
-          }
-          d_new = __builtin_amdgcn_readfirstlane(w);
-          grown = true;
-        }
-      }
-      if (grown) {
+      if (__ballot(top > m + kGrowth) != 0) {
         top = __builtin_fmaxf(m, top);
-        float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
         m = top;
         l *= f;
-        if constexpr (kQ) f = ldexpf(f, d_exp - d_new);
-        d_exp = d_new;
 #pragma unroll
         for (int t = 0; t < kVG * kVD; ++t) o[t] *= f;
       }
@@ -832,9 +798,6 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[4 * v + e] = mfma4(as_f32(vr[j][v][e]), p[j], o[4 * v + e]);
       } else if constexpr (kQ) {
-        const float up = ldexpf(1.0f, 6 - d_exp);
-#pragma unroll
-        for (int j = 0; j < kSlots; ++j) p[j] *= up;
         // of a pair of blocks, lanes below 8 keep the lower two dims, those above
         // the upper: the rest is swapped between them
         const uint32_t halves = n < 8 ? 0x05040100u : 0x03020706u;
@@ -853,14 +816,14 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           float y[8];
           scale_slots(p, dv[v >> 1], v & 1, y);
           u32x4 limb[kL];
-          limbs_f16(y, limb);
+          limbs_bf16(y, limb);
           u32x4 op[2];
 #pragma unroll
-          for (int d = 0; d < 2; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              op[d][j] = codes_f16(__builtin_amdgcn_perm(codes[2 * j + 1], codes[2 * j],
-                                                         0x0c040c00u + 0x00010001u * ((kPaired ? 2 * (v % 2) : 0) + d)));
+          for (int j = 0; j < 4; ++j) {
+            const bool second = kPaired && v % 2 != 0;
+            op[0][j] = second ? codes_bf16<2>(codes[2 * j], codes[2 * j + 1]) : codes_bf16<0>(codes[2 * j], codes[2 * j + 1]);
+            op[1][j] = second ? codes_bf16<3>(codes[2 * j], codes[2 * j + 1]) : codes_bf16<1>(codes[2 * j], codes[2 * j + 1]);
+          }
 #pragma unroll
           for (int k = 0; k < kL; ++k)
 #pragma unroll
@@ -902,7 +865,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           }
           u32x4 limb[kL];
           if constexpr (kType == kBF16) limbs_bf16(x, limb);
-          else limbs_f16_apart(x, limb);
+          else limbs_f16(x, limb);
 #pragma unroll
           for (int v = 0; v < kVG; ++v)
 #pragma unroll
@@ -962,8 +925,6 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
     m_lds[wave][n] = m;
     l_lds[wave][n] = l;
   }
-  float f = 1.0f;
-  if constexpr (kQ) f = ldexpf(1.0f, d_exp - 6);
   const int DS = D + 4, fit = kMergeFloats / (kWaves * DS);  // heads that fit at once
   const int slot_floats = ((a.group < kHeads ? a.group : kHeads) * (D + 2) + 3) / 4 * 4;
   const auto part = __builtin_amdgcn_make_buffer_rsrc(ta.part, 0, (int)ta.part_bytes, 0x00020000);
@@ -990,14 +951,14 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
           const int r = 4 * g + i, dim = 16 * kVD * v + (kPaired ? 4 * (r & 7) + 2 * (r >> 3) : kVD * r);
           if constexpr (kQ) {
             if (!kFull && dim >= D) continue;
-            to[dim] = o[v * kVD][i] * f;
-            to[dim + 1] = o[v * kVD + 1][i] * f;
+            to[dim] = o[v * kVD][i];
+            to[dim + 1] = o[v * kVD + 1][i];
           } else {
 #pragma unroll
             for (int d = 0; d < kVD; d += 4)
               if ((kFull && 32 * NC % (16 * kVD) == 0) || dim + d < D)
                 *reinterpret_cast<f32x4 *>(to + dim + d) = f32x4{o[v * kVD + d][i], o[v * kVD + d + 1][i],
-                                                                 o[v * kVD + d + 2][i], o[v * kVD + d + 3][i]} * f;
+                                                                 o[v * kVD + d + 2][i], o[v * kVD + d + 3][i]};
           }
         }
     }

@@ -811,8 +811,8 @@ def _parked(torch, d, kv, n, gap, seed):
 
 
 @pytest.mark.parametrize("gap", [8, 13, 17, 22, 40])
-@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("F16", 80), ("BF16", 128), ("F32", 128),
-                                  ("F16", 100)])
+@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("F16", 80), ("Q8_0", 128), ("Q8_0", 256), ("Q8_0", 64),
+                                  ("BF16", 128), ("F32", 128), ("F16", 100)])
 def test_attention_keeps_the_weights_below_a_token_whose_value_is_zero(torch, okq, tn, d, gap):
     """The output is what the small weights make it, and each of them is off by
     2e + 8u of itself, however far below the largest: tokens of the heavy one's
@@ -828,7 +828,7 @@ def test_attention_keeps_the_weights_below_a_token_whose_value_is_zero(torch, ok
         _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 1))
 
 
-@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("BF16", 128), ("F32", 128)])
+@pytest.mark.parametrize("tn,d", [("F16", 128), ("F16", 256), ("Q8_0", 128), ("Q8_0", 256), ("BF16", 128), ("F32", 128)])
 def test_attention_keeps_the_small_elements_of_a_query(torch, okq, tn, d):
     """A query whose first element is 2^26 times the others, which meet large
     keys: scores of about 1 that the large element has no part in."""
@@ -846,3 +846,28 @@ def test_attention_keeps_the_small_elements_of_a_query(torch, okq, tn, d):
     got = _attention(torch, okq, cache, table, q, lengths, 50, 1.0)
     torch.cuda.synchronize()
     _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 1))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_q8_0_blocks_of_very_different_scales(torch, okq, d):
+    """Each block's values keep their precision beside a block of 2^10 or 2^20
+    times its scale, and beside a token of a tiny weight and a huge scale."""
+    print(f"[gpu] q8_0 scales {d}", flush=True)
+    g = torch.Generator().manual_seed(d)
+    K, V = [], []
+    for n in (30, 300, 3000):
+        k, v = 0.3 * torch.randn(n, 2, d, generator=g), torch.randn(n, 2, d, generator=g)
+        v[:, :, :32] *= 2.0 ** 10
+        v[:, :, 32:64] *= torch.tensor([2.0 ** -10, 1.0])[torch.arange(n) % 2][:, None, None]
+        k[n // 3] = 0.0
+        k[n // 3, :, 0] = -4.0
+        v[n // 3, :, :32] *= 2.0 ** 8  # 32 nats below the rest
+        v[n // 3, :, 32:] = 0.0
+        K.append(k)
+        V.append(v)
+    cache, table, lengths = _written_cache(torch, okq, "Q8_0", d, 2, 16, K, V)
+    q = torch.randn(3, 4, d, generator=g).cuda() / d ** 0.5
+    q[:, :, 0] = 8.0
+    got = _attention(torch, okq, cache, table, q, lengths, 3000, 1.0)
+    torch.cuda.synchronize()
+    _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 2))
