@@ -330,10 +330,12 @@ okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, in
  * exp(f(scale * q . K)).  A sequence with nothing to see (length 0, hidden pages)
  * gets zeros and lse -inf; tokens outside the length or the window may hold
  * anything, NaN too; a visible infinity or NaN leaves no finite number in what
- * it reaches (a key: its heads' lse; a value: its column of out).  Products and
- * sums are f32 on the cached values; a row's result depends on the call's shape
- * and lengths only, not on timing.
- * seqs == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
+ * it reaches: a key, of either sign and capped or not, makes its heads' lse and
+ * out NaN, as a query does its head's; a value leaves none in its column of out
+ * (a Q8_0 block's scale: its 32), whatever the token's weight is.  A sum q . K
+ * past f32's range counts as infinite.  Products and sums are f32 on the cached
+ * values; a row's result depends on the call's shape and lengths only, not on
+ * timing.  seqs == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
  * reference, whose attention is on contiguous host rows
  * (crates/kernels/src/attention.rs). */
 okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, int64_t q_heads,

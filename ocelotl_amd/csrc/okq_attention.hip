@@ -21,6 +21,11 @@ namespace {
 
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
 
+// A score without its infinities: NaN in their place.  The products of an
+// infinite key with a query's limbs are infinite or NaN, whichever the bits of
+// the query make them, so the one rule for all caches is NaN.
+__device__ __forceinline__ float finite_or_nan(float s) { return __builtin_fmaf(s, 0.0f, s); }
+
 // Value i of a cached row.
 template <int kType>
 __device__ __forceinline__ float cached(const uint8_t *row, int i) {
@@ -110,7 +115,7 @@ __global__ __launch_bounds__(64 * row_waves(kV)) void attention_rows_kernel(Attn
         float dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < kV; ++j) dot += q[h][j] * k[u][j];
-        s[u] = wave_sum(dot) * a.scale;
+        s[u] = finite_or_nan(wave_sum(dot)) * a.scale;
         if (a.softcap > 0.0f) s[u] = a.softcap * tanhf(s[u] / a.softcap);
         s[u] = seen[u] ? s[u] : -INFINITY;
         top = fmaxf(top, s[u]);
@@ -748,7 +753,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
       }
       if (more) load_k(buf ^ 1);
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) p[j] *= to_log2;
+      for (int j = 0; j < kSlots; ++j) p[j] = finite_or_nan(p[j]) * to_log2;
       if (a.softcap > 0.0f) {
         tanh_all(p);
 #pragma unroll
@@ -937,7 +942,7 @@ __global__ __launch_bounds__(kThreads, NC <= 4 ? 2 : 1) void attention_tiles_ker
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] / sum;
     __builtin_memcpy(out + h * D + 4 * quad, &v, sizeof v);
-    if (lse && quad == 0) lse[h] = top == -INFINITY ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (lse && quad == 0) lse[h] = sum == 0.0f ? -INFINITY : ((top == -INFINITY ? 0.0f : top) + __builtin_amdgcn_logf(sum)) * kLn2;
   };
   for (int p0 = 0; p0 < heads; p0 += fit) {
     const int count = heads - p0 < fit ? heads - p0 : fit;

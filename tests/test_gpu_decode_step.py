@@ -871,3 +871,83 @@ def test_attention_of_q8_0_blocks_of_very_different_scales(torch, okq, d):
     got = _attention(torch, okq, cache, table, q, lengths, 3000, 1.0)
     torch.cuda.synchronize()
     _attn_check(torch, got, _attn_want(torch, cache, table, q, lengths, 1.0, 0.0, 0, 2))
+
+
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+@pytest.mark.parametrize("tn,d", [("BF16", 128), ("F16", 128), ("F16", 256), ("F32", 128), ("Q8_0", 128), ("BF16", 100),
+                                  ("F32", 33), ("Q8_0", 320)])
+def test_attention_of_an_infinite_key(torch, okq, tn, d, softcap):
+    """One infinity of either sign among the keys of one sequence and head: no
+    finite number in what reads it, whatever the queries' signs and bits are,
+    and the results of all else as without it."""
+    print(f"[gpu] infinite key {tn} {d} {softcap}", flush=True)
+    lengths, group = [40, 600], 3
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], d, 2, group, 16, lengths)
+    q[:, 0::3] = q[:, 0::3].to(torch.bfloat16).float()  # queries of few bits beside those of many
+    q[:, 1::3, :] = q[:, 1::3, :].abs()
+    plain = _attention(torch, okq, cache, table, q, lengths, 600, d ** -0.5, softcap)
+    torch.cuda.synchronize()
+    if tn == "Q8_0":
+        bad = torch.tensor([0x00, 0xFC], dtype=torch.uint8, device="cuda")  # a block's scale: -inf
+        at = slice(0, 2)
+    else:
+        bad = torch.tensor([-math.inf], device="cuda").to(_dtype(torch, TYPES[tn])).view(torch.uint8)
+        at = slice(0, len(bad))
+    key = cache.views[0][int(table[1, 20]), 1, 7]
+    was = key[at].clone()
+    for sign in (0x80, 0x00):
+        bad[-1] = (int(bad[-1]) & 0x7F) | sign
+        key[at] = bad
+        out, lse = _attention(torch, okq, cache, table, q, lengths, 600, d ** -0.5, softcap)
+        torch.cuda.synchronize()
+        assert out[1, group:].isnan().all() and lse[1, group:].isnan().all()
+        for a, b in zip((out, lse), plain):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1, :group], b[1, :group])
+    key[at] = was
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_an_infinite_q8_0_scale_among_the_values(torch, okq, d):
+    """It reaches its block's 32 columns in its head, and nothing else: not the
+    columns of another block of its token, whose scale is far above all others."""
+    print(f"[gpu] infinite scale {d}", flush=True)
+    lengths = [33, 500]
+    cache, table, q = _attn_inputs(torch, okq, Q8_0, d, 2, 2, 16, lengths)
+    row = cache.views[1][int(table[1, 12]), 1, 3]
+    if d > 96:
+        row[102:104] = torch.tensor([0x00, 0x70], dtype=torch.uint8, device="cuda")  # 2^13
+    want = _attn_want(torch, cache, table, q, lengths, d ** -0.5, 0.0, 0, 2)
+    row[34:36] = torch.tensor([0x00, 0x7C], dtype=torch.uint8, device="cuda")
+    out, lse = _attention(torch, okq, cache, table, q, lengths, 500, d ** -0.5)
+    torch.cuda.synchronize()
+    assert not torch.isfinite(out[1, 2:, 32:64]).any()
+    out[1, 2:, 32:64] = 0.0
+    for w in (want[0], want[2]):
+        w[1, 2:, 32:64] = 0.0
+    _attn_check(torch, (out, lse), want)
+
+
+@pytest.mark.parametrize("tn,d", [("BF16", 128), ("F16", 128), ("F16", 256), ("F32", 80), ("F16", 100), ("F32", 260)])
+def test_attention_of_an_infinite_value(torch, okq, tn, d):
+    """It reaches its column in its head, and nothing else, also where the
+    token's weight is next to nothing."""
+    print(f"[gpu] infinite value {tn} {d}", flush=True)
+    t = TYPES[tn]
+    lengths = [33, 500]
+    cache, table, q = _attn_inputs(torch, okq, t, d, 2, 2, 16, lengths)
+    for far in (False, True):
+        view = cache.views[0][int(table[1, 12]), 1, 3]
+        if far:  # the query points away from the key
+            view[:] = (q[1, 2:].sum(0) * -5).to(_dtype(torch, t)).view(torch.uint8)
+        want = _attn_want(torch, cache, table, q, lengths, d ** -0.5, 0.0, 0, 2)
+        row = cache.views[1][int(table[1, 12]), 1, 3].view(_dtype(torch, t))
+        was = row[5].item()
+        row[5] = math.inf
+        out, lse = _attention(torch, okq, cache, table, q, lengths, 500, d ** -0.5)
+        torch.cuda.synchronize()
+        row[5] = was
+        assert not torch.isfinite(out[1, 2:, 5]).any()
+        out[1, 2:, 5] = 0.0
+        for w in (want[0], want[2]):
+            w[1, 2:, 5] = 0.0
+        _attn_check(torch, (out, lse), want)
