@@ -276,20 +276,27 @@ okq_status get_workspace(int dev, hipStream_t s, size_t bytes, void **out, int s
   return workspace_status(grow_workspace(dev, s, bytes, bytes, out, slot), bytes);
 }
 
-// A slot whose kernels leave it zero: filled on the stream when it is new.
+// A slot whose kernels leave it zero: filled on the stream when it is new, and
+// taken as filled once that launch went through (the caller holds the stream's
+// lock in between).  A fill that a capture would only record fills nothing.
 okq_status get_zeroed_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot) {
   okq_status st = get_workspace(dev, s, bytes, out, slot);
   if (st != OKQ_OK) return st;
-  size_t fresh = 0;
+  size_t fresh;
   {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
-    Workspace &w = g_ws[{dev, s, slot}];
-    if (w.zeroed != w.ptr) {
-      w.zeroed = w.ptr;
-      fresh = w.bytes;
-    }
+    const Workspace &w = g_ws[{dev, s, slot}];
+    fresh = w.zeroed != w.ptr ? w.bytes : 0;
   }
-  return fresh ? hip_status(okq::launch_zero(*out, fresh / 4 * 4, s), "workspace fill") : ok();
+  if (!fresh) return ok();
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone)
+    return workspace_status(Grow::Capture, bytes);
+  st = hip_status(okq::launch_zero(*out, fresh / 4 * 4, s), "workspace fill");
+  if (st != OKQ_OK) return st;
+  std::lock_guard<std::mutex> lock(g_ws_mutex);
+  g_ws[{dev, s, slot}].zeroed = *out;
+  return ok();
 }
 
 // The workspace of a plan, its K split lowered where it cannot be had.
