@@ -1311,7 +1311,8 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
   if (rows < 0 || vocab < 1 || vocab > INT32_MAX - 65536)
     return fail(OKQ_E_SHAPE, "%s rows=%lld vocab=%lld: vocab must be at least 1 and below 2^31 - 65536", what,
                 (long long)rows, (long long)vocab);
-  if (rows > (1 << 22) / (vocab / 2048 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
+  // a row has at most vocab / 2048 + 1 workgroups of 1024 threads
+  if (rows > ((1 << 22) - 1) / (vocab / 2048 + 1)) return fail(OKQ_E_SHAPE, "%s rows*vocab exceeds u32 launch limits", what);
   if (history_stride < 0 || bias_stride < 0 || mask_stride < 0 || history_stride >= 1 << 30 || bias_stride >= 1 << 30)
     return fail(OKQ_E_SHAPE,
                 "%s history_stride=%lld bias_stride=%lld mask_stride=%lld must not be negative, the first two below 2^30", what,

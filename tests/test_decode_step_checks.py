@@ -177,3 +177,15 @@ def test_valid_calls_without_a_device_are_refused_as_such(okqlib):
 def test_sizes_past_what_the_kernels_index(okqlib, call, kw, text):
     assert call(**kw) == okq.E_SHAPE
     assert text in okq.last_error()
+
+
+@pytest.mark.parametrize("vocab,rows", [(1, 1 << 22), (1000, 1 << 22), (2047, 1 << 22), (2048, 1 << 21), (4096, 1398102)])
+def test_logits_rows_up_to_what_a_launch_counts(okqlib, vocab, rows):
+    """2^32 threads are one too many for a launch's count: refused; a row less is not."""
+    kw = dict(vocab=vocab, xs=vocab, os=vocab, hist=None, bids=None, mask=None)
+    assert logits(rows=rows, **kw) == okq.E_SHAPE
+    assert "launch limits" in okq.last_error()
+    n = ctypes.c_int()
+    assert okqlib.okq_device_count(ctypes.byref(n)) == okq.OK
+    if n.value == 0:  # a valid call gets as far as looking for a device
+        assert logits(rows=rows - 1, **kw) == okq.E_NODEV
