@@ -262,25 +262,25 @@ Grow grow_workspace(int dev, hipStream_t s, size_t bytes, size_t reserve, void *
   return Grow::Alloc;
 }
 
-okq_status workspace_status(Grow g, size_t bytes) {
+okq_status workspace_status(Grow g, size_t bytes, const char *whose = "GEMM") {
   if (g == Grow::Capture)
     return fail(OKQ_E_ALLOC,
-                "hip-gfx950: GEMM workspace of %zu bytes is not allocated for this stream and cannot be allocated "
+                "hip-gfx950: %s workspace of %zu bytes is not allocated for this stream and cannot be allocated "
                 "during graph capture; run one call of this size on the stream before capturing",
-                bytes);
-  if (g == Grow::Alloc) return fail(OKQ_E_ALLOC, "hip-gfx950: hipMalloc of a %zu-byte GEMM workspace failed", bytes);
+                whose, bytes);
+  if (g == Grow::Alloc) return fail(OKQ_E_ALLOC, "hip-gfx950: hipMalloc of a %zu-byte %s workspace failed", bytes, whose);
   return ok();
 }
 
-okq_status get_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot = 0) {
-  return workspace_status(grow_workspace(dev, s, bytes, bytes, out, slot), bytes);
+okq_status get_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot = 0, const char *whose = "GEMM") {
+  return workspace_status(grow_workspace(dev, s, bytes, bytes, out, slot), bytes, whose);
 }
 
 // A slot whose kernels leave it zero: filled on the stream when it is new, and
 // taken as filled once that launch went through (the caller holds the stream's
 // lock in between).  A fill that a capture would only record fills nothing.
-okq_status get_zeroed_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot) {
-  okq_status st = get_workspace(dev, s, bytes, out, slot);
+okq_status get_zeroed_workspace(int dev, hipStream_t s, size_t bytes, void **out, int slot, const char *whose) {
+  okq_status st = get_workspace(dev, s, bytes, out, slot, whose);
   if (st != OKQ_OK) return st;
   size_t fresh;
   {
@@ -291,7 +291,7 @@ okq_status get_zeroed_workspace(int dev, hipStream_t s, size_t bytes, void **out
   if (!fresh) return ok();
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone)
-    return workspace_status(Grow::Capture, bytes);
+    return workspace_status(Grow::Capture, bytes, whose);
   st = hip_status(okq::launch_zero(*out, fresh / 4 * 4, s), "workspace fill");
   if (st != OKQ_OK) return st;
   std::lock_guard<std::mutex> lock(g_ws_mutex);
@@ -1294,8 +1294,8 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   const okq::AttnPlan plan = okq::attention_plan(a, info.cu_count);
   void *part = nullptr, *arrived = nullptr;
   if (plan.part_bytes) {
-    st = get_workspace(dev, s, plan.part_bytes, &part, 3);
-    if (st == OKQ_OK && plan.arrived_bytes) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 4);
+    st = get_workspace(dev, s, plan.part_bytes, &part, 3, what);
+    if (st == OKQ_OK && plan.arrived_bytes) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 4, what);
     if (st != OKQ_OK && plan.splits) return st;
   }
   return hip_status(okq::launch_attention(a, plan, part, arrived, s), "paged_attention launch");
@@ -1361,7 +1361,7 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
   std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
   void *ws = nullptr;
   if (best) {
-    st = get_zeroed_workspace(dev, s, okq::logits_workspace(rows), &ws, 2);
+    st = get_zeroed_workspace(dev, s, okq::logits_workspace(rows), &ws, 2, what);
     if (st != OKQ_OK) return st;
   }
   return hip_status(okq::launch_logits(a, ws, info.cu_count, s), "logits_process launch");

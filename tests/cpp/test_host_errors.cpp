@@ -6,6 +6,7 @@
 #include <cstring>
 #include <map>
 #include <string>
+#include <utility>
 
 #include <hip/hip_runtime_api.h>
 
@@ -129,10 +130,31 @@ void refused_fills() {
   }
 }
 
+// A workspace that cannot be had is the call's own.
+void missing_workspaces() {
+  const std::pair<okq_status (*)(void *), const char *> calls[] = {{logits, "logits_process workspace"},
+                                                                   {split_attention, "paged_attention workspace"}};
+  int i = 0;
+  for (const auto &[call, words] : calls) {
+    g_capturing = true;
+    CHECK(launches(call, stream(i++), OKQ_E_ALLOC) == 0, "not during a capture");
+    CHECK(error().find(words) != std::string::npos && error().find("capture") != std::string::npos, error());
+    g_capturing = false;
+    g_no_memory = true;
+    CHECK(launches(call, stream(i++), OKQ_E_ALLOC) == 0, "not without memory");
+    CHECK(error().find(words) != std::string::npos && error().find("hipMalloc") != std::string::npos, error());
+    g_no_memory = false;
+  }
+  g_no_memory = true;
+  CHECK(attention(stream(i), 700, 16) == OKQ_OK, "a call that splits nothing goes on without");
+  g_no_memory = false;
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
-  const std::map<std::string, void (*)()> cases = {{"refused_fills", refused_fills}};
+  const std::map<std::string, void (*)()> cases = {{"refused_fills", refused_fills},
+                                                   {"missing_workspaces", missing_workspaces}};
   const auto it = cases.find(argc > 1 ? argv[1] : "");
   if (it == cases.end()) {
     std::printf("no such case\n");

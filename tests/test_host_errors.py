@@ -9,7 +9,7 @@ import pytest
 BINARY = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build", "test_host_errors")
 
 
-@pytest.mark.parametrize("case", ["refused_fills"])
+@pytest.mark.parametrize("case", ["refused_fills", "missing_workspaces"])
 def test_host_errors(case):
     assert os.path.exists(BINARY), f"{BINARY} is not built: run __graft_entry__.build() (make -C tests/cpp)"
     r = subprocess.run([BINARY, case], capture_output=True, text=True, timeout=120)
