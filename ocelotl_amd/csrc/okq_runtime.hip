@@ -1256,7 +1256,9 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   if (table_width < 0 || max_length < 0 || window < 0 || table_width > INT32_MAX || max_length > 1 << 30)
     return fail(OKQ_E_SHAPE, "%s table_width=%lld max_length=%lld window=%lld must not be negative nor exceed 32 bits",
                 what, (long long)table_width, (long long)max_length, (long long)window);
-  if (seqs > 0 && max_length / 16 + 1 > INT32_MAX / seqs)
+  // tokens past the table are never looked at
+  const int64_t longest = mul_ok(table_width, cache->page_tokens, span) ? std::min(max_length, span) : max_length;
+  if (seqs > 0 && longest / 16 + 1 > INT32_MAX / seqs)
     return fail(OKQ_E_SHAPE, "%s seqs=%lld of max_length=%lld exceed u32 launch limits", what, (long long)seqs,
                 (long long)max_length);
   if (!std::isfinite(scale) || !(softcap >= 0.0f) || softcap == INFINITY)
@@ -1283,7 +1285,7 @@ okq_status okq_paged_attention(const float *q, int64_t q_stride, int64_t seqs, i
   a.table = block_table;
   a.lengths = lengths;
   a.table_width = (int)table_width;
-  a.max_len = (int)(mul_ok(table_width, cache->page_tokens, span) ? std::min(max_length, span) : max_length);
+  a.max_len = (int)longest;
   a.scale = scale;
   a.softcap = softcap;
   a.window = (int)std::min<int64_t>(window, INT32_MAX);

@@ -189,3 +189,16 @@ def test_logits_rows_up_to_what_a_launch_counts(okqlib, vocab, rows):
     assert okqlib.okq_device_count(ctypes.byref(n)) == okq.OK
     if n.value == 0:  # a valid call gets as far as looking for a device
         assert logits(rows=rows - 1, **kw) == okq.E_NODEV
+
+
+def test_a_loose_max_length_is_bounded_by_the_table(okqlib):
+    """A max_length of the type's range is as good as the table's own: what a
+    launch counts is tokens that the table can name."""
+    kw = dict(seqs=64, longest=1 << 30)
+    assert attention(width=1 << 26, **kw) == okq.E_SHAPE
+    assert "launch limits" in okq.last_error()
+    n = ctypes.c_int()
+    assert okqlib.okq_device_count(ctypes.byref(n)) == okq.OK
+    if n.value == 0:  # a valid call gets as far as looking for a device
+        assert attention(width=4, **kw) == okq.E_NODEV
+        assert attention(width=0, table=None, **kw) == okq.E_NODEV
