@@ -305,7 +305,8 @@ typedef struct okq_kv_pages {
  * rows at slots[token] (int64; a slot outside the cache, -1 say, stores
  * nothing), or cache NULL (then v and slots are not read).  Keys and values
  * are rounded to the cache's type, to nearest even; Q8_0 blocks are
- * okq_quantize's bytes.  Tokens that share a slot race: its row may mix theirs.
+ * okq_quantize's bytes (of values without NaN, which Q8_0 cannot hold and whose
+ * codes are 0).  Tokens that share a slot race: its row may mix theirs.
  * tokens == 0 is a no-op.  The rotation follows crates/kernels/src/rope.rs
  * (its pairs are the halves); no counterpart in the reference fuses the three. */
 okq_status okq_qk_norm_rope(const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,

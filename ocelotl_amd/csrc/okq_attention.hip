@@ -220,15 +220,16 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 // The queries and probabilities are f32, the matrix instructions' operands 16
 // bits: each is split into limbs whose sum is the f32 value -- three bf16
 // (exactly; BF16 and Q8_0 caches), two f16 (to 2^-23, scaled by a power of two
-// into f16's range; F16 caches) --
-// and each limb gets its product.  Over F16 caches the second limb has a scale
-// of its own, so do the weights of a tile and head, and those too small for it
-// go in by themselves: a weight keeps its precision however far it lies below
-// the largest (a token whose value is near zero may have that one).  The price
-// is a sum per limb, added to O in f32: 24 sequences, window 1024, head_dim
-// 256, 14.6 us (13.8 with limbs of one scale), 517 tokens 8.3 (7.8), 131072
-// tokens 99.2 (98.6).  The cached values are exact operands as they are.  A tile's 48 products of bf16 take 768 cycles of the matrix unit
-// against the 16 KB that a SIMD's share of the memory takes 7400 cycles for.
+// into f16's range; F16 caches) -- and each limb gets its product.  Over F16
+// caches the second limb has a scale of its own, so do the weights of a tile
+// and head, and those too small for it go in by themselves: a weight keeps its
+// precision however far it lies below the largest (a token whose value is near
+// zero may have that one).  The price is a sum per limb, added to O in f32: 24
+// sequences, window 1024, head_dim 256, 14.6 us (13.8 with limbs of one scale),
+// 517 tokens 8.3 (7.8), 131072 tokens 99.2 (98.6).  The cached values are exact
+// operands as they are.  A tile's 48 products of bf16 take 768 cycles of the
+// matrix unit against the 16 KB that a SIMD's share of the memory takes 7400
+// cycles for.
 //
 // Q8_0 codes become bf16 exactly; a block's scale goes with its partial scores
 // (they leave the matrix unit per block) and, for V, with P before the limbs:
@@ -240,9 +241,9 @@ __global__ __launch_bounds__(256) void attention_rows_join_kernel(AttnArgs a, in
 // 8192, 268 MB: 54 us, 5.0 TB/s); Q8_0 what two waves a SIMD have in flight, as
 // its rows come in pieces of 2 and 8 bytes, beside the instructions that decode
 // them and split the weights block by block (131072 tokens, 285 MB: 75 us, 3.8
-// TB/s; 68 with two f16 limbs, which lose small weights); a short cache the chain length ->
-// page -> row -> result -> count -> join, each a trip to memory (517 tokens,
-// 2 MB: 8.2 us).
+// TB/s; 68 with two f16 limbs, which lose small weights); a short cache the
+// chain length -> page -> row -> result -> count -> join, each a trip to memory
+// (517 tokens, 2 MB: 7.9 us).
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -391,8 +392,8 @@ __device__ __forceinline__ T load_any(const void *p) {  // any alignment
 }
 
 // tanh of a lane's values, off by at most 3 steps of 2^-24: below 0.625 an odd
-// polynomial (least squares towards the least largest relative error, 4.4e-9),
-// beyond 1 - 2 / (exp(2 |x|) + 1), which loses nothing there.  Scores are
+// polynomial (towards the least largest relative error by Lawson's reweighted
+// least squares; 8.2e-9 with its coefficients in f32), beyond 1 - 2 / (exp(2 |x|) + 1), which loses nothing there.  Scores are
 // mostly far below their cap, and a wave without larger ones skips that half.
 // (The library's tanhf, with branches a value, took 5 us of a 20 us call.)
 template <int kN>
@@ -1128,7 +1129,7 @@ AttnPlan attention_plan(const AttnArgs &a, int cu_count) {
   const int64_t pairs = (int64_t)c.kv_heads * head_tiles, most = ((int64_t)a.max_len + tile - 1) / tile;
   // workgroups that run at once: above head_dim 128 a wave takes more than half
   // of a SIMD's registers (held to half, 4 sequences of 14563 tokens of Q8_0 and
-  // head_dim 256 take 49.8 us for 33.8)
+  // 4 heads of 256 take 77.4 us for 47.7)
   const int64_t aim = (c.head_dim <= 128 ? 2 : 1) * (int64_t)cu_count;
   // All chunks (units + seqs a head at most) at once where the sequences leave
   // room for that.  Where they do not, the card is full without a split, which

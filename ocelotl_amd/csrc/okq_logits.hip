@@ -83,7 +83,11 @@ __device__ __forceinline__ void choose(const LogitsArgs &a, int row, int slices,
 // workgroup that ends last on a row turns the largest key into the token.
 // Memory bounds it: the logits are read and written once (200 rows of 262144
 // with a mask, 426 MB: 85 us, 5.0 TB/s); a single row the chain logits or lists
-// -> LDS -> result -> meeting place (128256 entries, 1 MB: 5.7 us).
+// -> LDS -> result -> meeting place (128256 entries, 1 MB: 5.7 us).  Bias lists
+// of more than kThreads entries go through LDS kThreads at a time, with two
+// waits each and a search for a token's first entry (128256 entries: 6.2 us with
+// 1024 biases, 12.2 with 1025, 17.2 with 2000; 64 rows 14.4, 50 and 76): request
+// biases are tens, so that is left as it is.
 template <int V, bool kMarks, int kBias>  // a history; biases (with marks): 1 a list of kThreads at most, 2 a longer one
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, int slices, Meeting *meet) {
   constexpr int kSlice = 4 * kThreads * V, kWaves = kThreads / 64;
