@@ -951,3 +951,20 @@ def test_attention_of_an_infinite_value(torch, okq, tn, d):
         for w in (want[0], want[2]):
             w[1, 2:, 5] = 0.0
         _attn_check(torch, (out, lse), want)
+
+
+@pytest.mark.parametrize("tn,d", [("BF16", 128), ("F16", 128), ("F16", 256), ("F32", 128), ("Q8_0", 128), ("BF16", 100)])
+def test_attention_of_an_infinite_query(torch, okq, tn, d):
+    """NaN in its head of its sequence, and all else as without it."""
+    print(f"[gpu] infinite query {tn} {d}", flush=True)
+    lengths = [40, 600]
+    cache, table, q = _attn_inputs(torch, okq, TYPES[tn], d, 2, 3, 16, lengths)
+    plain = _attention(torch, okq, cache, table, q, lengths, 600, d ** -0.5)
+    torch.cuda.synchronize()
+    for bad in (math.inf, -math.inf, math.nan):
+        q[1, 4, 9] = bad
+        out, lse = _attention(torch, okq, cache, table, q, lengths, 600, d ** -0.5)
+        torch.cuda.synchronize()
+        assert out[1, 4].isnan().all() and lse[1, 4].isnan()
+        out[1, 4], lse[1, 4] = plain[0][1, 4], plain[1][1, 4]
+        assert torch.equal(out, plain[0]) and torch.equal(lse, plain[1])
