@@ -370,6 +370,78 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
                               const int32_t *bias_len, const uint32_t *mask, int64_t mask_stride, float *out,
                               int64_t out_stride, int32_t *best, void *stream);
 
+/* ---- a layer's experts, and the step between two blocks ------------------- */
+
+/* From one block of a layer to the next, per row:
+ *   b = post_norm ? branch * (1 / sqrt(sum(branch^2) / hidden + epsilon)) * post_norm : branch
+ *   sum = residual_scale * x + branch_scale * gate * b
+ *   normed = sum * (1 / sqrt(sum(sum^2) / hidden + epsilon)) * pre_norm
+ * x, branch, sum: device f32, row r at r * its stride (elements).  post_norm,
+ * pre_norm [hidden] f32; gate: row r at r * gate_stride, 0 for one row that all
+ * share; post_norm and gate NULL: left out.  normed: rows of normed_type
+ * (OKQ_TYPE_F32, F16 or BF16, rounded to nearest even once), with pre_norm;
+ * both NULL: the sum alone.  sum may be NULL (normed alone), x or branch, with
+ * that one's stride; no other overlap.  Everything up to the stores is f32.
+ * rows == 0 is a no-op.  The reference's blocks add and normalise in steps of
+ * their own (crates/models/src/qwen/qwen2_5/prefill.rs). */
+okq_status okq_residual_norm(const float *x, int64_t x_stride, const float *branch, int64_t branch_stride, int64_t rows,
+                             int64_t hidden, const float *post_norm, const float *gate, int64_t gate_stride,
+                             float branch_scale, float residual_scale, const float *pre_norm, float epsilon, float *sum,
+                             int64_t sum_stride, void *normed, uint32_t normed_type, int64_t normed_stride,
+                             void *stream);
+
+/* How okq_moe_route turns logits into scores. */
+enum {
+    OKQ_SCORE_SOFTMAX = 0, /* over all experts of the row */
+    OKQ_SCORE_SIGMOID = 1
+};
+
+/* The experts of every row, and their weights:
+ *   z = x W^T + bias;  p = score(z);  c = p + choice_bias
+ *   groups > 1: the experts lie in that many equal groups, of which the
+ *     top_groups with the largest sum of their group_best (1 or 2) largest c
+ *     stay, ties to the lowest; the others' experts are not chosen
+ *   ids[r]: the top_k experts of largest c, largest first, ties to the lowest
+ *   weights[r]: their p, divided by their sum (zeros where it is 0) if
+ *     renormalise, times scale
+ * x: device f32, row r at r * x_stride; w [experts, hidden] of w_type
+ * (OKQ_TYPE_F32, F16 or BF16); bias, choice_bias [experts] f32 or NULL; ids
+ * [rows, top_k] int32, weights [rows, top_k] f32, logits [rows, experts] f32
+ * or NULL: z.  All of it is computed in 64 bits and rounded at the stores, so
+ * a row's experts do not change with the rows around it.  An expert of c =
+ * -infinity is never chosen: where too few are left, ids are -1 and weights
+ * 0.  A row with a NaN among its z or c gets ids of -1 and weights of NaN.
+ * experts at most 512, groups at most 64, top_k at most 64 and at most the
+ * experts of top_groups groups.  rows == 0 is a no-op.  Uses a per-stream
+ * workspace.  No counterpart in the reference, whose only sparse model is
+ * refused (crates/models/src/qwen/qwen3_5.rs). */
+okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, uint32_t w_type, const void *w,
+                         int64_t experts, const float *bias, int score, const float *choice_bias, int64_t groups,
+                         int64_t top_groups, int64_t group_best, int64_t top_k, int renormalise, float scale,
+                         int32_t *ids, float *weights, float *logits, void *stream);
+
+/* The gated MLP of every row's experts:
+ *   out[r] = sum_j weights[r, j] * down_e(silu(gate_e(x[r])) * up_e(x[r])),  e = ids[r, j]
+ * gate_w, up_w (of one type) and down_w: GGUF tensors stacked over the experts,
+ * [hidden, intermediate, experts] and [intermediate, hidden, experts] in ne
+ * order, types Q8_0, Q4_K, Q5_K or Q6_K; hidden and intermediate are multiples
+ * of the block of the tensors whose rows they are.  x, out: device f32, row r
+ * at r * its stride, x 16-byte aligned with a stride that is a multiple of 4.
+ * ids, weights [rows, top_k]; an id outside [0, experts) adds nothing whatever
+ * its weight is, so a row of such ids gets zeros; the same id twice in a row
+ * adds twice.  top_k at most 64.  Each expert's weights are read once for up
+ * to 16 of its rows.  Activations keep 22 bits, sums are f32; a row's result
+ * does not depend on the rows around it beyond the choice of a kernel by the
+ * call's sizes, nor on timing.  A row of x that holds an infinity or a NaN, or
+ * whose gated values do, gets NaN throughout (where it has an expert).  rows
+ * == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
+ * reference (crates/kernels/src/mlp.rs has the dense MLP). */
+okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, int64_t intermediate,
+                         int64_t experts, int64_t top_k, const int32_t *ids, const float *weights,
+                         uint32_t gate_up_type, const void *gate_w, uint64_t gate_bytes, const void *up_w,
+                         uint64_t up_bytes, uint32_t down_type, const void *down_w, uint64_t down_bytes, float *out,
+                         int64_t out_stride, void *stream);
+
 /* The next compute kernel this thread launches through okq_dequantize,
  * okq_linear_out_by_in_q*, okq_gemv or okq_gemm* records `start` and `stop`
  * (hipEvent_t, created with timing enabled) at the begin and end of its

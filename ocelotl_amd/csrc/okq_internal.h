@@ -286,4 +286,61 @@ struct LogitsArgs {
 size_t logits_workspace(int64_t rows);
 hipError_t launch_logits(const LogitsArgs &a, void *workspace, int cu_count, hipStream_t s);
 
+// ---- a layer's experts, and the step between two blocks ------------------------
+
+// okq_residual_norm's arguments; post, gate, sum, and pre with normed may be null.
+struct ResidualArgs {
+  const float *x, *branch, *post, *gate, *pre;
+  float *sum;
+  void *normed;
+  int64_t x_stride, branch_stride, gate_stride, sum_stride, normed_stride;
+  int64_t rows, hidden;
+  int normed_type;  // OKQ_TYPE_F32, F16 or BF16
+  float branch_scale, residual_scale, eps;
+};
+hipError_t launch_residual_norm(const ResidualArgs &a, hipStream_t s);
+
+constexpr int kMaxExperts = 512, kMaxGroups = 64, kMaxTopK = 64;
+struct RouteArgs {
+  const float *x;
+  int64_t x_stride;
+  const void *w;
+  const float *bias, *choice_bias;
+  int rows, hidden, experts, w_type;
+  int sigmoid, groups, top_groups, group_best, top_k, renormalise;
+  float scale;
+  int32_t *ids;
+  float *weights, *logits;
+};
+// How a call runs: the rows go in tiles of 16; a tile's products are one
+// workgroup's, or split over (expert tiles) x (slices of the row) and joined
+// by the one that finishes last.
+struct RoutePlan {
+  int tiles, slices, span;  // span: values of a slice
+  bool whole;
+  size_t part_bytes, arrived_bytes, lds;
+};
+RoutePlan route_plan(const RouteArgs &a, int cu_count);
+hipError_t launch_route(const RouteArgs &a, const RoutePlan &plan, void *part, void *arrived, hipStream_t s);
+
+// okq_moe_mlp_q's arguments; gate_up_type and down_type: linear formats.
+struct MoeArgs {
+  const float *x;
+  int64_t x_stride, out_stride;
+  int rows, hidden, inner, experts, top_k;
+  const int32_t *ids;
+  const float *weights;
+  int gate_up_type, down_type;
+  const uint8_t *gate, *up, *down;
+  float *out;
+};
+// The workspace, and how many rows a pass over it takes (longer batches go in
+// several).
+struct MoePlan {
+  int64_t pass_rows;
+  size_t off_inner, off_pair, workspace;
+};
+MoePlan moe_plan(const MoeArgs &a, int cu_count);
+hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s);
+
 }  // namespace okq

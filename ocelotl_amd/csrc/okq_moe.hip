@@ -1,0 +1,569 @@
+// okq_moe.hip -- the gated MLP of every token's experts over stacked GGUF
+// tensors [experts][rows][blocks], and the weighted sum of their results:
+//
+//   out[t] = sum_j weight[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),  e = ids[t, j]
+//
+// A pair is a token and one of its experts, t * top_k + j.  Two products over
+// the pairs, expert by expert, and a sum over each token's: gate and up
+// together, whose waves hold both sums of a column and leave silu(gate) * up;
+// down, which leaves every pair's weighted row; the sum in the order of j.
+//
+// Numerics.  A row's activations are scaled by a power of two for every 256
+// of them and split into two fp16 planes, x = hi + lo to 2^-22; the weights'
+// integer parts are exact in fp16 (okq_mfma.h), so every product is exact and
+// only f32 sums round.  A row that holds an infinity or a NaN gets a NaN scale.
+#include <algorithm>
+
+#include "okq_device.h"
+#include "okq_internal.h"
+#include "okq_mfma.h"
+
+namespace okq {
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kPassPairs = 4096;  // pairs of one pass (its list of an expert's lies in LDS)
+
+// ---- a lane's share of 16 columns x 256 values of K --------------------------------
+// v_mfma_f32_16x16x32_f16: lane l holds row / column l % 16 and, at step t,
+// eight of the values of lane group g = l / 16: those from at(t, g) on.
+
+__device__ __forceinline__ h8 join8(h2 a, h2 b, h2 c, h2 d) { return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+struct ExpQ4K {
+  static constexpr int kType = kQ4_K;
+  static constexpr bool kMins = true, kLow = false;
+  // nibble plane t & 1 of bytes 8 (t / 2) .. of qs chunk g
+  __device__ static int at(int t, int g) { return 64 * g + 32 * (t & 1) + 8 * (t >> 1); }
+  struct Item {
+    u32x4 hd, q0, q1;
+  };
+  __device__ static void load(Item &it, Rsrc rs, uint32_t blk, int g) {
+    it.hd = bload4(rs, blk);
+    it.q0 = bload4(rs, blk + 16u + 32u * (uint32_t)g);
+    it.q1 = bload4(rs, blk + 32u + 32u * (uint32_t)g);
+  }
+  // scales of the chunk's two sub-blocks as (multiplier, offset) of 1024 + q
+  // and of 1024 + 16 q; their mins
+  struct Cur {
+    h2 sc[2], off[2];
+    h8 m;
+    float d, dmin;
+  };
+  __device__ static Cur header(const u32x4 &hd, int g) {
+    Cur c;
+    const uint32_t k = 2u * ((uint32_t)g & 1u);
+    const uint32_t sc4 = g < 2 ? hd.y & 0x3F3F3F3Fu : (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
+    const uint32_t m4 = g < 2 ? hd.z & 0x3F3F3F3Fu : ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u);
+    const h2 s0 = byte_pair(sc4, k), s1 = byte_pair(sc4, k + 1u), m0 = byte_pair(m4, k), m1 = byte_pair(m4, k + 1u);
+    auto by = [](h2 v, float f) { return v * h2{(_Float16)f, (_Float16)f}; };
+    c.sc[0] = s0;
+    c.off[0] = by(s0, -1024.0f);
+    c.sc[1] = by(s1, 0.0625f);
+    c.off[1] = by(s1, -64.0f);
+    const h2 z = {(_Float16)0.0f, (_Float16)0.0f};
+    c.m = join8(m0, m1, z, z);
+    c.d = f16_bits_hw(hd.x & 0xffffu);
+    c.dmin = f16_bits_hw(hd.x >> 16);
+    return c;
+  }
+  __device__ static Cur begin(const Item &it, int g) { return header(it.hd, g); }
+  __device__ static void frag(const Item &it, const Cur &c, int t, int, h8 &b1, h8 &) {
+    const int nib = t & 1, p8 = t >> 1;
+    const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0;
+    const uint32_t d0 = (p8 & 1) ? pc.z : pc.x, d1 = (p8 & 1) ? pc.w : pc.y;
+    const uint32_t mask = nib ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+    h2 p0, p1, p2, p3;
+    nib4(d0 & mask, c.sc[nib], c.off[nib], p0, p1);
+    nib4(d1 & mask, c.sc[nib], c.off[nib], p2, p3);
+    b1 = join8(p0, p1, p2, p3);
+  }
+};
+
+// Q4_K with the fifth bit from qh: bit 2 g + nibble plane of qh[l] for byte l.
+struct ExpQ5K {
+  static constexpr int kType = kQ5_K;
+  static constexpr bool kMins = true, kLow = false;
+  __device__ static int at(int t, int g) { return ExpQ4K::at(t, g); }
+  struct Item {
+    u32x4 hd, h0, h1, q0, q1;
+  };
+  using Cur = ExpQ4K::Cur;
+  __device__ static void load(Item &it, Rsrc rs, uint32_t blk, int g) {
+    it.hd = bload4(rs, blk);
+    it.h0 = bload4(rs, blk + 16u);
+    it.h1 = bload4(rs, blk + 32u);
+    it.q0 = bload4(rs, blk + 48u + 32u * (uint32_t)g);
+    it.q1 = bload4(rs, blk + 64u + 32u * (uint32_t)g);
+  }
+  __device__ static Cur begin(const Item &it, int g) { return ExpQ4K::header(it.hd, g); }
+  __device__ static void frag(const Item &it, const Cur &c, int t, int g, h8 &b1, h8 &) {
+    const int nib = t & 1, p8 = t >> 1;
+    const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0, hc = (p8 >> 1) ? it.h1 : it.h0;
+    const uint32_t d0 = (p8 & 1) ? pc.z : pc.x, d1 = (p8 & 1) ? pc.w : pc.y;
+    const uint32_t e0 = (p8 & 1) ? hc.z : hc.x, e1 = (p8 & 1) ? hc.w : hc.y;
+    // bit 4 of the byte on the low plane (1024 + q5), the exponent byte
+    // 0x64 | h on the high one (1024 + 256 h + 16 q4)
+    const uint32_t sh = 2u * (uint32_t)g + (uint32_t)nib;
+    const uint32_t f0 = (e0 >> sh) & 0x01010101u, f1 = (e1 >> sh) & 0x01010101u;
+    const uint32_t n0 = nib ? d0 & 0xF0F0F0F0u : (d0 & 0x0F0F0F0Fu) | (f0 << 4);
+    const uint32_t n1 = nib ? d1 & 0xF0F0F0F0u : (d1 & 0x0F0F0F0Fu) | (f1 << 4);
+    const uint32_t x0 = nib ? f0 | 0x64646464u : 0x64646464u, x1 = nib ? f1 | 0x64646464u : 0x64646464u;
+    const uint32_t lo = nib ? 0x05010400u : 0x04010400u, hi = nib ? 0x07030602u : 0x04030402u;
+    b1 = join8(nib_pair(__builtin_amdgcn_perm(x0, n0, lo), c.sc[nib], c.off[nib]),
+               nib_pair(__builtin_amdgcn_perm(x0, n0, hi), c.sc[nib], c.off[nib]),
+               nib_pair(__builtin_amdgcn_perm(x1, n1, lo), c.sc[nib], c.off[nib]),
+               nib_pair(__builtin_amdgcn_perm(x1, n1, hi), c.sc[nib], c.off[nib]));
+  }
+};
+
+// Blocks of 210 bytes: every 8-byte field is a window of three dwords from the
+// one below it, realigned.  The window of d ends at most 2 bytes past the
+// block, in a dword that holds d.
+struct ExpQ6K {
+  static constexpr int kType = kQ6_K;
+  static constexpr bool kMins = false, kLow = true;
+  // half t / 4, quarter t % 4
+  __device__ static int at(int t, int g) { return 128 * (t >> 2) + 32 * (t & 3) + 8 * g; }
+  struct Item {
+    u32x3 ql[4], qh[2];  // ql: (half, quarter & 1)
+    u32x4 sc4;
+    uint32_t sc1, r;
+  };
+  struct Cur {
+    uint32_t L[4][2], H[2][2], S[4];
+    float d;
+  };
+  __device__ static void load(Item &it, Rsrc rs, uint32_t blk, int g) {
+    const uint32_t r = blk & 3u, a = blk - r;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      it.ql[p] = __builtin_amdgcn_raw_buffer_load_b96(rs, a + 64u * (uint32_t)(p >> 1) + 32u * (uint32_t)(p & 1) + 8u * (uint32_t)g, 0, 0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      it.qh[h] = __builtin_amdgcn_raw_buffer_load_b96(rs, a + 128u + 32u * (uint32_t)h + 8u * (uint32_t)g, 0, 0);
+    it.sc4 = bload4(rs, a + 192u);
+    it.sc1 = __builtin_amdgcn_raw_buffer_load_b32(rs, a + 208u, 0, 0);
+    it.r = r;
+  }
+  __device__ static Cur begin(const Item &it, int) {
+    Cur c;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      c.L[p][0] = realign(it.ql[p].y, it.ql[p].x, it.r);
+      c.L[p][1] = realign(it.ql[p].z, it.ql[p].y, it.r);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      c.H[h][0] = realign(it.qh[h].y, it.qh[h].x, it.r);
+      c.H[h][1] = realign(it.qh[h].z, it.qh[h].y, it.r);
+    }
+    c.S[0] = realign(it.sc4.y, it.sc4.x, it.r);
+    c.S[1] = realign(it.sc4.z, it.sc4.y, it.r);
+    c.S[2] = realign(it.sc4.w, it.sc4.z, it.r);
+    c.S[3] = realign(it.sc1, it.sc4.w, it.r);
+    c.d = f16_bits_hw((it.sc1 >> (8u * it.r)) & 0xffffu);
+    return c;
+  }
+  __device__ static void frag(const Item &, const Cur &c, int t, int g, h8 &b1, h8 &b2) {
+    const int hh = t >> 2, qq = t & 3;
+    const uint32_t *lq = c.L[2 * hh + (qq & 1)], *hq = c.H[hh];
+    const int sh4 = 4 * (qq >> 1), sh2 = 2 * qq;
+    const uint32_t q0 = ((lq[0] >> sh4) & 0x0F0F0F0Fu) | (((hq[0] >> sh2) & 0x03030303u) << 4);
+    const uint32_t q1 = ((lq[1] >> sh4) & 0x0F0F0F0Fu) | (((hq[1] >> sh2) & 0x03030303u) << 4);
+    const int sc = __builtin_amdgcn_sbfe((int)c.S[2 * hh + (qq >> 1)], 8u * (2u * (uint32_t)(qq & 1) + ((uint32_t)g >> 1)), 8u);
+    const _Float16 sf = (_Float16)(float)sc;
+    const h2 sc2 = {sf, sf};
+    h2 p0, p1, p2, p3, l0, l1, l2, l3;
+    q6_4(q0, sc2, p0, p1, l0, l1);
+    q6_4(q1, sc2, p2, p3, l2, l3);
+    b1 = join8(p0, p1, p2, p3);
+    b2 = join8(l0, l1, l2, l3);
+  }
+};
+
+// Eight blocks of 34 bytes, 2 g and 2 g + 1 the lane group's.  d goes into the
+// two exact planes of d * q.  A row of K not a multiple of 256 ends inside an
+// item: what follows it (the next row's blocks, or nothing) meets zeros.
+struct ExpQ80 {
+  static constexpr int kType = kQ8_0;
+  static constexpr bool kMins = false, kLow = true;
+  __device__ static int at(int t, int g) { return 64 * g + 8 * t; }
+  struct Item {
+    u32x4 w0, w1, w2, w3;
+    u32x2 w4;
+    uint32_t r;
+  };
+  struct Cur {
+    uint32_t w[17];
+    h2 d0, d1;
+    float d;
+  };
+  __device__ static void load(Item &it, Rsrc rs, uint32_t blk, int g) {
+    const uint32_t at = blk + 68u * (uint32_t)g, r = at & 3u, a = at - r;
+    it.w0 = bload4(rs, a);
+    it.w1 = bload4(rs, a + 16u);
+    it.w2 = bload4(rs, a + 32u);
+    it.w3 = bload4(rs, a + 48u);
+    it.w4 = __builtin_amdgcn_raw_buffer_load_b64(rs, a + 64u, 0, 0);
+    it.r = r;
+  }
+  __device__ static Cur begin(const Item &it, int) {
+    const uint32_t raw[18] = {it.w0.x, it.w0.y, it.w0.z, it.w0.w, it.w1.x, it.w1.y, it.w1.z, it.w1.w, it.w2.x,
+                              it.w2.y, it.w2.z, it.w2.w, it.w3.x, it.w3.y, it.w3.z, it.w3.w, it.w4.x, it.w4.y};
+    Cur c;
+#pragma unroll
+    for (int i = 0; i < 17; ++i) c.w[i] = realign(raw[i + 1], raw[i], it.r);
+    const _Float16 d0 = __builtin_bit_cast(_Float16, (uint16_t)(c.w[0] & 0xffffu));
+    const _Float16 d1 = __builtin_bit_cast(_Float16, (uint16_t)(c.w[8] >> 16));
+    c.d0 = h2{d0, d0};
+    c.d1 = h2{d1, d1};
+    c.d = 1.0f;
+    return c;
+  }
+  __device__ static void frag(const Item &, const Cur &c, int t, int, h8 &b1, h8 &b2) {
+    const int blk = t >> 2, o = 2 * (t & 3);
+    const uint32_t qa = blk ? c.w[9 + o] : realign(c.w[o + 1], c.w[o], 2u);
+    const uint32_t qb = blk ? c.w[10 + o] : realign(c.w[o + 2], c.w[o + 1], 2u);
+    h2 p0, p1, p2, p3, l0, l1, l2, l3;
+    q8_4(qa, blk ? c.d1 : c.d0, p0, p1, l0, l1);
+    q8_4(qb, blk ? c.d1 : c.d0, p2, p3, l2, l3);
+    b1 = join8(p0, p1, p2, p3);
+    b2 = join8(l0, l1, l2, l3);
+  }
+};
+
+// A lane's row of activations for one item: both planes' fragments, the sums
+// of its two sub-blocks of 32 as (hi, lo) pairs (Q4_K, Q5_K), and the scale.
+struct ActA {
+  h8 hi[8], lo[8], sums;
+  float scale;
+};
+
+template <class F>
+__device__ __forceinline__ void load_row(float4 raw[16], const float *row, int k0, int K, int g) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int k = k0 + F::at(t, g);
+    const bool in = F::kType != kQ8_0 || k < K;  // other formats' rows are whole items
+    const float4 *p = reinterpret_cast<const float4 *>(row + (in ? k : 0));
+    raw[2 * t] = p[0];
+    raw[2 * t + 1] = p[1];
+    if (!in) raw[2 * t] = raw[2 * t + 1] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+}
+
+// The lane groups of a row share their scale 2^s: the largest |x| of its 256
+// lies in [512, 1024).
+template <class F>
+__device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
+  uint32_t top = 0;
+  auto value = [&](int t, int e) {
+    const float4 v = raw[2 * t + (e >> 2)];
+    return (e & 3) == 0 ? v.x : (e & 3) == 1 ? v.y : (e & 3) == 2 ? v.z : v.w;
+  };
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = as_u32(value(t, e)) & 0x7fffffffu;  // NaN above infinity above every finite value
+      top = top > b ? top : b;
+    }
+  uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
+  top = top > o ? top : o;
+  o = (uint32_t)__shfl_xor((int)top, 32);
+  top = top > o ? top : o;
+  const bool odd = top >= 0x7f800000u;
+  const int s = top > 0 && !odd ? __builtin_amdgcn_frexp_expf(as_f32(top)) - 10 : 0;
+  A.scale = odd ? __builtin_nanf("") : ldexpf(1.0f, s);
+  float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = ldexpf(value(t, e), -s);
+      const _Float16 h = (_Float16)w, l = (_Float16)(w - (float)h);
+      A.hi[t][e] = h;
+      A.lo[t][e] = l;
+      if (F::kMins) sum[t & 1] += (float)h + (float)l;  // what the planes hold
+    }
+  if (F::kMins) {
+    const _Float16 h0 = (_Float16)sum[0], h1 = (_Float16)sum[1];
+    const _Float16 z = (_Float16)0.0f;
+    A.sums = h8{h0, (_Float16)(sum[0] - (float)h0), h1, (_Float16)(sum[1] - (float)h1), z, z, z, z};
+  }
+}
+
+// acc (rows 4 g .. 4 g + 3 of the lane's column) += the item's products; rs:
+// the rows' scales.
+template <class F>
+__device__ __forceinline__ void contract(f4 &acc, const typename F::Item &it, const ActA &A, const f4 &rs, int g) {
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  const typename F::Cur c = F::begin(it, g);
+  f4 s = zero;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    h8 b1, b2;
+    F::frag(it, c, t, g, b1, b2);
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.hi[t], b1, s, 0, 0, 0);
+    if constexpr (F::kLow) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.hi[t], b2, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.lo[t], b1, s, 0, 0, 0);  // lo * b2 is below 2^-22 of the product
+  }
+  if constexpr (F::kMins) {
+    const f4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.sums, c.m, zero, 0, 0, 0);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[v] = fmaf(rs[v], fmaf(-c.dmin, m[v], c.d * s[v]), acc[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[v] = fmaf(c.d * rs[v], s[v], acc[v]);
+  }
+}
+
+// One product over the pairs: y[p] = act(W_e x_p), p's expert e.
+struct MoeProduct {
+  const float *x;       // rows of K: of tokens (top_k pairs share one), or of pairs (share 1)
+  int64_t x_stride;
+  int share;
+  const uint8_t *w[2];  // stacked tensors of the pass: gate and up, or down
+  uint64_t w_bytes;     // of each
+  uint64_t expert_bytes;
+  const int32_t *ids;
+  const float *weights;  // down: a pair's factor
+  float *y;              // [pairs][N]
+  int pairs, experts, K, N, nsb, row_bytes;
+  int kw, slots;         // waves of a column tile, tiles side by side
+};
+
+}  // namespace
+
+// A workgroup has one expert's columns [slots * T tiles of 16]; its kw waves
+// of a tile share out K and meet in LDS.  It lists the expert's pairs from
+// ids by itself (a launch that did it for all would cost more than 4 us; the
+// ids are a few KB in the L2), so workgroups of experts without pairs end at
+// once.  With fewer pairs than experts a workgroup has a pair's expert, and
+// goes on if no earlier pair has the same.  Rows go 16 at a time: a row's
+// activations stay in registers while T column tiles' weights pass, and the
+// next items are in flight behind the current ones.
+template <class F, int NM, int T>
+__global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
+  __shared__ uint16_t list[kPassPairs];
+  __shared__ int count[kWaves];
+  __shared__ f4 red[kWaves][NM * T][64];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int waves = (int)blockDim.x >> 6;
+  const int n = lane & 15, g = lane >> 4;
+  const int job = (int)blockIdx.y;
+  const bool by_pair = a.pairs < a.experts;
+  const int e = by_pair ? __builtin_amdgcn_readfirstlane(a.ids[job]) : job;
+  if (e < 0 || e >= a.experts) return;
+
+  // the expert's pairs in order: every wave counts its share of the ids, then
+  // writes behind the waves before it
+  const int share = (a.pairs + 64 * waves - 1) / (64 * waves) * 64, lo = wave * share, hi = std::min(a.pairs, lo + share);
+  int mine = 0;
+  for (int p = lo; p < hi; p += 64)
+    mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p + lane < hi && a.ids[std::min(p + lane, hi - 1)] == e));
+  if (lane == 0) count[wave] = mine;
+  __syncthreads();
+  int at = 0, m = 0;
+  for (int w = 0; w < waves; ++w) {
+    at += w < wave ? count[w] : 0;
+    m += count[w];
+  }
+  if (mine)
+    for (int p = lo; p < hi; p += 64) {
+      const bool hit = p + lane < hi && a.ids[std::min(p + lane, hi - 1)] == e;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(hit);
+      if (hit) list[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = (uint16_t)(p + lane);
+      at += __builtin_popcountll(mask);
+    }
+  __syncthreads();
+  if (m == 0 || (by_pair && list[0] != job)) return;
+
+  const int slot = wave / a.kw, ks = wave - slot * a.kw;
+  const int tile0 = ((int)blockIdx.x * a.slots + slot) * T;
+  const uint32_t sb = (uint32_t)(F::kType == kQ8_0 ? 8 * kQ8Bytes : sb_bytes_of(F::kType));
+  // the expert's weights from the dword at or below its first byte, to the
+  // last dword that holds a byte of the stack
+  Rsrc rs[NM];
+  uint32_t skew[NM];
+#pragma unroll
+  for (int i = 0; i < NM; ++i) {
+    const uint64_t from = (uint64_t)e * a.expert_bytes;
+    const uint8_t *base = a.w[i] + from;
+    skew[i] = (uint32_t)(reinterpret_cast<uintptr_t>(base) & 3u);
+    const uint64_t left = (a.w_bytes - from + skew[i] + 3u) & ~3ull;
+    rs[i] = make_rsrc(base - skew[i], (uint32_t)std::min<uint64_t>(left, 0xFFFFFFFCull));
+  }
+  uint32_t col_at[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) col_at[t] = (uint32_t)std::min((tile0 + t) * 16 + n, a.N - 1) * (uint32_t)a.row_bytes;
+  typename F::Item S[NM * T];
+  auto load_item = [&](int i, int s) {
+    const uint32_t blk = col_at[i / NM] + skew[i % NM] + (uint32_t)s * sb;
+    F::load(S[i], rs[i % NM], s < a.nsb ? blk : 0xFFFFF000u, g);
+  };
+
+  for (int r0 = 0; r0 < m; r0 += 16) {
+    const int p = list[std::min(r0 + n, m - 1)];
+    const float *row = a.x + (int64_t)(p / a.share) * a.x_stride;
+    f4 acc[NM * T];
+#pragma unroll
+    for (int i = 0; i < NM * T; ++i) acc[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NM * T; ++i) load_item(i, ks);
+    for (int s = ks; s < a.nsb; s += a.kw) {
+      ActA A;
+      {
+        float4 raw[16];
+        load_row<F>(raw, row, s * 256, a.K, g);
+        convert<F>(A, raw);
+      }
+      f4 scales;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) scales[v] = __shfl(A.scale, 4 * g + v);
+#pragma unroll
+      for (int i = 0; i < NM * T; ++i) {
+        contract<F>(acc[i], S[i], A, scales, g);
+        load_item(i, s + a.kw);
+      }
+    }
+    // the tile's waves meet in their order
+    if (r0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NM * T; ++i) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (ks == 0) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        f4 sum[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+          sum[i] = red[wave][NM * t + i][lane];
+          for (int w = 1; w < a.kw; ++w) sum[i] += red[wave + w][NM * t + i][lane];
+        }
+        const int col = (tile0 + t) * 16 + n;
+        if (col < a.N)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (r0 + 4 * g + v < m) {
+              const int q = list[r0 + 4 * g + v];
+              float y = sum[0][v];
+              if constexpr (NM == 2) y = (y * (1.0f / (1.0f + expf(-y)))) * sum[1][v];
+              else y *= a.weights[q];
+              a.y[(int64_t)q * a.N + col] = y;
+            }
+      }
+    }
+  }
+}
+
+// out[t] = the sum of its pairs' rows, in their order; zeros for none.
+template <int N>
+__global__ __launch_bounds__(256) void moe_sum_kernel(const float *__restrict__ y, const int32_t *__restrict__ ids,
+                                                      int top_k, int experts, int hidden, float *__restrict__ out,
+                                                      int64_t out_stride) {
+  typedef float fN __attribute__((ext_vector_type(N)));
+  const int64_t t = blockIdx.y;
+  const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * N;
+  if (c >= hidden) return;
+  fN sum = {};
+  for (int j = 0; j < top_k; ++j)
+    if ((uint32_t)ids[t * top_k + j] < (uint32_t)experts)
+      sum += *reinterpret_cast<const fN *>(y + (t * top_k + j) * hidden + c);
+  *reinterpret_cast<fN *>(out + t * out_stride + c) = sum;
+}
+
+static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+MoePlan moe_plan(const MoeArgs &a, int) {
+  MoePlan p{};
+  p.pass_rows = std::min<int64_t>(a.rows, kPassPairs / a.top_k);
+  const size_t pairs = (size_t)p.pass_rows * a.top_k;
+  p.off_inner = 0;
+  p.off_pair = up256(pairs * a.inner * sizeof(float));
+  p.workspace = p.off_pair + up256(pairs * a.hidden * sizeof(float));
+  return p;
+}
+
+template <class F, int NM>
+static hipError_t launch_product(MoeProduct a, int cu_count, hipStream_t s) {
+  // as few rounds of super-blocks a wave as eight waves leave, then as few
+  // waves as that takes; the others take further column tiles
+  const int rounds = (a.nsb + kWaves - 1) / kWaves;
+  a.kw = (a.nsb + rounds - 1) / rounds;
+  a.slots = kWaves / a.kw;
+  const int tiles = (a.N + 15) / 16, jobs = std::min(a.pairs, a.experts);
+  const dim3 block(64 * a.kw * a.slots);
+  // two tiles a wave halve what a row's activations cost; one where the
+  // workgroups would not go round
+  if ((int64_t)jobs * ((tiles + 2 * a.slots - 1) / (2 * a.slots)) >= 4 * cu_count)
+    launch_timed(moe_stream_kernel<F, NM, 2>, dim3((tiles + 2 * a.slots - 1) / (2 * a.slots), jobs), block, 0u, s, a);
+  else
+    launch_timed(moe_stream_kernel<F, NM, 1>, dim3((tiles + a.slots - 1) / a.slots, jobs), block, 0u, s, a);
+  return hipGetLastError();
+}
+
+template <int NM>
+static hipError_t launch_product(int type, const MoeProduct &a, int cu_count, hipStream_t s) {
+  if (type == kQ4_K) return launch_product<ExpQ4K, NM>(a, cu_count, s);
+  if (type == kQ5_K) return launch_product<ExpQ5K, NM>(a, cu_count, s);
+  if (type == kQ6_K) return launch_product<ExpQ6K, NM>(a, cu_count, s);
+  return launch_product<ExpQ80, NM>(a, cu_count, s);
+}
+
+static MoeProduct product(int type, int K, int N, int experts) {
+  MoeProduct p{};
+  p.K = K;
+  p.N = N;
+  p.experts = experts;
+  p.nsb = (K + 255) / 256;
+  p.row_bytes = type == kQ8_0 ? K / 32 * kQ8Bytes : K / 256 * sb_bytes_of(type);
+  p.expert_bytes = (uint64_t)N * (uint64_t)p.row_bytes;
+  p.w_bytes = p.expert_bytes * (uint64_t)experts;
+  return p;
+}
+
+hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s) {
+  float *inner = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.off_inner);
+  float *pair = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.off_pair);
+  for (int64_t t0 = 0; t0 < a.rows; t0 += plan.pass_rows) {
+    const int64_t rows = std::min<int64_t>(plan.pass_rows, a.rows - t0);
+    MoeProduct g = product(a.gate_up_type, a.hidden, a.inner, a.experts);
+    g.x = a.x + t0 * a.x_stride;
+    g.x_stride = a.x_stride;
+    g.share = a.top_k;
+    g.w[0] = a.gate;
+    g.w[1] = a.up;
+    g.ids = a.ids + t0 * a.top_k;
+    g.y = inner;
+    g.pairs = (int)(rows * a.top_k);
+    hipError_t e = launch_product<2>(a.gate_up_type, g, cu_count, s);
+    if (e != hipSuccess) return e;
+    MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
+    d.x = inner;
+    d.x_stride = a.inner;
+    d.share = 1;
+    d.w[0] = a.down;
+    d.ids = g.ids;
+    d.weights = a.weights + t0 * a.top_k;
+    d.y = pair;
+    d.pairs = g.pairs;
+    e = launch_product<1>(a.down_type, d, cu_count, s);
+    if (e != hipSuccess) return e;
+    float *out = a.out + t0 * a.out_stride;
+    const bool wide = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && a.out_stride % 4 == 0;
+    const int n = wide ? 4 : 1;
+    const dim3 grid((unsigned)((a.hidden / n + 255) / 256), (unsigned)rows);
+    if (wide)
+      launch_timed(moe_sum_kernel<4>, grid, dim3(256), 0u, s, (const float *)pair, g.ids, a.top_k, a.experts, a.hidden, out, a.out_stride);
+    else
+      launch_timed(moe_sum_kernel<1>, grid, dim3(256), 0u, s, (const float *)pair, g.ids, a.top_k, a.experts, a.hidden, out, a.out_stride);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace okq

@@ -233,7 +233,9 @@ std::map<std::tuple<int, hipStream_t, int>, Workspace> g_ws;
 // Slot 0 serves the linear itself (GEMM planes, bf16 widening); slot 1 holds
 // a neighbour's output (normalised or gated activations) that a linear then
 // reads, so the two never alias; slot 2 the keys of okq_logits_process, slots
-// 3 and 4 the chunks' results and the counters of okq_paged_attention.
+// 3 and 4 the chunks' results and the counters of okq_paged_attention, slots 5
+// and 6 the slices' products and the counters of okq_moe_route, slot 7 what
+// okq_moe_mlp_q keeps between its launches.
 enum class Grow { Ok, Capture, Alloc };
 
 // At least `bytes`; a buffer that has to grow, or could outside a capture,
@@ -491,15 +493,15 @@ okq_status validate_pages(const char *what, const okq_kv_pages &c, okq::KvPages 
   return ok();
 }
 
-// `rows` rows of `width` 4-byte elements, `stride` apart.
+// `rows` rows of `width` elements of `size` bytes, `stride` apart.
 okq_status validate_rows(const char *what, const char *name, const void *p, int64_t rows, int64_t width,
-                         int64_t stride) {
+                         int64_t stride, unsigned size = 4) {
   int64_t n;
   if (stride < (rows > 1 ? width : 0) || !mul_ok(rows, std::max(stride, width), n) || n > INT64_MAX / 8)
     return fail(OKQ_E_SHAPE, "%s %s stride=%lld does not hold rows of %lld, or overflows", what, name,
                 (long long)stride, (long long)width);
   if (!p) return fail(OKQ_E_ARG, "%s %s is null", what, name);
-  if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(OKQ_E_ALIGN, "%s %s must be 4-byte aligned", what, name);
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(OKQ_E_ALIGN, "%s %s must be %u-byte aligned", what, name, size);
   return ok();
 }
 
@@ -1367,6 +1369,204 @@ okq_status okq_logits_process(const float *logits, int64_t logits_stride, int64_
     if (st != OKQ_OK) return st;
   }
   return hip_status(okq::launch_logits(a, ws, info.cu_count, s), "logits_process launch");
+}
+
+okq_status okq_residual_norm(const float *x, int64_t x_stride, const float *branch, int64_t branch_stride, int64_t rows,
+                             int64_t hidden, const float *post_norm, const float *gate, int64_t gate_stride,
+                             float branch_scale, float residual_scale, const float *pre_norm, float epsilon, float *sum,
+                             int64_t sum_stride, void *normed, uint32_t normed_type, int64_t normed_stride,
+                             void *stream) {
+  const char *what = "residual_norm";
+  if (rows < 0 || hidden < 1 || rows >= 1 << 22 || hidden > INT32_MAX)  // a workgroup of up to 1024 threads a row
+    return fail(OKQ_E_SHAPE, "%s rows=%lld hidden=%lld: hidden must be at least 1 and below 2^31, rows below 2^22", what,
+                (long long)rows, (long long)hidden);
+  if (!(epsilon >= 0.0f) || epsilon == INFINITY || !std::isfinite(branch_scale) || !std::isfinite(residual_scale))
+    return fail(OKQ_E_ARG, "%s epsilon must be finite and non-negative and the scales finite, got %g, %g and %g", what,
+                epsilon, branch_scale, residual_scale);
+  if (!normed != !pre_norm) return fail(OKQ_E_ARG, "%s normed and pre_norm come together", what);
+  if (!normed && !sum) return fail(OKQ_E_ARG, "%s needs sum or normed", what);
+  if (normed && normed_type != OKQ_TYPE_F32 && normed_type != OKQ_TYPE_F16 && normed_type != OKQ_TYPE_BF16)
+    return fail(OKQ_E_TYPE, "unsupported %s output: tensor type %s (%u); supported: F32, F16, BF16", what,
+                type_name(normed_type), normed_type);
+  if (rows == 0) return ok();
+  okq_status st = validate_rows(what, "x", x, rows, hidden, x_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "branch", branch, rows, hidden, branch_stride);
+  if (st == OKQ_OK && post_norm) st = validate_rows(what, "post_norm", post_norm, 1, hidden, hidden);
+  if (st == OKQ_OK && gate) st = validate_rows(what, "gate", gate, gate_stride ? rows : 1, hidden, gate_stride);
+  if (st == OKQ_OK && pre_norm) st = validate_rows(what, "pre_norm", pre_norm, 1, hidden, hidden);
+  if (st == OKQ_OK && sum) st = validate_rows(what, "sum", sum, rows, hidden, sum_stride);
+  if (st == OKQ_OK && normed) st = validate_rows(what, "normed", normed, rows, hidden, normed_stride, normed_type == OKQ_TYPE_F32 ? 4 : 2);
+  if (st != OKQ_OK) return st;
+  if ((sum == x && sum_stride != x_stride) || (sum == branch && sum_stride != branch_stride))
+    return fail(OKQ_E_SHAPE, "%s sum_stride=%lld: a sum in place keeps the stride of the rows that it replaces", what,
+                (long long)sum_stride);
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  okq::ResidualArgs a{};
+  a.x = x;
+  a.branch = branch;
+  a.post = post_norm;
+  a.gate = gate;
+  a.pre = pre_norm;
+  a.sum = sum;
+  a.normed = normed;
+  a.x_stride = x_stride;
+  a.branch_stride = branch_stride;
+  a.gate_stride = gate_stride;
+  a.sum_stride = sum_stride;
+  a.normed_stride = normed_stride;
+  a.rows = rows;
+  a.hidden = hidden;
+  a.normed_type = (int)normed_type;
+  a.branch_scale = branch_scale;
+  a.residual_scale = residual_scale;
+  a.eps = epsilon;
+  return hip_status(okq::launch_residual_norm(a, static_cast<hipStream_t>(stream)), "residual_norm launch");
+}
+
+okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, uint32_t w_type, const void *w,
+                         int64_t experts, const float *bias, int score, const float *choice_bias, int64_t groups,
+                         int64_t top_groups, int64_t group_best, int64_t top_k, int renormalise, float scale,
+                         int32_t *ids, float *weights, float *logits, void *stream) {
+  const char *what = "moe_route";
+  if (w_type != OKQ_TYPE_F32 && w_type != OKQ_TYPE_F16 && w_type != OKQ_TYPE_BF16)
+    return fail(OKQ_E_TYPE, "unsupported %s weight: tensor type %s (%u); supported: F32, F16, BF16", what,
+                type_name(w_type), w_type);
+  if (rows < 0 || hidden < 1 || experts < 1 || rows > INT32_MAX || hidden > 1 << 30 || experts > okq::kMaxExperts)
+    return fail(OKQ_E_SHAPE, "%s rows=%lld hidden=%lld experts=%lld: hidden must be 1 to 2^30, experts 1 to %d", what,
+                (long long)rows, (long long)hidden, (long long)experts, okq::kMaxExperts);
+  if (groups < 1 || groups > okq::kMaxGroups || experts % groups != 0 || top_groups < 1 || top_groups > groups)
+    return fail(OKQ_E_SHAPE, "%s groups=%lld top_groups=%lld: up to %d equal groups of %lld experts, top_groups 1 to groups",
+                what, (long long)groups, (long long)top_groups, okq::kMaxGroups, (long long)experts);
+  if (top_k < 1 || top_k > okq::kMaxTopK || top_k > experts / groups * top_groups)
+    return fail(OKQ_E_SHAPE, "%s top_k=%lld must be 1 to %d and at most the %lld experts of top_groups groups", what,
+                (long long)top_k, okq::kMaxTopK, (long long)(experts / groups * top_groups));
+  if (score != OKQ_SCORE_SOFTMAX && score != OKQ_SCORE_SIGMOID)
+    return fail(OKQ_E_ARG, "%s score=%d must be OKQ_SCORE_SOFTMAX or OKQ_SCORE_SIGMOID", what, score);
+  if (group_best != 1 && group_best != 2) return fail(OKQ_E_ARG, "%s group_best=%lld must be 1 or 2", what, (long long)group_best);
+  if (!std::isfinite(scale)) return fail(OKQ_E_ARG, "%s scale must be finite, got %g", what, scale);
+  if (rows == 0) return ok();
+  okq_status st = validate_rows(what, "x", x, rows, hidden, x_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "ids", ids, rows, top_k, top_k);
+  if (st == OKQ_OK) st = validate_rows(what, "weights", weights, rows, top_k, top_k);
+  if (st == OKQ_OK && logits) st = validate_rows(what, "logits", logits, rows, experts, experts);
+  if (st == OKQ_OK && bias) st = validate_rows(what, "bias", bias, 1, experts, experts);
+  if (st == OKQ_OK && choice_bias) st = validate_rows(what, "choice_bias", choice_bias, 1, experts, experts);
+  if (st != OKQ_OK) return st;
+  if (!w) return fail(OKQ_E_ARG, "%s w is null", what);
+  if (reinterpret_cast<uintptr_t>(w) & (w_type == OKQ_TYPE_F32 ? 3u : 1u))
+    return fail(OKQ_E_ALIGN, "%s w must be aligned to its elements", what);
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  okq::RouteArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.w = w;
+  a.bias = bias;
+  a.choice_bias = choice_bias;
+  a.rows = (int)rows;
+  a.hidden = (int)hidden;
+  a.experts = (int)experts;
+  a.w_type = (int)w_type;
+  a.sigmoid = score == OKQ_SCORE_SIGMOID;
+  a.groups = (int)groups;
+  a.top_groups = (int)top_groups;
+  a.group_best = (int)group_best;
+  a.top_k = (int)top_k;
+  a.renormalise = renormalise != 0;
+  a.scale = scale;
+  a.ids = ids;
+  a.weights = weights;
+  a.logits = logits;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
+  const okq::RoutePlan plan = okq::route_plan(a, info.cu_count);
+  void *part = nullptr, *arrived = nullptr;
+  if (plan.part_bytes) {
+    st = get_workspace(dev, s, plan.part_bytes, &part, 5, what);
+    if (st == OKQ_OK) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 6, what);
+    if (st != OKQ_OK) return st;
+  }
+  return hip_status(okq::launch_route(a, plan, part, arrived, s), "moe_route launch");
+}
+
+okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, int64_t intermediate,
+                         int64_t experts, int64_t top_k, const int32_t *ids, const float *weights,
+                         uint32_t gate_up_type, const void *gate_w, uint64_t gate_bytes, const void *up_w,
+                         uint64_t up_bytes, uint32_t down_type, const void *down_w, uint64_t down_bytes, float *out,
+                         int64_t out_stride, void *stream) {
+  const char *what = "moe_mlp";
+  if (rows < 0 || experts < 1 || rows > INT32_MAX || experts > 1 << 16)
+    return fail(OKQ_E_SHAPE, "%s rows=%lld experts=%lld: experts must be 1 to 65536", what, (long long)rows, (long long)experts);
+  if (top_k < 1 || top_k > okq::kMaxTopK)
+    return fail(OKQ_E_SHAPE, "%s top_k=%lld must be 1 to %d", what, (long long)top_k, okq::kMaxTopK);
+  const struct Tensor {
+    const char *name;
+    int64_t K, N;
+    uint32_t type;
+    const void *w;
+    uint64_t bytes;
+  } tensors[3] = {{"gate", hidden, intermediate, gate_up_type, gate_w, gate_bytes},
+                  {"up", hidden, intermediate, gate_up_type, up_w, up_bytes},
+                  {"down", intermediate, hidden, down_type, down_w, down_bytes}};
+  for (const Tensor &t : tensors) {
+    TypeInfo ti;
+    if (!type_info(t.type, ti) || !ti.linear) return unsupported_type(t.type, "moe_mlp weight");
+    if (t.K < 1 || t.N < 1 || t.K > INT32_MAX / 2 || t.N > INT32_MAX / 2 || t.K % ti.elems != 0)
+      return fail(OKQ_E_SHAPE, "%s %s rows of %lld values for %lld outputs: not a positive multiple of the %s block size %lld, or too large",
+                  what, t.name, (long long)t.K, (long long)t.N, type_name(t.type), (long long)ti.elems);
+    int64_t one, all;
+    if (!mul_ok(t.N, t.K / ti.elems * ti.bytes, one) || one > (int64_t)UINT32_MAX - 1024 || !mul_ok(one, experts, all))
+      return fail(OKQ_E_SHAPE, "%s %s: an expert of 4 GiB or more", what, t.name);
+    if ((uint64_t)all != t.bytes)
+      return fail(OKQ_E_SHAPE, "%s %s bytes=%llu does not match experts*outputs*row_bytes=%lld*%lld*%lld=%lld", what,
+                  t.name, (unsigned long long)t.bytes, (long long)experts, (long long)t.N, (long long)(one / t.N),
+                  (long long)all);
+  }
+  if (rows == 0) return ok();
+  okq_status st = validate_rows(what, "x", x, rows, hidden, x_stride);
+  if (st == OKQ_OK) st = validate_rows(what, "ids", ids, rows, top_k, top_k);
+  if (st == OKQ_OK) st = validate_rows(what, "weights", weights, rows, top_k, top_k);
+  if (st == OKQ_OK) st = validate_rows(what, "out", out, rows, hidden, out_stride);
+  if (st != OKQ_OK) return st;
+  for (const Tensor &t : tensors) {
+    if (!t.w) return fail(OKQ_E_ARG, "%s %s weight is null", what, t.name);
+    if (reinterpret_cast<uintptr_t>(t.w) & 3u) return fail(OKQ_E_ALIGN, "%s %s weight must be 4-byte aligned", what, t.name);
+  }
+  if ((reinterpret_cast<uintptr_t>(x) & 15u) || (rows > 1 && x_stride % 4 != 0))
+    return fail(OKQ_E_ALIGN, "%s x must be 16-byte aligned and x_stride=%lld a multiple of 4", what, (long long)x_stride);
+  int dev;
+  DevInfo info;
+  st = current_device(dev, info);
+  if (st != OKQ_OK) return st;
+  okq::MoeArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.out_stride = out_stride;
+  a.rows = (int)rows;
+  a.hidden = (int)hidden;
+  a.inner = (int)intermediate;
+  a.experts = (int)experts;
+  a.top_k = (int)top_k;
+  a.ids = ids;
+  a.weights = weights;
+  a.gate_up_type = (int)gate_up_type;
+  a.down_type = (int)down_type;
+  a.gate = static_cast<const uint8_t *>(gate_w);
+  a.up = static_cast<const uint8_t *>(up_w);
+  a.down = static_cast<const uint8_t *>(down_w);
+  a.out = out;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
+  const okq::MoePlan plan = okq::moe_plan(a, info.cu_count);
+  void *ws = nullptr;
+  st = get_workspace(dev, s, plan.workspace, &ws, 7, what);
+  if (st != OKQ_OK) return st;
+  return hip_status(okq::launch_moe(a, plan, ws, info.cu_count, s), "moe_mlp launch");
 }
 
 okq_status okq_linear_out_by_in_q_noalloc(const float *x, int64_t rows, int64_t in_features, uint32_t w_type,

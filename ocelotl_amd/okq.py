@@ -68,6 +68,12 @@ SIGNATURES = {
                                    _vp, _vp]),
     "okq_logits_process": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
                                   _vp, _i64, _vp, _i64, _vp, _vp]),
+    "okq_residual_norm": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _f32, _f32, _vp, _f32, _vp, _i64, _vp,
+                                 _u32, _i64, _vp]),
+    "okq_moe_route": (_int, [_vp, _i64, _i64, _i64, _u32, _vp, _i64, _vp, _int, _vp, _i64, _i64, _i64, _i64, _int, _f32,
+                             _vp, _vp, _vp, _vp]),
+    "okq_moe_mlp_q": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _u32, _vp, _u64, _vp, _u64, _u32, _vp,
+                             _u64, _vp, _i64, _vp]),
     "okq_set_launch_events": (_int, [_vp, _vp]),
     "okq_quantize": (_int, [_u32, _vp, _i64, _vp, _vp]),
     "okq_fill_normal": (_int, [_u64, _i64, _i64, ctypes.c_float, _vp, _vp]),
