@@ -429,7 +429,7 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
  * at r * its stride, x 16-byte aligned with a stride that is a multiple of 4.
  * ids, weights [rows, top_k]; an id outside [0, experts) adds nothing whatever
  * its weight is, so a row of such ids gets zeros; the same id twice in a row
- * adds twice.  top_k at most 64.  Each expert's weights are read once for up
+ * adds twice.  experts at most 4096, top_k at most 64.  Each expert's weights are read once for up
  * to 16 of its rows.  Activations keep 22 bits, sums are f32; a row's result
  * does not depend on the rows around it beyond the choice of a kernel by the
  * call's sizes, nor on timing.  A row of x that holds an infinity or a NaN, or

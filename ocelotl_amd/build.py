@@ -38,6 +38,7 @@ EXTRA = {"okq_prep.hip": ["-ffp-contract=off"], "okq_gemv.hip": ["-ffp-contract=
          "okq_gemm_q6.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "okq_gemm_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "okq_moe.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "okq_experts.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "okq_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

@@ -334,13 +334,38 @@ struct MoeArgs {
   const uint8_t *gate, *up, *down;
   float *out;
 };
+constexpr int kMoeMaxExperts = 4096;  // counted in LDS
 // The workspace, and how many rows a pass over it takes (longer batches go in
-// several).
+// several).  tiled: the pairs sorted by expert into MFMA tiles of up to 128
+// rows (okq_experts.hip); else each expert's weights stream past 16 of its
+// rows at a time.
 struct MoePlan {
+  bool tiled;
   int64_t pass_rows;
-  size_t off_inner, off_pair, workspace;
+  size_t off_inner, off_pair, off_order, off_x, workspace;
 };
 MoePlan moe_plan(const MoeArgs &a, int cu_count);
 hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s);
+
+// Rows of one expert that share MFMA tiles: [row0, row0 + rows) of the pairs
+// sorted by expert, blocks of 32 (1 to 4).
+struct ExpertTile {
+  int expert, row0, rows, blocks;
+};
+// An expert product over those tiles.
+struct ExpertMat {
+  const uint8_t *w[2];  // stacks: gate and up, or down
+  uint64_t w_bytes, expert_bytes;
+  const int *order;      // sorted place -> pair
+  const float *weights;  // of the pairs
+  float *y;              // [place][n]
+  int n, row_bytes, top_k;
+};
+// Most tiles that `pairs` of `experts` can take, and the launch over those that
+// `tiles` (behind a count of them) names: x as planes of M rows of K.
+inline int64_t expert_tiles(int64_t pairs, int64_t experts) { return pairs / 128 + (experts < pairs ? experts : pairs); }
+hipError_t launch_experts(int type, bool gate_up, const _Float16 *xhi, const _Float16 *xlo, const void *xsum,
+                          const float *rscale, int M, int K, const ExpertMat &mat, const int *count,
+                          const ExpertTile *tiles, int64_t most_tiles, hipStream_t s);
 
 }  // namespace okq

@@ -459,32 +459,234 @@ __global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
   }
 }
 
-// out[t] = the sum of its pairs' rows, in their order; zeros for none.
+// ---- many rows: the pairs sorted by expert ------------------------------------------
+
+// order: the pairs by expert; place: each pair's place in it (-1: no such
+// expert); count: tiles, and pairs with an expert; the tiles.  One workgroup:
+// the ids of 4096 tokens are 128 KB, and their counts meet in LDS.  (Pairs of
+// an expert come in any order: a row's result does not depend on its place.)
+__global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs, int experts,
+                                                        int *__restrict__ order, int *__restrict__ place,
+                                                        int *__restrict__ count, ExpertTile *__restrict__ tiles) {
+  constexpr int kPer = kMoeMaxExperts / 1024;
+  __shared__ int next[kMoeMaxExperts];
+  __shared__ int2 waves[16];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int e = tid; e < kMoeMaxExperts; e += 1024) next[e] = 0;
+  __syncthreads();
+#pragma unroll 8
+  for (int p = tid; p < pairs; p += 1024) {
+    const int e = ids[p];
+    if ((uint32_t)e < (uint32_t)experts) atomicAdd(&next[e], 1);
+  }
+  __syncthreads();
+  // rows and tiles ahead of each expert: kPer experts a thread
+  int m[kPer], rows = 0, mine = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    m[i] = next[kPer * tid + i];
+    rows += m[i];
+    mine += (m[i] + 127) / 128;
+  }
+  int r = rows, t = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int ro = __shfl_up(r, d), to = __shfl_up(t, d);
+    r += lane >= d ? ro : 0;
+    t += lane >= d ? to : 0;
+  }
+  if (lane == 63) waves[wave] = int2{r, t};
+  __syncthreads();
+  r -= rows;
+  t -= mine;
+  for (int w = 0; w < wave; ++w) {
+    r += waves[w].x;
+    t += waves[w].y;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    next[kPer * tid + i] = r;
+    for (int at = 0; at < m[i]; at += 128) {
+      const int n = m[i] - at < 128 ? m[i] - at : 128;
+      tiles[t++] = ExpertTile{kPer * tid + i, r + at, n, (n + 31) / 32};
+    }
+    r += m[i];
+  }
+  if (tid == 1023) {
+    count[0] = t;
+    count[1] = r;
+  }
+  __syncthreads();
+#pragma unroll 8
+  for (int p = tid; p < pairs; p += 1024) {
+    const int e = ids[p];
+    int at = -1;
+    if ((uint32_t)e < (uint32_t)experts) {
+      at = atomicAdd(&next[e], 1);
+      order[at] = p;
+    }
+    place[p] = at;
+  }
+}
+
+// Rows of K values as two fp16 planes of rows of Kp (zeros behind K), their
+// per-32 sums and scales: a wave a row, CH chunks of 8 values a lane (0: as
+// many as the row has, read twice).  count: rows that there are, where only
+// the device knows.
+template <int CH>
+__global__ __launch_bounds__(256) void moe_planes_kernel(const float *__restrict__ x, int64_t x_stride, int rows,
+                                                         const int *__restrict__ count, int K, int Kp,
+                                                         _Float16 *__restrict__ hi, _Float16 *__restrict__ lo,
+                                                         h2 *__restrict__ sums, float *__restrict__ rscale) {
+  const int lane = (int)threadIdx.x & 63, row = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+  if (row >= (count ? count[1] : rows)) return;
+  const float *from = x + (int64_t)row * x_stride;
+  const int chunks = Kp / 8, full = K / 8;
+  auto get = [&](int c, float v[8]) {
+    const float4 *p = reinterpret_cast<const float4 *>(from + 8 * (c < full ? c : 0));
+    const float4 a = p[0], b = p[1];
+    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c < full ? w[e] : 0.0f;
+  };
+  auto top_of = [](uint32_t top, const float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = as_u32(v[e]) & 0x7fffffffu;
+      top = top > b ? top : b;
+    }
+    return top;
+  };
+  float v[CH ? CH : 1][8];
+  uint32_t top = 0;
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) get(lane + 64 * i, v[i]);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) top = top_of(top, v[i]);
+  } else {
+    for (int c = lane; c < full; c += 64) {
+      get(c, v[0]);
+      top = top_of(top, v[0]);
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)top, d);
+    top = top > o ? top : o;
+  }
+  const bool odd = top >= 0x7f800000u;
+  const int s = top > 0 && !odd ? __builtin_amdgcn_frexp_expf(as_f32(top)) - 10 : 0;
+  if (lane == 0) rscale[row] = odd ? __builtin_nanf("") : ldexpf(1.0f, s);
+  auto put = [&](int c, const float w[8]) {
+    h8 h, l;
+    float t = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = ldexpf(w[e], -s);
+      h[e] = (_Float16)y;
+      l[e] = (_Float16)(y - (float)h[e]);
+      t += (float)h[e] + (float)l[e];  // what the planes hold
+    }
+    t += dpp_row_f<0xB1>(t);
+    t += dpp_row_f<0x4E>(t);
+    if (c < chunks) {
+      const int64_t at = (int64_t)row * Kp + 8 * c;
+      *reinterpret_cast<h8 *>(hi + at) = h;
+      *reinterpret_cast<h8 *>(lo + at) = l;
+      if ((c & 3) == 0) sums[at / 32] = h2{(_Float16)t, (_Float16)(t - (float)(_Float16)t)};
+    }
+  };
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) put(lane + 64 * i, v[i]);
+  } else {
+    for (int c0 = 0; c0 < chunks; c0 += 64) {
+      get(c0 + lane, v[0]);
+      put(c0 + lane, v[0]);
+    }
+  }
+}
+
+// out[t] = the sum of its pairs' rows, in their order; zeros for none.  place:
+// where a pair's row is; without it, its own place if it has an expert.
 template <int N>
 __global__ __launch_bounds__(256) void moe_sum_kernel(const float *__restrict__ y, const int32_t *__restrict__ ids,
-                                                      int top_k, int experts, int hidden, float *__restrict__ out,
-                                                      int64_t out_stride) {
+                                                      const int *__restrict__ place, int top_k, int experts, int hidden,
+                                                      float *__restrict__ out, int64_t out_stride) {
   typedef float fN __attribute__((ext_vector_type(N)));
-  const int64_t t = blockIdx.y;
-  const int c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * N;
+  const int64_t t = blockIdx.x;
+  const int c = ((int)blockIdx.y * 256 + (int)threadIdx.x) * N;
   if (c >= hidden) return;
   fN sum = {};
-  for (int j = 0; j < top_k; ++j)
-    if ((uint32_t)ids[t * top_k + j] < (uint32_t)experts)
-      sum += *reinterpret_cast<const fN *>(y + (t * top_k + j) * hidden + c);
+  for (int j = 0; j < top_k; ++j) {
+    const int64_t p = t * top_k + j;
+    const int64_t at = place ? place[p] : (uint32_t)ids[p] < (uint32_t)experts ? p : -1;
+    if (at >= 0) sum += *reinterpret_cast<const fN *>(y + at * hidden + c);
+  }
   *reinterpret_cast<fN *>(out + t * out_stride + c) = sum;
 }
 
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+static int whole(int k) { return (k + 255) / 256 * 256; }
+
+// Planes of `rows` rows of K values at a place of the workspace.
+struct Planes {
+  size_t hi, lo, sums, rscale, end;
+  Planes(size_t at, int64_t rows, int K) {
+    const size_t n = (size_t)rows * (size_t)whole(K);
+    hi = at;
+    lo = hi + up256(n * 2);
+    sums = lo + up256(n * 2);
+    rscale = sums + up256(n / 8);
+    end = rscale + up256((size_t)rows * 4);
+  }
+};
 
 MoePlan moe_plan(const MoeArgs &a, int) {
   MoePlan p{};
-  p.pass_rows = std::min<int64_t>(a.rows, kPassPairs / a.top_k);
+  p.tiled = (int64_t)a.rows * a.top_k >= 12 * (int64_t)a.experts && (int64_t)a.rows * a.top_k > 32;
+  // a pass of sorted pairs keeps to 1 GiB of results and 16 bits of blocks
+  const int64_t most = p.tiled ? std::max<int64_t>(256, std::min<int64_t>(65536, (1 << 30) / (8 * (int64_t)whole(a.inner) + 4 * (int64_t)a.hidden)))
+                               : kPassPairs;
+  p.pass_rows = std::max<int64_t>(1, std::min<int64_t>(a.rows, most / a.top_k));
   const size_t pairs = (size_t)p.pass_rows * a.top_k;
   p.off_inner = 0;
   p.off_pair = up256(pairs * a.inner * sizeof(float));
   p.workspace = p.off_pair + up256(pairs * a.hidden * sizeof(float));
+  if (p.tiled) {
+    p.off_order = p.workspace;
+    p.off_x = p.off_order + 2 * up256(pairs * sizeof(int)) + 256 + up256(expert_tiles(pairs, a.experts) * sizeof(ExpertTile));
+    p.workspace = Planes(Planes(p.off_x, p.pass_rows, a.hidden).end, pairs, a.inner).end;
+  }
   return p;
+}
+
+static hipError_t launch_planes(const float *x, int64_t x_stride, int64_t rows, const int *count, int K, uint8_t *ws,
+                                const Planes &p, hipStream_t s) {
+  const int Kp = whole(K), ch = (Kp / 8 + 63) / 64;
+  const dim3 grid((unsigned)((rows + 3) / 4));
+  _Float16 *hi = reinterpret_cast<_Float16 *>(ws + p.hi), *lo = reinterpret_cast<_Float16 *>(ws + p.lo);
+  h2 *sums = reinterpret_cast<h2 *>(ws + p.sums);
+  float *rscale = reinterpret_cast<float *>(ws + p.rscale);
+#define OKQ_PLANES(CH_) \
+  launch_timed(moe_planes_kernel<CH_>, grid, dim3(256), 0u, s, x, x_stride, (int)rows, count, K, Kp, hi, lo, sums, rscale)
+  if (ch == 1) OKQ_PLANES(1);
+  else if (ch == 2) OKQ_PLANES(2);
+  else if (ch <= 4) OKQ_PLANES(4);
+  else if (ch <= 8) OKQ_PLANES(8);
+  else OKQ_PLANES(0);
+#undef OKQ_PLANES
+  return hipGetLastError();
+}
+
+static hipError_t launch_sum(const MoeArgs &a, const float *y, const int32_t *ids, const int *place, int64_t rows,
+                             float *out, hipStream_t s) {
+  const bool wide = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && a.out_stride % 4 == 0;
+  const dim3 grid((unsigned)rows, (unsigned)((a.hidden / (wide ? 4 : 1) + 255) / 256));
+  if (wide) launch_timed(moe_sum_kernel<4>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden, out, a.out_stride);
+  else launch_timed(moe_sum_kernel<1>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden, out, a.out_stride);
+  return hipGetLastError();
 }
 
 template <class F, int NM>
@@ -525,42 +727,82 @@ static MoeProduct product(int type, int K, int N, int experts) {
   return p;
 }
 
+// A pass over `rows` rows from t0 on, the pairs sorted.
+static hipError_t tiled_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws, int64_t t0, int64_t rows, hipStream_t s) {
+  const int64_t pairs = rows * a.top_k, room = plan.pass_rows * a.top_k;
+  float *inner = reinterpret_cast<float *>(ws + plan.off_inner), *pair = reinterpret_cast<float *>(ws + plan.off_pair);
+  int *order = reinterpret_cast<int *>(ws + plan.off_order), *place = order + up256(room * sizeof(int)) / sizeof(int);
+  int *count = place + up256(room * sizeof(int)) / sizeof(int);
+  ExpertTile *tiles = reinterpret_cast<ExpertTile *>(count + 64);
+  const Planes px(plan.off_x, plan.pass_rows, a.hidden), ph(px.end, room, a.inner);
+  const int32_t *ids = a.ids + t0 * a.top_k;
+  launch_timed(moe_sort_kernel, dim3(1), dim3(1024), 0u, s, ids, (int)pairs, a.experts, order, place, count, tiles);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) e = launch_planes(a.x + t0 * a.x_stride, a.x_stride, rows, nullptr, a.hidden, ws, px, s);
+  if (e != hipSuccess) return e;
+  auto run = [&](int type, bool gate_up, const MoeProduct &m, const Planes &p, int64_t n, float *y) {
+    ExpertMat mat{};
+    mat.w[0] = m.w[0];
+    mat.w[1] = m.w[1];
+    mat.w_bytes = m.w_bytes;
+    mat.expert_bytes = m.expert_bytes;
+    mat.order = order;
+    mat.weights = a.weights + t0 * a.top_k;
+    mat.y = y;
+    mat.n = m.N;
+    mat.row_bytes = m.row_bytes;
+    mat.top_k = a.top_k;
+    return launch_experts(type, gate_up, reinterpret_cast<_Float16 *>(ws + p.hi), reinterpret_cast<_Float16 *>(ws + p.lo),
+                          ws + p.sums, reinterpret_cast<float *>(ws + p.rscale), (int)n, whole(m.K), mat, count, tiles,
+                          expert_tiles(pairs, a.experts), s);
+  };
+  MoeProduct g = product(a.gate_up_type, a.hidden, a.inner, a.experts);
+  g.w[0] = a.gate;
+  g.w[1] = a.up;
+  e = run(a.gate_up_type, true, g, px, rows, inner);
+  if (e == hipSuccess) e = launch_planes(inner, a.inner, pairs, count, a.inner, ws, ph, s);
+  if (e != hipSuccess) return e;
+  MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
+  d.w[0] = a.down;
+  e = run(a.down_type, false, d, ph, pairs, pair);
+  if (e != hipSuccess) return e;
+  return launch_sum(a, pair, ids, place, rows, a.out + t0 * a.out_stride, s);
+}
+
+// The same with each expert's weights streamed past its rows.
+static hipError_t stream_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws, int64_t t0, int64_t rows, int cu_count,
+                              hipStream_t s) {
+  float *inner = reinterpret_cast<float *>(ws + plan.off_inner), *pair = reinterpret_cast<float *>(ws + plan.off_pair);
+  MoeProduct g = product(a.gate_up_type, a.hidden, a.inner, a.experts);
+  g.x = a.x + t0 * a.x_stride;
+  g.x_stride = a.x_stride;
+  g.share = a.top_k;
+  g.w[0] = a.gate;
+  g.w[1] = a.up;
+  g.ids = a.ids + t0 * a.top_k;
+  g.y = inner;
+  g.pairs = (int)(rows * a.top_k);
+  hipError_t e = launch_product<2>(a.gate_up_type, g, cu_count, s);
+  if (e != hipSuccess) return e;
+  MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
+  d.x = inner;
+  d.x_stride = a.inner;
+  d.share = 1;
+  d.w[0] = a.down;
+  d.ids = g.ids;
+  d.weights = a.weights + t0 * a.top_k;
+  d.y = pair;
+  d.pairs = g.pairs;
+  e = launch_product<1>(a.down_type, d, cu_count, s);
+  if (e != hipSuccess) return e;
+  return launch_sum(a, pair, g.ids, nullptr, rows, a.out + t0 * a.out_stride, s);
+}
+
 hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s) {
-  float *inner = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.off_inner);
-  float *pair = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + plan.off_pair);
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
   for (int64_t t0 = 0; t0 < a.rows; t0 += plan.pass_rows) {
     const int64_t rows = std::min<int64_t>(plan.pass_rows, a.rows - t0);
-    MoeProduct g = product(a.gate_up_type, a.hidden, a.inner, a.experts);
-    g.x = a.x + t0 * a.x_stride;
-    g.x_stride = a.x_stride;
-    g.share = a.top_k;
-    g.w[0] = a.gate;
-    g.w[1] = a.up;
-    g.ids = a.ids + t0 * a.top_k;
-    g.y = inner;
-    g.pairs = (int)(rows * a.top_k);
-    hipError_t e = launch_product<2>(a.gate_up_type, g, cu_count, s);
-    if (e != hipSuccess) return e;
-    MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
-    d.x = inner;
-    d.x_stride = a.inner;
-    d.share = 1;
-    d.w[0] = a.down;
-    d.ids = g.ids;
-    d.weights = a.weights + t0 * a.top_k;
-    d.y = pair;
-    d.pairs = g.pairs;
-    e = launch_product<1>(a.down_type, d, cu_count, s);
-    if (e != hipSuccess) return e;
-    float *out = a.out + t0 * a.out_stride;
-    const bool wide = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && a.out_stride % 4 == 0;
-    const int n = wide ? 4 : 1;
-    const dim3 grid((unsigned)((a.hidden / n + 255) / 256), (unsigned)rows);
-    if (wide)
-      launch_timed(moe_sum_kernel<4>, grid, dim3(256), 0u, s, (const float *)pair, g.ids, a.top_k, a.experts, a.hidden, out, a.out_stride);
-    else
-      launch_timed(moe_sum_kernel<1>, grid, dim3(256), 0u, s, (const float *)pair, g.ids, a.top_k, a.experts, a.hidden, out, a.out_stride);
-    e = hipGetLastError();
+    const hipError_t e = plan.tiled ? tiled_pass(a, plan, ws, t0, rows, s) : stream_pass(a, plan, ws, t0, rows, cu_count, s);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -1500,8 +1500,9 @@ okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t
                          uint64_t up_bytes, uint32_t down_type, const void *down_w, uint64_t down_bytes, float *out,
                          int64_t out_stride, void *stream) {
   const char *what = "moe_mlp";
-  if (rows < 0 || experts < 1 || rows > INT32_MAX || experts > 1 << 16)
-    return fail(OKQ_E_SHAPE, "%s rows=%lld experts=%lld: experts must be 1 to 65536", what, (long long)rows, (long long)experts);
+  if (rows < 0 || experts < 1 || rows > INT32_MAX || experts > okq::kMoeMaxExperts)
+    return fail(OKQ_E_SHAPE, "%s rows=%lld experts=%lld: experts must be 1 to %d", what, (long long)rows,
+                (long long)experts, okq::kMoeMaxExperts);
   if (top_k < 1 || top_k > okq::kMaxTopK)
     return fail(OKQ_E_SHAPE, "%s top_k=%lld must be 1 to %d", what, (long long)top_k, okq::kMaxTopK);
   const struct Tensor {
