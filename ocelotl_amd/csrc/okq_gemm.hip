@@ -366,13 +366,6 @@ struct DecMats {
   int tile0[kDecMats];
 };
 
-// Workgroup barrier for LDS only: waits for this wave's LDS operations, not
-// for its vector-memory loads (loads issued ahead stay in flight across it).
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);  // gfx9 encoding: lgkmcnt(0), vmcnt and expcnt unconstrained
-  __builtin_amdgcn_s_barrier();
-}
-
 // Activation row r of a decode-batch plane (row pitch P halves, P = 8 mod
 // 256) starts at dec_row(r, P) halves: rows 8-15 of each 16-row group sit
 // 64 halves (128 B) further.  A ds_read_b128 serves 32 lanes per pass over

@@ -361,9 +361,11 @@ struct ExpertMat {
   float *y;              // [place][n]
   int n, row_bytes, top_k;
 };
-// Most tiles that `pairs` of `experts` can take, and the launch over those that
+// Most tiles of `height` rows that `pairs` of `experts` can take, and the launch over those that
 // `tiles` (behind a count of them) names: x as planes of M rows of K.
-inline int64_t expert_tiles(int64_t pairs, int64_t experts) { return pairs / 128 + (experts < pairs ? experts : pairs); }
+inline int64_t expert_tiles(int64_t pairs, int64_t experts, int64_t height) {
+  return pairs / height + (experts < pairs ? experts : pairs);
+}
 hipError_t launch_experts(int type, bool gate_up, const _Float16 *xhi, const _Float16 *xlo, const void *xsum,
                           const float *rscale, int M, int K, const ExpertMat &mat, const int *count,
                           const ExpertTile *tiles, int64_t most_tiles, hipStream_t s);

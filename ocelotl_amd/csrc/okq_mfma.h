@@ -83,4 +83,12 @@ __device__ __forceinline__ h2 byte_pair(uint32_t four, uint32_t j) {
   return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, four, 0x04000400u + 0x00010001u * j)) +
          h2{(_Float16)-1024.0f, (_Float16)-1024.0f};
 }
+
+// Workgroup barrier for LDS only: waits for this wave's LDS operations, not
+// for its vector-memory loads (loads issued ahead stay in flight across it).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // gfx9 encoding: lgkmcnt(0), vmcnt and expcnt unconstrained
+  __builtin_amdgcn_s_barrier();
+}
+
 }  // namespace okq

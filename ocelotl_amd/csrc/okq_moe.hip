@@ -23,7 +23,8 @@ namespace okq {
 namespace {
 
 constexpr int kWaves = 8;
-constexpr int kPassPairs = 4096;  // pairs of one pass (its list of an expert's lies in LDS)
+constexpr int kFewPairs = 64;    // not sorted: a lane each
+constexpr int kBatch = 4;         // column tiles whose waves meet in LDS together
 
 // ---- a lane's share of 16 columns x 256 values of K --------------------------------
 // v_mfma_f32_16x16x32_f16: lane l holds row / column l % 16 and, at step t,
@@ -54,8 +55,11 @@ struct ExpQ4K {
   __device__ static Cur header(const u32x4 &hd, int g) {
     Cur c;
     const uint32_t k = 2u * ((uint32_t)g & 1u);
-    const uint32_t sc4 = g < 2 ? hd.y & 0x3F3F3F3Fu : (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u);
-    const uint32_t m4 = g < 2 ? hd.z & 0x3F3F3F3Fu : ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u);
+    // (masks: a choice between the two became a branch)
+    const uint32_t early = g < 2 ? 0xFFFFFFFFu : 0u;
+    auto pick = [&](uint32_t a, uint32_t b) { return (a & early) | (b & ~early); };
+    const uint32_t sc4 = pick(hd.y & 0x3F3F3F3Fu, (hd.w & 0x0F0F0F0Fu) | ((hd.y >> 2) & 0x30303030u));
+    const uint32_t m4 = pick(hd.z & 0x3F3F3F3Fu, ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u));
     const h2 s0 = byte_pair(sc4, k), s1 = byte_pair(sc4, k + 1u), m0 = byte_pair(m4, k), m1 = byte_pair(m4, k + 1u);
     auto by = [](h2 v, float f) { return v * h2{(_Float16)f, (_Float16)f}; };
     c.sc[0] = s0;
@@ -258,7 +262,11 @@ __device__ __forceinline__ void load_row(float4 raw[16], const float *row, int k
 // lies in [512, 1024).
 template <class F>
 __device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
-  uint32_t top = 0;
+  // the largest magnitude as a bit pattern (NaN above infinity above every
+  // finite value): the largest of the positive ones in signed order, of the
+  // negative ones in unsigned order
+  int pos = 0;
+  uint32_t neg = 0;
   auto value = [&](int t, int e) {
     const float4 v = raw[2 * t + (e >> 2)];
     return (e & 3) == 0 ? v.x : (e & 3) == 1 ? v.y : (e & 3) == 2 ? v.z : v.w;
@@ -267,9 +275,12 @@ __device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t b = as_u32(value(t, e)) & 0x7fffffffu;  // NaN above infinity above every finite value
-      top = top > b ? top : b;
+      const uint32_t b = as_u32(value(t, e));
+      pos = pos > (int)b ? pos : (int)b;
+      neg = neg > b ? neg : b;
     }
+  neg &= 0x7fffffffu;  // without a negative value: the positives' largest once more
+  uint32_t top = neg > (uint32_t)pos ? neg : (uint32_t)pos;
   uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
   top = top > o ? top : o;
   o = (uint32_t)__shfl_xor((int)top, 32);
@@ -278,16 +289,33 @@ __device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
   const int s = top > 0 && !odd ? __builtin_amdgcn_frexp_expf(as_f32(top)) - 10 : 0;
   A.scale = odd ? __builtin_nanf("") : ldexpf(1.0f, s);
   float sum[2] = {0.0f, 0.0f};
+  const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+  auto put = [&](int t, auto &&plane, auto &&rest) {
 #pragma unroll
-  for (int t = 0; t < 8; ++t)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float w = ldexpf(value(t, e), -s);
-      const _Float16 h = (_Float16)w, l = (_Float16)(w - (float)h);
-      A.hi[t][e] = h;
-      A.lo[t][e] = l;
-      if (F::kMins) sum[t & 1] += (float)h + (float)l;  // what the planes hold
+    for (int e = 0; e < 8; e += 2) {
+      const h2 h = {(_Float16)plane(value(t, e)), (_Float16)plane(value(t, e + 1))};
+      const h2 l = {(_Float16)rest(value(t, e), h[0]), (_Float16)rest(value(t, e + 1), h[1])};
+      A.hi[t][e] = h[0];
+      A.hi[t][e + 1] = h[1];
+      A.lo[t][e] = l[0];
+      A.lo[t][e + 1] = l[1];
+      // sums of what the planes hold
+      if (F::kMins) sum[t & 1] = __builtin_amdgcn_fdot2(l, one, __builtin_amdgcn_fdot2(h, one, sum[t & 1], false), false);
     }
+    __builtin_amdgcn_sched_barrier(0);  // planes take the raw values' registers, piece by piece
+  };
+  // 2^-s a normal f32 (every row of the wave): one mixed multiply-add a plane
+  if (__builtin_amdgcn_ballot_w64(s < -100 || s > 100) == 0) {
+    const float f = ldexpf(1.0f, -s);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      put(t, [&](float v) { return __builtin_fmaf(v, f, 0.0f); },
+          [&](float v, _Float16 h) { return __builtin_fmaf(v, f, -(float)h); });
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      put(t, [&](float v) { return ldexpf(v, -s); }, [&](float v, _Float16 h) { return ldexpf(v, -s) - (float)h; });
+  }
   if (F::kMins) {
     const _Float16 h0 = (_Float16)sum[0], h1 = (_Float16)sum[1];
     const _Float16 z = (_Float16)0.0f;
@@ -301,15 +329,17 @@ template <class F>
 __device__ __forceinline__ void contract(f4 &acc, const typename F::Item &it, const ActA &A, const f4 &rs, int g) {
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   const typename F::Cur c = F::begin(it, g);
-  f4 s = zero;
+  f4 s = zero, low = zero;  // two chains: a product waits for the one before it in its own
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
     h8 b1, b2;
     F::frag(it, c, t, g, b1, b2);
     s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.hi[t], b1, s, 0, 0, 0);
-    if constexpr (F::kLow) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.hi[t], b2, s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.lo[t], b1, s, 0, 0, 0);  // lo * b2 is below 2^-22 of the product
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.lo[t], b1, low, 0, 0, 0);
+    // (lo * b2 is below 2^-22 of the product)
+    if constexpr (F::kLow) low = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.hi[t], b2, low, 0, 0, 0);
   }
+  s += low;
   if constexpr (F::kMins) {
     const f4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.sums, c.m, zero, 0, 0, 0);
 #pragma unroll
@@ -330,143 +360,206 @@ struct MoeProduct {
   uint64_t expert_bytes;
   const int32_t *ids;
   const float *weights;  // down: a pair's factor
+  const int *order, *count;  // sorted pairs and the number of jobs (null: few pairs, not sorted)
+  const ExpertTile *jobs;    // up to 16 rows of an expert each
   float *y;              // [pairs][N]
   int pairs, experts, K, N, nsb, row_bytes;
-  int kw, slots;         // waves of a column tile, tiles side by side
+  int slices;            // of K, each with a part of y [slices][NM][pairs][N]; 1: the product itself
+  int slots, steps;      // column tiles side by side in a workgroup; steps over all columns
+  int rounds;            // few pairs: steps of a workgroup
 };
 
 }  // namespace
 
-// A workgroup has one expert's columns [slots * T tiles of 16]; its kw waves
-// of a tile share out K and meet in LDS.  It lists the expert's pairs from
-// ids by itself (a launch that did it for all would cost more than 4 us; the
-// ids are a few KB in the L2), so workgroups of experts without pairs end at
-// once.  With fewer pairs than experts a workgroup has a pair's expert, and
-// goes on if no earlier pair has the same.  Rows go 16 at a time: a row's
-// activations stay in registers while T column tiles' weights pass, and the
-// next items are in flight behind the current ones.
-template <class F, int NM, int T>
+// A workgroup has one slice of K of at most kWaves items, and passes over steps
+// of `slots` column tiles of up to 16 rows of one expert (a job).  A wave keeps
+// its item's activations in registers (16 rows, both planes: 64 of them) while
+// the weights of one tile after the other come through a ring of D, so that
+// each weight is read once and nothing but weights is read in the loop; the
+// waves of a slice meet in LDS, kBatch tiles at a time in one of two buffers,
+// one barrier a batch.
+//
+// Sorted pairs: the workgroups of a slice share out all jobs' steps evenly,
+// whatever the experts' shares of the rows are.  With one workgroup an expert's
+// columns, unused experts left CUs idle and one of 17 rows took twice the time
+// of the others: 96 rows of 8 of 256 experts, gate and up 169 -> 87 us.
+//
+// A few pairs (kFewPairs at most) whose experts mostly differ are not sorted (a
+// launch of 5 us): every workgroup has a pair's expert and lists its pairs by
+// itself, going on if no earlier pair has the same, `rounds` steps and as many
+// turns as it has 16 rows.
+template <class F, int NM, int D>
 __global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
-  __shared__ uint16_t list[kPassPairs];
-  __shared__ int count[kWaves];
-  __shared__ f4 red[kWaves][NM * T][64];
+  __shared__ f4 red[2][kBatch][kWaves][NM][64];
+  __shared__ uint8_t lists[kWaves][kFewPairs];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int waves = (int)blockDim.x >> 6;
-  const int n = lane & 15, g = lane >> 4;
-  const int job = (int)blockIdx.y;
-  const bool by_pair = a.pairs < a.experts;
-  const int e = by_pair ? __builtin_amdgcn_readfirstlane(a.ids[job]) : job;
-  if (e < 0 || e >= a.experts) return;
-
-  // the expert's pairs in order: every wave counts its share of the ids, then
-  // writes behind the waves before it
-  const int share = (a.pairs + 64 * waves - 1) / (64 * waves) * 64, lo = wave * share, hi = std::min(a.pairs, lo + share);
-  int mine = 0;
-  for (int p = lo; p < hi; p += 64)
-    mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p + lane < hi && a.ids[std::min(p + lane, hi - 1)] == e));
-  if (lane == 0) count[wave] = mine;
-  __syncthreads();
-  int at = 0, m = 0;
-  for (int w = 0; w < waves; ++w) {
-    at += w < wave ? count[w] : 0;
-    m += count[w];
-  }
-  if (mine)
-    for (int p = lo; p < hi; p += 64) {
-      const bool hit = p + lane < hi && a.ids[std::min(p + lane, hi - 1)] == e;
-      const uint64_t mask = __builtin_amdgcn_ballot_w64(hit);
-      if (hit) list[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = (uint16_t)(p + lane);
-      at += __builtin_popcountll(mask);
-    }
-  __syncthreads();
-  if (m == 0 || (by_pair && list[0] != job)) return;
-
-  const int slot = wave / a.kw, ks = wave - slot * a.kw;
-  const int tile0 = ((int)blockIdx.x * a.slots + slot) * T;
+  const int waves = (int)blockDim.x >> 6, z = (int)blockIdx.z;
+  const int s0 = z * a.nsb / a.slices, kw = (z + 1) * a.nsb / a.slices - s0;  // the slice's items
+  const int slot = __builtin_amdgcn_readfirstlane(wave / kw), ks = wave - slot * kw, item = s0 + ks;
+  const bool idle = slot >= a.slots;  // a slice with fewer items than its launch has waves for
   const uint32_t sb = (uint32_t)(F::kType == kQ8_0 ? 8 * kQ8Bytes : sb_bytes_of(F::kType));
-  // the expert's weights from the dword at or below its first byte, to the
-  // last dword that holds a byte of the stack
-  Rsrc rs[NM];
-  uint32_t skew[NM];
-#pragma unroll
-  for (int i = 0; i < NM; ++i) {
-    const uint64_t from = (uint64_t)e * a.expert_bytes;
-    const uint8_t *base = a.w[i] + from;
-    skew[i] = (uint32_t)(reinterpret_cast<uintptr_t>(base) & 3u);
-    const uint64_t left = (a.w_bytes - from + skew[i] + 3u) & ~3ull;
-    rs[i] = make_rsrc(base - skew[i], (uint32_t)std::min<uint64_t>(left, 0xFFFFFFFCull));
-  }
-  uint32_t col_at[T];
-#pragma unroll
-  for (int t = 0; t < T; ++t) col_at[t] = (uint32_t)std::min((tile0 + t) * 16 + n, a.N - 1) * (uint32_t)a.row_bytes;
-  typename F::Item S[NM * T];
-  auto load_item = [&](int i, int s) {
-    const uint32_t blk = col_at[i / NM] + skew[i % NM] + (uint32_t)s * sb;
-    F::load(S[i], rs[i % NM], s < a.nsb ? blk : 0xFFFFF000u, g);
-  };
 
-  for (int r0 = 0; r0 < m; r0 += 16) {
-    const int p = list[std::min(r0 + n, m - 1)];
-    const float *row = a.x + (int64_t)(p / a.share) * a.x_stride;
-    f4 acc[NM * T];
+  // the steps [u, end) of this workgroup, job * steps + step (sorted pairs), or
+  // of its expert's turns
+  int u, end, expert = 0, m = 0;
+  if (a.order) {
+    const int64_t all = (int64_t)a.count[0] * a.steps;
+    u = (int)(all * blockIdx.x / gridDim.x);
+    end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  } else {
+    const int id = a.ids[std::min(lane, a.pairs - 1)], job = (int)blockIdx.y;
+    expert = __builtin_amdgcn_readlane(id, job);
+    const uint64_t all = __builtin_amdgcn_ballot_w64(lane < a.pairs && id == expert);
+    if ((uint32_t)expert >= (uint32_t)a.experts || __builtin_ctzll(all) != job) return;
+    m = __builtin_popcountll(all);
+    if (all >> lane & 1) lists[wave][__builtin_popcountll(all & ((1ull << lane) - 1))] = (uint8_t)lane;
+    wave_sync();
+    u = 0;
+    end = (m + 15) / 16;
+  }
+  int parity = 0;
+  while (u < end) {
+    // (opaque, so that a job's addresses are not formed ahead of the loop, where
+    // they would take the registers that the loads need)
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int n = l & 15, g = l >> 4;
+    int step0, steps, rows, pair;
+    if (a.order) {
+      const int job = u / a.steps;
+      const ExpertTile t = a.jobs[job];
+      expert = t.expert;
+      rows = t.rows;
+      step0 = u - job * a.steps;
+      steps = std::min(a.steps - step0, end - u);
+      u += steps;
+      pair = a.order[t.row0 + std::min(n, rows - 1)];
+    } else {
+      rows = std::min(16, m - 16 * u);
+      step0 = (int)blockIdx.x * a.rounds;
+      steps = std::min(a.steps - step0, a.rounds);
+      pair = lists[wave][16 * u + std::min(n, rows - 1)];
+      u += 1;
+    }
+    // the expert's weights from the dword at or below its first byte, to the
+    // last dword that holds a byte of the stack
+    Rsrc rs[NM];
+    uint32_t skew[NM];
 #pragma unroll
-    for (int i = 0; i < NM * T; ++i) acc[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < NM; ++i) {
+      const uint64_t from = (uint64_t)expert * a.expert_bytes;
+      const uint8_t *base = a.w[i] + from;
+      skew[i] = (uint32_t)(reinterpret_cast<uintptr_t>(base) & 3u);
+      const uint64_t left = (a.w_bytes - from + skew[i] + 3u) & ~3ull;
+      rs[i] = make_rsrc(base - skew[i], (uint32_t)std::min<uint64_t>(left, 0xFFFFFFFCull));
+    }
+    typename F::Item S[D][NM];
+    // the weights of the wave's i-th tile (past the steps, or columns past the
+    // last: past the stack, nothing)
+    auto load_tile = [&](typename F::Item *it, int i) {
+      const int col = ((step0 + i) * a.slots + slot) * 16 + n;
+      const bool in = !idle && i < steps && col < a.N;
+      const uint32_t at = (uint32_t)col * (uint32_t)a.row_bytes + (uint32_t)item * sb;
 #pragma unroll
-    for (int i = 0; i < NM * T; ++i) load_item(i, ks);
-    for (int s = ks; s < a.nsb; s += a.kw) {
-      ActA A;
-      {
-        float4 raw[16];
-        load_row<F>(raw, row, s * 256, a.K, g);
-        convert<F>(A, raw);
-      }
-      f4 scales;
+      for (int k = 0; k < NM; ++k) F::load(it[k], rs[k], in ? at + skew[k] : 0xFFFFF000u, g);
+    };
+    ActA A;
+    f4 scales, factor = {};  // of the four rows whose sums the lane holds
+    int mine[4];             // their pairs
+#pragma unroll
+    for (int v = 0; v < 4; ++v) mine[v] = __shfl(pair, 4 * g + v);
+    {
+      float4 raw[16];
+      load_row<F>(raw, a.x + (int64_t)(pair / a.share) * a.x_stride, item * 256, a.K, g);
+      __builtin_amdgcn_sched_barrier(0);  // the activations ahead of the weights: loads return in order
+#pragma unroll
+      for (int d = 0; d < D; ++d) load_tile(S[d], d);
+      if constexpr (NM == 1)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) factor[v] = a.weights[mine[v]];
+      __builtin_amdgcn_sched_barrier(0);
+      convert<F>(A, raw);
 #pragma unroll
       for (int v = 0; v < 4; ++v) scales[v] = __shfl(A.scale, 4 * g + v);
-#pragma unroll
-      for (int i = 0; i < NM * T; ++i) {
-        contract<F>(acc[i], S[i], A, scales, g);
-        load_item(i, s + a.kw);
-      }
     }
-    // the tile's waves meet in their order
-    if (r0) __syncthreads();
+    for (int i0 = 0; i0 < steps; i0 += D) {
 #pragma unroll
-    for (int i = 0; i < NM * T; ++i) red[wave][i][lane] = acc[i];
-    __syncthreads();
-    if (ks == 0) {
+      for (int d = 0; d < D; ++d) {
+        const int i = i0 + d;  // (may be one past the last: zeros, not stored)
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
+        for (int k = 0; k < NM; ++k) {
+          f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+          contract<F>(acc, S[d][k], A, scales, g);
+          red[parity][i % kBatch][wave][k][l] = acc;
+        }
+        // into the registers that this tile's weights have left (issued any
+        // earlier, they took others, and moving them waited for every load)
+        __builtin_amdgcn_sched_barrier(0);
+        load_tile(S[d], i + D);
+      }
+      const int done = std::min(i0 + D, steps);
+      if (done % kBatch != 0 && done < steps) continue;
+      lds_barrier();  // the weights stay in flight
+      // the batch's tiles, a wave each, over their items in order; the next
+      // batch goes to the other buffer, and other waves first
+      const int from = (done - 1) / kBatch * kBatch, n_tiles = (done - from) * a.slots;
+      for (int j = parity ? waves - 1 - wave : wave; j < n_tiles; j += waves) {
+        const int b = j / a.slots, sl = j - b * a.slots;
         f4 sum[NM];
 #pragma unroll
-        for (int i = 0; i < NM; ++i) {
-          sum[i] = red[wave][NM * t + i][lane];
-          for (int w = 1; w < a.kw; ++w) sum[i] += red[wave + w][NM * t + i][lane];
-        }
-        const int col = (tile0 + t) * 16 + n;
-        if (col < a.N)
+        for (int k = 0; k < NM; ++k) {
+          f4 v[kWaves];
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (r0 + 4 * g + v < m) {
-              const int q = list[r0 + 4 * g + v];
-              float y = sum[0][v];
-              if constexpr (NM == 2) y = (y * (1.0f / (1.0f + expf(-y)))) * sum[1][v];
-              else y *= a.weights[q];
-              a.y[(int64_t)q * a.N + col] = y;
-            }
+          for (int w = 0; w < kWaves; ++w)
+            v[w] = w < kw ? red[parity][b][sl * kw + w][k][l] : f4{0.0f, 0.0f, 0.0f, 0.0f};
+          sum[k] = v[0];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) sum[k] += v[w];
+        }
+        const int col = ((step0 + from + b) * a.slots + sl) * 16 + n;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int64_t q = mine[v];
+          if (4 * g + v >= rows || col >= a.N) continue;
+          if (NM == 2 && a.slices > 1) {
+            float *y = a.y + ((int64_t)z * NM * a.pairs + q) * a.N + col;
+            y[0] = sum[0][v];
+            y[(int64_t)a.pairs * a.N] = sum[NM - 1][v];
+          } else if (NM == 2) {
+            a.y[q * a.N + col] = (sum[0][v] * (1.0f / (1.0f + expf(-sum[0][v])))) * sum[NM - 1][v];
+          } else {
+            a.y[((int64_t)z * a.pairs + q) * a.N + col] = sum[0][v] * factor[v];
+          }
+        }
       }
+      parity ^= 1;
     }
   }
+}
+
+// silu(gate) * up from the slices' parts [slices][2][n].
+__global__ __launch_bounds__(256) void moe_gate_kernel(const float4 *__restrict__ part, int slices, int64_t n4,
+                                                       float4 *__restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4) return;
+  float4 g = part[i], u = part[n4 + i];
+  for (int z = 1; z < slices; ++z) {
+    const float4 a = part[2 * z * n4 + i], b = part[(2 * z + 1) * n4 + i];
+    g = float4{g.x + a.x, g.y + a.y, g.z + a.z, g.w + a.w};
+    u = float4{u.x + b.x, u.y + b.y, u.z + b.z, u.w + b.w};
+  }
+  auto f = [](float v, float w) { return (v * (1.0f / (1.0f + expf(-v)))) * w; };
+  y[i] = float4{f(g.x, u.x), f(g.y, u.y), f(g.z, u.z), f(g.w, u.w)};
 }
 
 // ---- many rows: the pairs sorted by expert ------------------------------------------
 
 // order: the pairs by expert; place: each pair's place in it (-1: no such
-// expert); count: tiles, and pairs with an expert; the tiles.  One workgroup:
+// expert); count: tiles of up to `height` rows, and pairs with an expert; the tiles.  One workgroup:
 // the ids of 4096 tokens are 128 KB, and their counts meet in LDS.  (Pairs of
 // an expert come in any order: a row's result does not depend on its place.)
 __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs, int experts,
-                                                        int *__restrict__ order, int *__restrict__ place,
+                                                        int height, int *__restrict__ order, int *__restrict__ place,
                                                         int *__restrict__ count, ExpertTile *__restrict__ tiles) {
   constexpr int kPer = kMoeMaxExperts / 1024;
   __shared__ int next[kMoeMaxExperts];
@@ -486,7 +579,7 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
   for (int i = 0; i < kPer; ++i) {
     m[i] = next[kPer * tid + i];
     rows += m[i];
-    mine += (m[i] + 127) / 128;
+    mine += (m[i] + height - 1) / height;
   }
   int r = rows, t = mine;
 #pragma unroll
@@ -506,8 +599,8 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     next[kPer * tid + i] = r;
-    for (int at = 0; at < m[i]; at += 128) {
-      const int n = m[i] - at < 128 ? m[i] - at : 128;
+    for (int at = 0; at < m[i]; at += height) {
+      const int n = m[i] - at < height ? m[i] - at : height;
       tiles[t++] = ExpertTile{kPer * tid + i, r + at, n, (n + 31) / 32};
     }
     r += m[i];
@@ -609,11 +702,13 @@ __global__ __launch_bounds__(256) void moe_planes_kernel(const float *__restrict
 }
 
 // out[t] = the sum of its pairs' rows, in their order; zeros for none.  place:
-// where a pair's row is; without it, its own place if it has an expert.
+// where a pair's row is; without it, its own place if it has an expert.  Rows
+// may come in slices to add up.
 template <int N>
 __global__ __launch_bounds__(256) void moe_sum_kernel(const float *__restrict__ y, const int32_t *__restrict__ ids,
                                                       const int *__restrict__ place, int top_k, int experts, int hidden,
-                                                      float *__restrict__ out, int64_t out_stride) {
+                                                      int slices, int64_t slice, float *__restrict__ out,
+                                                      int64_t out_stride) {
   typedef float fN __attribute__((ext_vector_type(N)));
   const int64_t t = blockIdx.x;
   const int c = ((int)blockIdx.y * 256 + (int)threadIdx.x) * N;
@@ -622,7 +717,8 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(const float *__restrict__ 
   for (int j = 0; j < top_k; ++j) {
     const int64_t p = t * top_k + j;
     const int64_t at = place ? place[p] : (uint32_t)ids[p] < (uint32_t)experts ? p : -1;
-    if (at >= 0) sum += *reinterpret_cast<const fN *>(y + at * hidden + c);
+    if (at >= 0)
+      for (int z = 0; z < slices; ++z) sum += *reinterpret_cast<const fN *>(y + z * slice + at * hidden + c);
   }
   *reinterpret_cast<fN *>(out + t * out_stride + c) = sum;
 }
@@ -643,24 +739,43 @@ struct Planes {
   }
 };
 
+// Slices of K of at most kWaves items.
+static int k_slices(int K) { return ((K + 255) / 256 + kWaves - 1) / kWaves; }
+
 MoePlan moe_plan(const MoeArgs &a, int) {
   MoePlan p{};
   p.tiled = (int64_t)a.rows * a.top_k >= 12 * (int64_t)a.experts && (int64_t)a.rows * a.top_k > 32;
-  // a pass of sorted pairs keeps to 1 GiB of results and 16 bits of blocks
-  const int64_t most = p.tiled ? std::max<int64_t>(256, std::min<int64_t>(65536, (1 << 30) / (8 * (int64_t)whole(a.inner) + 4 * (int64_t)a.hidden)))
-                               : kPassPairs;
+  const size_t gs = p.tiled ? 1 : k_slices(a.hidden), ds = p.tiled ? 1 : k_slices(a.inner);
+  // a pass keeps to about 1 GiB of results, and to what its kernels count in
+  // 32 bits
+  const int64_t one = 4 * ((int64_t)a.inner * (gs > 1 ? 1 + 2 * gs : 2) + (int64_t)a.hidden * ds);
+  const int64_t most = std::max<int64_t>(256, std::min<int64_t>(65536, (1 << 30) / one));
   p.pass_rows = std::max<int64_t>(1, std::min<int64_t>(a.rows, most / a.top_k));
   const size_t pairs = (size_t)p.pass_rows * a.top_k;
   p.off_inner = 0;
   p.off_pair = up256(pairs * a.inner * sizeof(float));
-  p.workspace = p.off_pair + up256(pairs * a.hidden * sizeof(float));
-  if (p.tiled) {
-    p.off_order = p.workspace;
-    p.off_x = p.off_order + 2 * up256(pairs * sizeof(int)) + 256 + up256(expert_tiles(pairs, a.experts) * sizeof(ExpertTile));
+  p.off_order = p.off_pair + up256(pairs * a.hidden * ds * sizeof(float));
+  p.off_x = p.off_order + 2 * up256(pairs * sizeof(int)) + 256 +
+            up256(expert_tiles(pairs, a.experts, p.tiled ? 128 : 16) * sizeof(ExpertTile));
+  if (p.tiled)
     p.workspace = Planes(Planes(p.off_x, p.pass_rows, a.hidden).end, pairs, a.inner).end;
-  }
+  else
+    p.workspace = p.off_x + (gs > 1 ? up256(2 * gs * pairs * a.inner * sizeof(float)) : 0);
   return p;
 }
+
+// The sorted pairs' places in the workspace.
+struct Sorted {
+  int *order, *place, *count;
+  ExpertTile *tiles;
+  Sorted(uint8_t *ws, const MoePlan &p, int top_k) {
+    const size_t n = up256((size_t)p.pass_rows * top_k * sizeof(int)) / sizeof(int);
+    order = reinterpret_cast<int *>(ws + p.off_order);
+    place = order + n;
+    count = place + n;
+    tiles = reinterpret_cast<ExpertTile *>(count + 64);
+  }
+};
 
 static hipError_t launch_planes(const float *x, int64_t x_stride, int64_t rows, const int *count, int K, uint8_t *ws,
                                 const Planes &p, hipStream_t s) {
@@ -681,29 +796,35 @@ static hipError_t launch_planes(const float *x, int64_t x_stride, int64_t rows, 
 }
 
 static hipError_t launch_sum(const MoeArgs &a, const float *y, const int32_t *ids, const int *place, int64_t rows,
-                             float *out, hipStream_t s) {
+                             int slices, float *out, hipStream_t s) {
+  const int64_t slice = rows * a.top_k * a.hidden;
   const bool wide = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && a.out_stride % 4 == 0;
   const dim3 grid((unsigned)rows, (unsigned)((a.hidden / (wide ? 4 : 1) + 255) / 256));
-  if (wide) launch_timed(moe_sum_kernel<4>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden, out, a.out_stride);
-  else launch_timed(moe_sum_kernel<1>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden, out, a.out_stride);
+  if (wide) launch_timed(moe_sum_kernel<4>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden,
+                         slices, slice, out, a.out_stride);
+  else launch_timed(moe_sum_kernel<1>, grid, dim3(256), 0u, s, y, ids, place, a.top_k, a.experts, a.hidden,
+                         slices, slice, out, a.out_stride);
   return hipGetLastError();
 }
 
 template <class F, int NM>
 static hipError_t launch_product(MoeProduct a, int cu_count, hipStream_t s) {
-  // as few rounds of super-blocks a wave as eight waves leave, then as few
-  // waves as that takes; the others take further column tiles
-  const int rounds = (a.nsb + kWaves - 1) / kWaves;
-  a.kw = (a.nsb + rounds - 1) / rounds;
-  a.slots = kWaves / a.kw;
-  const int tiles = (a.N + 15) / 16, jobs = std::min(a.pairs, a.experts);
-  const dim3 block(64 * a.kw * a.slots);
-  // two tiles a wave halve what a row's activations cost; one where the
-  // workgroups would not go round
-  if ((int64_t)jobs * ((tiles + 2 * a.slots - 1) / (2 * a.slots)) >= 4 * cu_count)
-    launch_timed(moe_stream_kernel<F, NM, 2>, dim3((tiles + 2 * a.slots - 1) / (2 * a.slots), jobs), block, 0u, s, a);
+  const int kw = (a.nsb + a.slices - 1) / a.slices;  // items of the longest slice
+  a.slots = kWaves / kw;
+  a.steps = ((a.N + 15) / 16 + a.slots - 1) / a.slots;
+  const dim3 block(64 * kw * a.slots);
+  // one workgroup a CU (its registers fill it), each with an even share of the steps
+  const int groups = std::max(1, cu_count / a.slices);
+  dim3 grid(groups, 1, a.slices);
+  if (!a.order) {
+    a.rounds = (int)((a.pairs * (int64_t)a.steps + groups - 1) / groups);
+    grid = dim3((a.steps + a.rounds - 1) / a.rounds, a.pairs, a.slices);
+  }
+  // Two tiles in flight a wave, where the registers hold them and there are more
+  if ((a.order || a.rounds > 2) && (NM == 1 || !F::kLow))
+    launch_timed(moe_stream_kernel<F, NM, NM == 1 || !F::kLow ? 2 : 1>, grid, block, 0u, s, a);
   else
-    launch_timed(moe_stream_kernel<F, NM, 1>, dim3((tiles + a.slots - 1) / a.slots, jobs), block, 0u, s, a);
+    launch_timed(moe_stream_kernel<F, NM, 1>, grid, block, 0u, s, a);
   return hipGetLastError();
 }
 
@@ -721,6 +842,7 @@ static MoeProduct product(int type, int K, int N, int experts) {
   p.N = N;
   p.experts = experts;
   p.nsb = (K + 255) / 256;
+  p.slices = k_slices(K);
   p.row_bytes = type == kQ8_0 ? K / 32 * kQ8Bytes : K / 256 * sb_bytes_of(type);
   p.expert_bytes = (uint64_t)N * (uint64_t)p.row_bytes;
   p.w_bytes = p.expert_bytes * (uint64_t)experts;
@@ -731,12 +853,11 @@ static MoeProduct product(int type, int K, int N, int experts) {
 static hipError_t tiled_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws, int64_t t0, int64_t rows, hipStream_t s) {
   const int64_t pairs = rows * a.top_k, room = plan.pass_rows * a.top_k;
   float *inner = reinterpret_cast<float *>(ws + plan.off_inner), *pair = reinterpret_cast<float *>(ws + plan.off_pair);
-  int *order = reinterpret_cast<int *>(ws + plan.off_order), *place = order + up256(room * sizeof(int)) / sizeof(int);
-  int *count = place + up256(room * sizeof(int)) / sizeof(int);
-  ExpertTile *tiles = reinterpret_cast<ExpertTile *>(count + 64);
+  const Sorted so(ws, plan, a.top_k);
   const Planes px(plan.off_x, plan.pass_rows, a.hidden), ph(px.end, room, a.inner);
   const int32_t *ids = a.ids + t0 * a.top_k;
-  launch_timed(moe_sort_kernel, dim3(1), dim3(1024), 0u, s, ids, (int)pairs, a.experts, order, place, count, tiles);
+  launch_timed(moe_sort_kernel, dim3(1), dim3(1024), 0u, s, ids, (int)pairs, a.experts, 128, so.order, so.place,
+               so.count, so.tiles);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) e = launch_planes(a.x + t0 * a.x_stride, a.x_stride, rows, nullptr, a.hidden, ws, px, s);
   if (e != hipSuccess) return e;
@@ -746,27 +867,27 @@ static hipError_t tiled_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws,
     mat.w[1] = m.w[1];
     mat.w_bytes = m.w_bytes;
     mat.expert_bytes = m.expert_bytes;
-    mat.order = order;
+    mat.order = so.order;
     mat.weights = a.weights + t0 * a.top_k;
     mat.y = y;
     mat.n = m.N;
     mat.row_bytes = m.row_bytes;
     mat.top_k = a.top_k;
     return launch_experts(type, gate_up, reinterpret_cast<_Float16 *>(ws + p.hi), reinterpret_cast<_Float16 *>(ws + p.lo),
-                          ws + p.sums, reinterpret_cast<float *>(ws + p.rscale), (int)n, whole(m.K), mat, count, tiles,
-                          expert_tiles(pairs, a.experts), s);
+                          ws + p.sums, reinterpret_cast<float *>(ws + p.rscale), (int)n, whole(m.K), mat, so.count, so.tiles,
+                          expert_tiles(pairs, a.experts, 128), s);
   };
   MoeProduct g = product(a.gate_up_type, a.hidden, a.inner, a.experts);
   g.w[0] = a.gate;
   g.w[1] = a.up;
   e = run(a.gate_up_type, true, g, px, rows, inner);
-  if (e == hipSuccess) e = launch_planes(inner, a.inner, pairs, count, a.inner, ws, ph, s);
+  if (e == hipSuccess) e = launch_planes(inner, a.inner, pairs, so.count, a.inner, ws, ph, s);
   if (e != hipSuccess) return e;
   MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
   d.w[0] = a.down;
   e = run(a.down_type, false, d, ph, pairs, pair);
   if (e != hipSuccess) return e;
-  return launch_sum(a, pair, ids, place, rows, a.out + t0 * a.out_stride, s);
+  return launch_sum(a, pair, ids, so.place, rows, 1, a.out + t0 * a.out_stride, s);
 }
 
 // The same with each expert's weights streamed past its rows.
@@ -780,9 +901,28 @@ static hipError_t stream_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws
   g.w[0] = a.gate;
   g.w[1] = a.up;
   g.ids = a.ids + t0 * a.top_k;
-  g.y = inner;
+  g.y = g.slices > 1 ? reinterpret_cast<float *>(ws + plan.off_x) : inner;
   g.pairs = (int)(rows * a.top_k);
+  // One row's experts differ; of more rows', half of the experts' number still
+  // mostly do (26 pairs of 8 experts, 4096 x 14336, unsorted: 590 us, most
+  // workgroups having found an earlier pair of their expert; sorted: 300)
+  if (g.pairs > kFewPairs || (rows > 1 && 2 * g.pairs > a.experts)) {
+    const Sorted so(ws, plan, a.top_k);
+    launch_timed(moe_sort_kernel, dim3(1), dim3(1024), 0u, s, g.ids, g.pairs, a.experts, 16, so.order, so.place, so.count,
+                 so.tiles);
+    const hipError_t sorted = hipGetLastError();
+    if (sorted != hipSuccess) return sorted;
+    g.order = so.order;
+    g.count = so.count;
+    g.jobs = so.tiles;
+  }
   hipError_t e = launch_product<2>(a.gate_up_type, g, cu_count, s);
+  if (e == hipSuccess && g.slices > 1) {  // (a pair without an expert: whatever lies there, which nothing reads)
+    const int64_t n4 = (int64_t)g.pairs * a.inner / 4;
+    launch_timed(moe_gate_kernel, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0u, s,
+                 reinterpret_cast<const float4 *>(g.y), g.slices, n4, reinterpret_cast<float4 *>(inner));
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) return e;
   MoeProduct d = product(a.down_type, a.inner, a.hidden, a.experts);
   d.x = inner;
@@ -793,9 +933,12 @@ static hipError_t stream_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws
   d.weights = a.weights + t0 * a.top_k;
   d.y = pair;
   d.pairs = g.pairs;
+  d.order = g.order;
+  d.count = g.count;
+  d.jobs = g.jobs;
   e = launch_product<1>(a.down_type, d, cu_count, s);
   if (e != hipSuccess) return e;
-  return launch_sum(a, pair, g.ids, nullptr, rows, a.out + t0 * a.out_stride, s);
+  return launch_sum(a, pair, g.ids, nullptr, rows, d.slices, a.out + t0 * a.out_stride, s);
 }
 
 hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s) {
