@@ -561,16 +561,29 @@ __global__ __launch_bounds__(256) void moe_gate_kernel(const float4 *__restrict_
 __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs, int experts,
                                                         int height, int *__restrict__ order, int *__restrict__ place,
                                                         int *__restrict__ count, ExpertTile *__restrict__ tiles) {
-  constexpr int kPer = kMoeMaxExperts / 1024;
+  constexpr int kPer = kMoeMaxExperts / 1024, kHeld = 16;
   __shared__ int next[kMoeMaxExperts];
   __shared__ int2 waves[16];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int e = tid; e < kMoeMaxExperts; e += 1024) next[e] = 0;
   __syncthreads();
-#pragma unroll 8
-  for (int p = tid; p < pairs; p += 1024) {
-    const int e = ids[p];
-    if ((uint32_t)e < (uint32_t)experts) atomicAdd(&next[e], 1);
+  // kHeld ids of a thread are requested at once; the first of them stay for the
+  // second pass
+  int held[kHeld];
+  auto get = [&](int p0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int p = p0 + 1024 * i + tid;
+      const int e = ids[p < pairs ? p : 0];
+      held[i] = p < pairs && (uint32_t)e < (uint32_t)experts ? e : -1;
+    }
+  };
+  const int last = (pairs - 1) / (1024 * kHeld) * (1024 * kHeld);
+  for (int p0 = last; p0 >= 0; p0 -= 1024 * kHeld) {
+    get(p0);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (held[i] >= 0) atomicAdd(&next[held[i]], 1);
   }
   __syncthreads();
   // rows and tiles ahead of each expert: kPer experts a thread
@@ -610,15 +623,17 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
     count[1] = r;
   }
   __syncthreads();
-#pragma unroll 8
-  for (int p = tid; p < pairs; p += 1024) {
-    const int e = ids[p];
-    int at = -1;
-    if ((uint32_t)e < (uint32_t)experts) {
-      at = atomicAdd(&next[e], 1);
-      order[at] = p;
+  for (int p0 = 0; p0 <= last; p0 += 1024 * kHeld) {
+    if (p0) get(p0);
+    int at[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) at[i] = held[i] >= 0 ? atomicAdd(&next[held[i]], 1) : -1;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int p = p0 + 1024 * i + tid;
+      if (p < pairs) place[p] = at[i];
+      if (at[i] >= 0) order[at[i]] = p;
     }
-    place[p] = at;
   }
 }
 

@@ -23,7 +23,11 @@ namespace {
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;
-constexpr int kWaves = 8, kRows = 16;  // of a workgroup; token rows of a tile
+constexpr int kRows = 16;  // token rows of a tile
+// waves of a workgroup of NT expert tiles: a row each for the choice where a
+// tile's registers leave room
+constexpr int waves_of(int NT) { return NT == 1 ? 16 : 8; }
+constexpr int kMostSlices = 4;
 
 template <int kType>
 struct WType {
@@ -38,19 +42,17 @@ struct WType<kBF16> {
   typedef __bf16 type;
 };
 
-// Values k .. k + 3 of a row of n (none past its end), one load each, or one
-// for all four.
+// Values k .. k + 3 of a row, one load each, or one for all four.
 template <class T, bool kWide>
-__device__ __forceinline__ void get4(const T *row, int k, int n, float v[4]) {
+__device__ __forceinline__ void get4(const T *row, int k, T v[4]) {
   if constexpr (kWide) {
     typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 t = {};
-    if (k < n) t = *reinterpret_cast<const T4 *>(row + k);  // n a multiple of 4
+    const T4 t = *reinterpret_cast<const T4 *>(row + k);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+    for (int e = 0; e < 4; ++e) v[e] = t[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = k + e < n ? (float)row[k + e] : 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = row[k + e];
   }
 }
 
@@ -88,33 +90,48 @@ __device__ __forceinline__ double wave_fold(double v, bool sum) {
   return v;
 }
 
-// The choice for one row by one wave.  z: its logits in LDS, E of them, left
-// as scores; c: as many values of scratch.
-__device__ __forceinline__ void choose(const RouteArgs &a, int row, double *z, double *c, int lane) {
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane));
+}
+
+// The choice for one row by one wave: experts lane, lane + 64, ... of up to 64 N
+// in registers.  z: its logits in LDS, left as what groups are chosen by.
+template <int N>
+__device__ __forceinline__ void choose(const RouteArgs &a, int row, double *z, int lane) {
   const int E = a.experts;
-  double top = -INFINITY;
+  double p[N], c[N], top = -INFINITY;
   bool nan = false;
-  for (int e = lane; e < E; e += 64) {
-    if (a.logits) a.logits[(int64_t)row * E + e] = (float)z[e];
-    nan = nan || __builtin_isnan(z[e]);
-    top = __builtin_fmax(top, z[e]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = lane + 64 * i;
+    p[i] = e < E ? z[e] : -INFINITY;
+    if (a.logits && e < E) a.logits[(int64_t)row * E + e] = (float)p[i];
+    nan = nan || __builtin_isnan(p[i]);
+    top = __builtin_fmax(top, p[i]);
   }
   if (a.sigmoid) {
-    for (int e = lane; e < E; e += 64) z[e] = 1.0 / (1.0 + exp(-z[e]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = 1.0 / (1.0 + exp(-p[i]));
   } else {
     top = wave_fold(top, false);
     double sum = 0.0;
-    for (int e = lane; e < E; e += 64) {
-      z[e] = exp(z[e] - top);
-      sum += z[e];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      p[i] = exp(p[i] - top);
+      sum += lane + 64 * i < E ? p[i] : 0.0;
     }
     sum = wave_fold(sum, true);
-    for (int e = lane; e < E; e += 64) z[e] /= sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] /= sum;
   }
-  for (int e = lane; e < E; e += 64) {
-    const double v = a.choice_bias ? z[e] + (double)a.choice_bias[e] : z[e];
-    nan = nan || __builtin_isnan(v);
-    c[e] = v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = lane + 64 * i;
+    c[i] = p[i] + (a.choice_bias && e < E ? (double)a.choice_bias[e] : 0.0);
+    nan = nan || (e < E && __builtin_isnan(c[i]));
+    if (e >= E) c[i] = -INFINITY;
   }
   const int64_t at = (int64_t)row * a.top_k;
   if (__builtin_amdgcn_ballot_w64(nan) != 0) {
@@ -124,48 +141,60 @@ __device__ __forceinline__ void choose(const RouteArgs &a, int row, double *z, d
     }
     return;
   }
-  wave_sync();
   if (a.groups > 1) {
-    // lane g: group g's best one or two, then its place among the groups
-    const int size = E / a.groups;
+    // 2^share lanes a group, each with its best one or two of every so many;
+    // they meet, then the group's place among the groups
+    const int size = E / a.groups, share = 31 - __builtin_clz(64 / a.groups);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 64 * i < E) z[lane + 64 * i] = c[i];
+    wave_sync();
+    const int group = lane >> share;
     double one = -INFINITY, two = -INFINITY;
-    if (lane < a.groups)
-      for (int i = 0; i < size; ++i) {
-        const double v = c[lane * size + i];
+    if (group < a.groups)
+      for (int i = lane & ((1 << share) - 1); i < size; i += 1 << share) {
+        const double v = z[group * size + i];
         two = __builtin_fmax(two, __builtin_fmin(one, v));
         one = __builtin_fmax(one, v);
       }
-    const uint64_t mine = order_of(a.group_best == 2 && size > 1 ? one + two : one);
+    for (int d = 1; d < 1 << share; d *= 2) {
+      const double o = __shfl_xor(one, d), t = __shfl_xor(two, d);
+      two = __builtin_fmax(__builtin_fmin(one, o), __builtin_fmax(two, t));
+      one = __builtin_fmax(one, o);
+    }
+    const double mine = a.group_best == 2 && size > 1 ? one + two : one;
     int place = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), g) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, g);
-      place += o > mine || (o == mine && g < lane) ? 1 : 0;
+      const double o = lane_of(mine, g << share);
+      place += o > mine || (o == mine && g < group) ? 1 : 0;
     }
-    const uint64_t stay = __builtin_amdgcn_ballot_w64(lane < a.groups && place < a.top_groups);
-    wave_sync();
-    for (int e = lane; e < E; e += 64)
-      if (!((stay >> (e / size)) & 1)) c[e] = -INFINITY;
-    wave_sync();
+    const uint64_t stay = __builtin_amdgcn_ballot_w64(group < a.groups && place < a.top_groups);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!((stay >> ((((lane + 64 * i) / size) << share) & 63)) & 1)) c[i] = -INFINITY;
   }
   // one expert after the other; lane j keeps the j-th
+  uint64_t key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) key[i] = order_of(c[i]);
   double sum = 0.0, kept = 0.0;
   int id = -1;
   for (int j = 0; j < a.top_k; ++j) {
-    uint64_t key = kOrderNone;
+    uint64_t best = kOrderNone;
+    double score = 0.0;
     int index = 0x7ffffffe;
-    for (int e = lane; e < E; e += 64) {
-      const uint64_t k = order_of(c[e]);
-      if (k > key) key = k, index = e;
-    }
-    uint64_t best;
-    const int e = wave_best(key, index, best);
-    if (best == kOrderNone) break;  // nothing left but -infinity
-    const double p = z[e];
-    sum += p;
-    if (lane == j) kept = p, id = e;
-    if (lane == (e & 63)) c[e] = -INFINITY;
-    wave_sync();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (key[i] > best) best = key[i], score = p[i], index = lane + 64 * i;
+    uint64_t all;
+    const int e = wave_best(best, index, all);
+    if (all == kOrderNone) break;  // nothing left but -infinity
+    const double chosen = lane_of(score, e & 63);
+    sum += chosen;
+    if (lane == j) kept = chosen, id = e;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (e == lane + 64 * i) key[i] = kOrderNone;
   }
   if (lane < a.top_k) {
     if (a.renormalise) kept = sum > 0.0 ? kept / sum : 0.0;
@@ -180,67 +209,111 @@ __device__ __forceinline__ void choose(const RouteArgs &a, int row, double *z, d
 // of the tokens and of the experts, and of each 16 values of K the four from
 // 4 (l / 16) on, one load of each for four products.  (The order of K inside
 // a step is the same on both sides, so it does not matter which value is
-// which.)  The f64 pipe takes 64 cycles a product, which bounds long batches:
-// 2048 flops a conversion of two values, so nothing is staged.
+// which.)  The f64 pipe takes 64 cycles a product, which bounds long batches.
 //
-// whole: the workgroup has all experts of its 16 rows, wt waves side by side
-// over the expert tiles and kWaves / wt over K.  Otherwise it has one expert
-// tile and one slice of K, its waves split that, and the tile's last
-// workgroup adds the slices up in their order.
-template <int kType, bool kWide>
-__global__ __launch_bounds__(kWaves * 64) void route_kernel(RouteArgs a, RoutePlan plan, double *part, uint32_t *arrived) {
+// A workgroup's waves split K between them, and each takes NT expert tiles at
+// once: every value is read and widened once a workgroup.  (A tile a wave, all
+// waves over the same tokens' rows, read those from the L2 eight times: 4096 x
+// 2048 with 128 experts 75 us, now TIME.)  They meet in LDS in pairs.
+//
+// whole: the workgroup has all experts of its 16 rows.  Otherwise it has NT
+// tiles and one slice of K, and the rows' last workgroup adds the slices up in
+// their order.
+template <int kType, bool kWide, int NT>
+__global__ __launch_bounds__(waves_of(NT) * 64) void route_kernel(RouteArgs a, RoutePlan plan, double *part,
+                                                                  uint32_t *arrived) {
   typedef typename WType<kType>::type T;
+  constexpr int kWaves = waves_of(NT);
+  constexpr int kAhead = NT == 1 ? 4 : 8 / NT < 2 ? 2 : 8 / NT;  // chunks of 16 values in flight
   extern __shared__ __align__(16) double lds[];
-  __shared__ double meet[kWaves][256];
+  __shared__ f64x4 meet[kWaves / 2][NT][64];
   __shared__ int last;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int E = a.experts, tiles = (E + 15) / 16, K = a.hidden;
-  const int row0 = (int)blockIdx.x * kRows;
-  double *z = lds, *c = lds + kRows * E;  // [16][E]
+  const int row0 = (int)blockIdx.x * kRows, rows = std::min(kRows, a.rows - row0);
+  double *z = lds;  // [16][E]
 
-  const int wt = plan.whole ? (tiles >= 8 ? 8 : tiles > 2 ? 4 : tiles) : 1, wk = kWaves / wt;
-  const int ks = wave / wt;  // this wave's share of K
   const int k_lo = plan.whole ? 0 : (int)blockIdx.z * plan.span, k_hi = plan.whole ? K : std::min(K, k_lo + plan.span);
   const int chunks = (k_hi - k_lo + 15) / 16;
-  const int c_lo = chunks * ks / wk, c_hi = chunks * (ks + 1) / wk;
+  const int c_lo = chunks * wave / kWaves, c_hi = chunks * (wave + 1) / kWaves, c_full = std::min(c_hi, (k_hi - k_lo) / 16);
   const float *xr = a.x + (int64_t)std::min(row0 + n, a.rows - 1) * a.x_stride;
-  // element i of lane l in D: row 4 i + l / 16, column l % 16
-  for (int t0 = plan.whole ? 0 : (int)blockIdx.y; t0 < (plan.whole ? tiles : (int)blockIdx.y + 1); t0 += wt) {
-    const int t = t0 + wave % wt;
-    const T *wr = static_cast<const T *>(a.w) + (int64_t)std::min(16 * t + n, E - 1) * K;
-    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-    if (t < tiles) {
-#pragma unroll 4
-      for (int ch = c_lo; ch < c_hi; ++ch) {
-        float xv[4], wv[4];
-        const int k = k_lo + 16 * ch + 4 * g;
-        get4<float, kWide>(xr, k, k_hi, xv);
-        get4<T, kWide>(wr, k, k_hi, wv);
+  for (int t0 = plan.whole ? 0 : (int)blockIdx.y * NT; t0 < (plan.whole ? tiles : (int)blockIdx.y * NT + 1); t0 += NT) {
+    f64x4 acc[NT] = {};
+    const T *wr[NT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv[e], (double)wv[e], acc, 0, 0, 0);
+    for (int t = 0; t < NT; ++t) wr[t] = static_cast<const T *>(a.w) + (int64_t)std::min(16 * (t0 + t) + n, E - 1) * K;
+    // past the last whole chunk it is loaded again, and dropped
+    float xv[kAhead][4];
+    T wv[kAhead][NT][4];
+    auto load = [&](int i, int ch) {
+      const int k = k_lo + 16 * std::min(ch, c_full - 1) + 4 * g;
+      get4<float, kWide>(xr, k, xv[i]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) get4<T, kWide>(wr[t], k, wv[i][t]);
+    };
+    auto times = [&](int i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv[i][e], (double)(float)wv[i][t][e], acc[t], 0, 0, 0);
+    };
+    if (c_lo < c_full) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) load(i, c_lo + i);
+      int ch = c_lo;
+      for (; ch + kAhead <= c_full; ch += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          times(i);
+          __builtin_amdgcn_sched_barrier(0);
+          load(i, ch + i + kAhead);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (ch + i < c_full) times(i);
     }
-    if (wk > 1) {  // the waves of one expert tile meet, in their order
+    if (c_full < c_hi) {  // the last chunk of the row, zeros behind its end
+      const int k = k_lo + 16 * c_full + 4 * g;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) meet[wave][64 * i + lane] = acc[i];
+      for (int e = 0; e < 4; ++e) {
+        const int at = std::min(k + e, K - 1);
+        const float x = xr[at];
+        xv[0][e] = k + e < K ? x : 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const T w = wr[t][at];
+          wv[0][t][e] = k + e < K ? w : (T)0.0f;
+        }
+      }
+      times(0);
+    }
+    for (int half = kWaves / 2; half > 0; half /= 2) {
+      if (wave >= half && wave < 2 * half)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) meet[wave - half][t][lane] = acc[t];
       __syncthreads();
-      if (ks == 0)
-        for (int o = 1; o < wk; ++o)
+      if (wave < half)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] += meet[wave + o * wt][64 * i + lane];
+        for (int t = 0; t < NT; ++t) acc[t] += meet[wave][t][lane];
       __syncthreads();
     }
-    if (ks == 0 && 16 * t + n < E) {
-      const int e = 16 * t + n;
+    if (wave == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * i + g;
-        if (plan.whole) {
-          z[r * E + e] = acc[i] + (a.bias ? (double)a.bias[e] : 0.0);
-        } else {
-          double *to = part + (((int64_t)blockIdx.x * plan.slices + blockIdx.z) * kRows + r) * E + e;
-          __hip_atomic_store(to, acc[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int t = 0; t < NT; ++t) {
+        const int e = 16 * (t0 + t) + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * i + g;  // element i of lane l in D: row 4 i + l / 16, column l % 16
+          if (r >= rows || e >= E) continue;
+          if (plan.whole) {
+            z[r * E + e] = acc[t][i] + (a.bias ? (double)a.bias[e] : 0.0);
+          } else {
+            double *to = part + (((int64_t)blockIdx.x * plan.slices + blockIdx.z) * kRows + r) * E + e;
+            __hip_atomic_store(to, acc[t][i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
         }
       }
     }
@@ -256,30 +329,37 @@ __global__ __launch_bounds__(kWaves * 64) void route_kernel(RouteArgs a, RoutePl
     if (!last) return;
     if (tid == 0) __hip_atomic_store(mine, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const double *from = part + (int64_t)blockIdx.x * plan.slices * kRows * E;
-    for (int i = tid; i < kRows * E; i += kWaves * 64) {
-      double v = a.bias ? (double)a.bias[i % E] : 0.0;
-      double s = 0.0;
-      for (int o = 0; o < plan.slices; ++o)
-        s += __hip_atomic_load(from + (int64_t)o * kRows * E + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      z[i] = s + v;
+    for (int i = tid; i < rows * E; i += kWaves * 64) {
+      double v[kMostSlices];  // requested together
+#pragma unroll
+      for (int o = 0; o < kMostSlices; ++o)
+        v[o] = o < plan.slices ? __hip_atomic_load(from + (int64_t)o * kRows * E + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+#pragma unroll
+      for (int o = 1; o < kMostSlices; ++o) v[0] += v[o];
+      z[i] = v[0] + (a.bias ? (double)a.bias[i % E] : 0.0);
     }
   }
   __syncthreads();
-  for (int r = wave; r < kRows && row0 + r < a.rows; r += kWaves) choose(a, row0 + r, z + r * E, c + r * E, lane);
+  for (int r = wave; r < rows; r += kWaves) {
+    if (E <= 128) choose<2>(a, row0 + r, z + r * E, lane);
+    else if (E <= 256) choose<4>(a, row0 + r, z + r * E, lane);
+    else choose<8>(a, row0 + r, z + r * E, lane);
+  }
 }
 
 RoutePlan route_plan(const RouteArgs &a, int cu_count) {
   RoutePlan p{};
   p.tiles = (a.rows + kRows - 1) / kRows;
-  p.lds = (size_t)2 * kRows * a.experts * sizeof(double);
+  p.lds = (size_t)kRows * a.experts * sizeof(double);
   const int et = (a.experts + 15) / 16;
   // a workgroup per tile of rows once those fill half the card
   p.whole = p.tiles >= cu_count / 2;
   if (!p.whole) {
-    // slices of at least 512 values (64 a wave), about two workgroups a CU
-    const int want = std::max(1, 2 * cu_count / (p.tiles * et));
-    const int most = std::max(1, a.hidden / 512);
-    const int s = std::min({want, most, 16});
+    // an expert tile a workgroup, slices of at least 1024 values (64 a wave),
+    // about a workgroup a CU
+    const int want = std::max(1, cu_count / (p.tiles * et));
+    const int most = std::max(1, a.hidden / 1024);
+    const int s = std::min({want, most, kMostSlices});
     p.span = ((a.hidden + s - 1) / s + 15) / 16 * 16;
     p.slices = (a.hidden + p.span - 1) / p.span;
     p.part_bytes = (size_t)p.tiles * p.slices * kRows * a.experts * sizeof(double);
@@ -288,21 +368,25 @@ RoutePlan route_plan(const RouteArgs &a, int cu_count) {
   return p;
 }
 
-hipError_t launch_route(const RouteArgs &a, const RoutePlan &p, void *part, void *arrived, hipStream_t s) {
+template <int kType, bool kWide>
+static void launch_route(const RouteArgs &a, const RoutePlan &p, double *part, uint32_t *arrived, hipStream_t s) {
   const int et = (a.experts + 15) / 16;
   const dim3 grid((unsigned)p.tiles, p.whole ? 1u : (unsigned)et, p.whole ? 1u : (unsigned)p.slices);
+  const unsigned lds = (unsigned)p.lds;
+  if (!p.whole || et == 1) launch_timed(route_kernel<kType, kWide, 1>, grid, dim3(waves_of(1) * 64), lds, s, a, p, part, arrived);
+  else if (et <= 4) launch_timed(route_kernel<kType, kWide, 4>, grid, dim3(waves_of(4) * 64), lds, s, a, p, part, arrived);
+  else launch_timed(route_kernel<kType, kWide, 8>, grid, dim3(waves_of(8) * 64), lds, s, a, p, part, arrived);
+}
+
+hipError_t launch_route(const RouteArgs &a, const RoutePlan &p, void *part, void *arrived, hipStream_t s) {
   const bool wide = a.hidden % 4 == 0 && a.x_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
   double *pt = static_cast<double *>(part);
   uint32_t *ar = static_cast<uint32_t *>(arrived);
-#define OKQ_ROUTE(T_)                                                                                          \
-  {                                                                                                            \
-    if (wide) launch_timed(route_kernel<T_, true>, grid, dim3(kWaves * 64), (unsigned)p.lds, s, a, p, pt, ar);  \
-    else launch_timed(route_kernel<T_, false>, grid, dim3(kWaves * 64), (unsigned)p.lds, s, a, p, pt, ar);      \
-  }
-  if (a.w_type == kF16) OKQ_ROUTE(kF16)
-  else if (a.w_type == kBF16) OKQ_ROUTE(kBF16)
-  else OKQ_ROUTE(kF32)
+#define OKQ_ROUTE(T_) wide ? launch_route<T_, true>(a, p, pt, ar, s) : launch_route<T_, false>(a, p, pt, ar, s)
+  if (a.w_type == kF16) OKQ_ROUTE(kF16);
+  else if (a.w_type == kBF16) OKQ_ROUTE(kBF16);
+  else OKQ_ROUTE(kF32);
 #undef OKQ_ROUTE
   return hipGetLastError();
 }
