@@ -405,14 +405,15 @@ enum {
  *   weights[r]: their p, divided by their sum (zeros where it is 0) if
  *     renormalise, times scale
  * x: device f32, row r at r * x_stride; w [experts, hidden] of w_type
- * (OKQ_TYPE_F32, F16 or BF16); bias, choice_bias [experts] f32 or NULL; ids
+ * (OKQ_TYPE_F32, F16 or BF16); bias, choice_bias [experts] f32 or NULL, the
+ * latter finite or -infinity; ids
  * [rows, top_k] int32, weights [rows, top_k] f32, logits [rows, experts] f32
  * or NULL: z.  All of it is computed in 64 bits and rounded at the stores, so
  * a row's experts do not change with the rows around it.  An expert of c =
  * -infinity is never chosen: where too few are left, ids are -1 and weights
  * 0.  A row with a NaN among its z or c gets ids of -1 and weights of NaN.
  * experts at most 512, groups at most 64, top_k at most 64 and at most the
- * experts of top_groups groups.  rows == 0 is a no-op.  Uses a per-stream
+ * experts of top_groups groups, rows at most 2^26.  rows == 0 is a no-op.  Uses a per-stream
  * workspace.  No counterpart in the reference, whose only sparse model is
  * refused (crates/models/src/qwen/qwen3_5.rs). */
 okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, uint32_t w_type, const void *w,
@@ -425,7 +426,7 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
  * gate_w, up_w (of one type) and down_w: GGUF tensors stacked over the experts,
  * [hidden, intermediate, experts] and [intermediate, hidden, experts] in ne
  * order, types Q8_0, Q4_K, Q5_K or Q6_K; hidden and intermediate are multiples
- * of the block of the tensors whose rows they are.  x, out: device f32, row r
+ * of the block of the tensors whose rows they are, at most 2^23.  x, out: device f32, row r
  * at r * its stride, x 16-byte aligned with a stride that is a multiple of 4.
  * ids, weights [rows, top_k]; an id outside [0, experts) adds nothing whatever
  * its weight is, so a row of such ids gets zeros; the same id twice in a row

@@ -318,7 +318,8 @@ struct RouteArgs {
 struct RoutePlan {
   int tiles, slices, span;  // span: values of a slice
   bool whole;
-  size_t part_bytes, arrived_bytes, lds;
+  size_t part_bytes, arrived_bytes;  // arrived: zero before and after every call
+  size_t lds;
 };
 RoutePlan route_plan(const RouteArgs &a, int cu_count);
 hipError_t launch_route(const RouteArgs &a, const RoutePlan &plan, void *part, void *arrived, hipStream_t s);
@@ -335,6 +336,7 @@ struct MoeArgs {
   float *out;
 };
 constexpr int kMoeMaxExperts = 4096;  // counted in LDS
+constexpr int64_t kMoeMaxWidth = 1 << 23;  // of hidden and intermediate: a row's pairs and tiles count in 32 bits
 // The workspace, and how many rows a pass over it takes (longer batches go in
 // several).  tiled: the pairs sorted by expert into MFMA tiles of up to 128
 // rows (okq_experts.hip); else each expert's weights stream past 16 of its
@@ -343,8 +345,9 @@ struct MoePlan {
   bool tiled;
   int64_t pass_rows;
   size_t off_inner, off_pair, off_order, off_x, workspace;
+  size_t reserve;  // what any call of the same tensors with no more rows needs, at least
 };
-MoePlan moe_plan(const MoeArgs &a, int cu_count);
+MoePlan moe_plan(const MoeArgs &a);
 hipError_t launch_moe(const MoeArgs &a, const MoePlan &plan, void *workspace, int cu_count, hipStream_t s);
 
 // Rows of one expert that share MFMA tiles: [row0, row0 + rows) of the pairs

@@ -757,14 +757,14 @@ struct Planes {
 // Slices of K of at most kWaves items.
 static int k_slices(int K) { return ((K + 255) / 256 + kWaves - 1) / kWaves; }
 
-MoePlan moe_plan(const MoeArgs &a, int) {
+static MoePlan plan_of(const MoeArgs &a, bool tiled) {
   MoePlan p{};
-  p.tiled = (int64_t)a.rows * a.top_k >= 12 * (int64_t)a.experts && (int64_t)a.rows * a.top_k > 32;
+  p.tiled = tiled;
   const size_t gs = p.tiled ? 1 : k_slices(a.hidden), ds = p.tiled ? 1 : k_slices(a.inner);
   // a pass keeps to about 1 GiB of results, and to what its kernels count in
   // 32 bits
   const int64_t one = 4 * ((int64_t)a.inner * (gs > 1 ? 1 + 2 * gs : 2) + (int64_t)a.hidden * ds);
-  const int64_t most = std::max<int64_t>(256, std::min<int64_t>(65536, (1 << 30) / one));
+  const int64_t most = std::min<int64_t>({65536, (1 << 30) / one, (UINT32_MAX - (1 << 20)) / (2 * (int64_t)whole(std::max(a.inner, a.hidden)))});
   p.pass_rows = std::max<int64_t>(1, std::min<int64_t>(a.rows, most / a.top_k));
   const size_t pairs = (size_t)p.pass_rows * a.top_k;
   p.off_inner = 0;
@@ -776,6 +776,23 @@ MoePlan moe_plan(const MoeArgs &a, int) {
     p.workspace = Planes(Planes(p.off_x, p.pass_rows, a.hidden).end, pairs, a.inner).end;
   else
     p.workspace = p.off_x + (gs > 1 ? up256(2 * gs * pairs * a.inner * sizeof(float)) : 0);
+  return p;
+}
+
+MoePlan moe_plan(const MoeArgs &a) {
+  // Sorted tiles from 28 rows an expert on average, where they begin to be the
+  // faster ones: at 24 and 32, us streamed / tiled, 2048 x 768 Q4_K and Q6_K with
+  // 128 experts 237 / 248 and 298 / 275, 2048 x 1536 Q5_K and Q8_0 with 32 150 /
+  // 157 and 173 / 168, 4096 x 4096 Q6_K with 8 199 / 215 and 251 / 239.
+  const int64_t least = 28 * (int64_t)a.experts;  // pairs
+  const bool tiled = (int64_t)a.rows * a.top_k >= least;
+  MoePlan p = plan_of(a, tiled);
+  p.reserve = p.workspace;
+  if (tiled) {
+    MoeArgs streamed = a;
+    streamed.rows = (int)((least + a.top_k - 1) / a.top_k);
+    p.reserve = std::max(p.reserve, plan_of(streamed, false).workspace);
+  }
   return p;
 }
 

@@ -357,14 +357,16 @@ RoutePlan route_plan(const RouteArgs &a, int cu_count) {
   if (!p.whole) {
     // an expert tile a workgroup, slices of at least 1024 values (64 a wave),
     // about a workgroup a CU
-    const int want = std::max(1, cu_count / (p.tiles * et));
+    const int want = std::max(1, std::min(cu_count / (p.tiles * et), cu_count / 2 / p.tiles));
     const int most = std::max(1, a.hidden / 1024);
     const int s = std::min({want, most, kMostSlices});
     p.span = ((a.hidden + s - 1) / s + 15) / 16 * 16;
     p.slices = (a.hidden + p.span - 1) / p.span;
-    p.part_bytes = (size_t)p.tiles * p.slices * kRows * a.experts * sizeof(double);
-    p.arrived_bytes = (size_t)p.tiles * 128;
   }
+  // the same for every call (tiles * slices is at most half of cu_count, or
+  // cu_count / et), so that any first call makes room for a captured one
+  p.part_bytes = (size_t)cu_count * kRows * kMaxExperts / 2 * sizeof(double);
+  p.arrived_bytes = (size_t)cu_count / 2 * 128;
   return p;
 }
 

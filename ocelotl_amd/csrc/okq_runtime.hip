@@ -1434,8 +1434,8 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
   if (w_type != OKQ_TYPE_F32 && w_type != OKQ_TYPE_F16 && w_type != OKQ_TYPE_BF16)
     return fail(OKQ_E_TYPE, "unsupported %s weight: tensor type %s (%u); supported: F32, F16, BF16", what,
                 type_name(w_type), w_type);
-  if (rows < 0 || hidden < 1 || experts < 1 || rows > INT32_MAX || hidden > 1 << 30 || experts > okq::kMaxExperts)
-    return fail(OKQ_E_SHAPE, "%s rows=%lld hidden=%lld experts=%lld: hidden must be 1 to 2^30, experts 1 to %d", what,
+  if (rows < 0 || hidden < 1 || experts < 1 || rows > 1 << 26 || hidden > 1 << 30 || experts > okq::kMaxExperts)
+    return fail(OKQ_E_SHAPE, "%s rows=%lld hidden=%lld experts=%lld: rows must be at most 2^26, hidden 1 to 2^30, experts 1 to %d", what,
                 (long long)rows, (long long)hidden, (long long)experts, okq::kMaxExperts);
   if (groups < 1 || groups > okq::kMaxGroups || experts % groups != 0 || top_groups < 1 || top_groups > groups)
     return fail(OKQ_E_SHAPE, "%s groups=%lld top_groups=%lld: up to %d equal groups of %lld experts, top_groups 1 to groups",
@@ -1486,11 +1486,9 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
   std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
   const okq::RoutePlan plan = okq::route_plan(a, info.cu_count);
   void *part = nullptr, *arrived = nullptr;
-  if (plan.part_bytes) {
-    st = get_workspace(dev, s, plan.part_bytes, &part, 5, what);
-    if (st == OKQ_OK) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 6, what);
-    if (st != OKQ_OK) return st;
-  }
+  st = get_workspace(dev, s, plan.part_bytes, &part, 5, what);
+  if (st == OKQ_OK) st = get_zeroed_workspace(dev, s, plan.arrived_bytes, &arrived, 6, what);
+  if (st != OKQ_OK && !plan.whole) return st;
   return hip_status(okq::launch_route(a, plan, part, arrived, s), "moe_route launch");
 }
 
@@ -1517,8 +1515,9 @@ okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t
   for (const Tensor &t : tensors) {
     TypeInfo ti;
     if (!type_info(t.type, ti) || !ti.linear) return unsupported_type(t.type, "moe_mlp weight");
-    if (t.K < 1 || t.N < 1 || t.K > INT32_MAX / 2 || t.N > INT32_MAX / 2 || t.K % ti.elems != 0)
-      return fail(OKQ_E_SHAPE, "%s %s rows of %lld values for %lld outputs: not a positive multiple of the %s block size %lld, or too large",
+    if (t.K < 1 || t.N < 1 || t.K > okq::kMoeMaxWidth || t.N > okq::kMoeMaxWidth || t.K % ti.elems != 0)
+      return fail(OKQ_E_SHAPE,
+                  "%s %s rows of %lld values for %lld outputs: not a positive multiple of the %s block size %lld, or above 2^23",
                   what, t.name, (long long)t.K, (long long)t.N, type_name(t.type), (long long)ti.elems);
     int64_t one, all;
     if (!mul_ok(t.N, t.K / ti.elems * ti.bytes, one) || one > (int64_t)UINT32_MAX - 1024 || !mul_ok(one, experts, all))
@@ -1563,9 +1562,9 @@ okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t
   a.out = out;
   hipStream_t s = static_cast<hipStream_t>(stream);
   std::lock_guard<std::recursive_mutex> enqueue(stream_lock(dev, s));
-  const okq::MoePlan plan = okq::moe_plan(a, info.cu_count);
+  const okq::MoePlan plan = okq::moe_plan(a);
   void *ws = nullptr;
-  st = get_workspace(dev, s, plan.workspace, &ws, 7, what);
+  st = workspace_status(grow_workspace(dev, s, plan.workspace, plan.reserve, &ws, 7), plan.workspace, what);
   if (st != OKQ_OK) return st;
   return hip_status(okq::launch_moe(a, plan, ws, info.cu_count, s), "moe_mlp launch");
 }

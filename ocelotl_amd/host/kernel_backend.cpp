@@ -593,6 +593,71 @@ Result<void> HipKernelBackend::logits_process_d(const DeviceTensor &logits, size
                                   (int64_t)vocab, best, stream_));
 }
 
+Result<void> HipKernelBackend::residual_norm_d(const DeviceTensor &x, const DeviceTensor &branch, size_t rows,
+                                               size_t hidden, const DeviceTensor *post_norm, const DeviceTensor *gate,
+                                               float branch_scale, float residual_scale, const DeviceTensor *pre_norm,
+                                               float epsilon, const DeviceTensor *sum,
+                                               const DeviceTensor *normed) const {
+  const char *call = "residual_norm";
+  const bool one_gate = gate && gate->len() == hidden;
+  Result<void> r = tensor_len(call, "x", x, rows * hidden);
+  if (!r.is_err()) r = tensor_len(call, "branch", branch, rows * hidden);
+  if (!r.is_err() && post_norm) r = tensor_len(call, "post_norm", *post_norm, hidden);
+  if (!r.is_err() && gate && !one_gate) r = tensor_len(call, "gate", *gate, rows * hidden);
+  if (!r.is_err() && pre_norm) r = tensor_len(call, "pre_norm", *pre_norm, hidden);
+  if (!r.is_err() && sum) r = tensor_len(call, "sum", *sum, rows * hidden);
+  if (!r.is_err() && normed) r = tensor_len(call, "normed", *normed, rows * hidden);
+  if (r.is_err()) return r;
+  const int64_t h = (int64_t)hidden;
+  return check(okq_residual_norm(x.device_ptr(), h, branch.device_ptr(), h, (int64_t)rows, h, ptr_or_null(post_norm),
+                                 ptr_or_null(gate), one_gate ? 0 : h, branch_scale, residual_scale,
+                                 ptr_or_null(pre_norm), epsilon, sum ? sum->device_ptr() : nullptr, h,
+                                 normed ? normed->device_ptr() : nullptr, OKQ_TYPE_F32, h, stream_));
+}
+
+Result<void> HipKernelBackend::moe_route_d(const DeviceTensor &x, size_t rows, size_t hidden,
+                                           const DeviceTensor &weight, size_t experts, const RouteOptions &o,
+                                           int32_t *ids, const DeviceTensor &weights,
+                                           const DeviceTensor *logits) const {
+  const char *call = "moe_route";
+  Result<void> r = tensor_len(call, "x", x, rows * hidden);
+  if (!r.is_err()) r = tensor_len(call, "weight", weight, experts * hidden);
+  for (const DeviceTensor *t : {o.bias, o.choice_bias})
+    if (!r.is_err() && t) r = tensor_len(call, "bias", *t, experts);
+  if (!r.is_err()) r = tensor_len(call, "weights", weights, rows * o.top_k);
+  if (!r.is_err() && logits) r = tensor_len(call, "logits", *logits, rows * experts);
+  if (r.is_err()) return r;
+  return check(okq_moe_route(x.device_ptr(), (int64_t)hidden, (int64_t)rows, (int64_t)hidden, OKQ_TYPE_F32,
+                             weight.device_ptr(), (int64_t)experts, ptr_or_null(o.bias), o.score,
+                             ptr_or_null(o.choice_bias), (int64_t)o.groups, (int64_t)o.top_groups,
+                             (int64_t)o.group_best, (int64_t)o.top_k, o.renormalise ? 1 : 0, o.scale, ids,
+                             weights.device_ptr(), logits ? logits->device_ptr() : nullptr, stream_));
+}
+
+Result<void> HipKernelBackend::moe_mlp_d(const DeviceTensor &x, size_t rows, size_t hidden, size_t intermediate,
+                                         size_t experts, size_t top_k, const int32_t *ids, const DeviceTensor &weights,
+                                         const QuantizedWeight &gate, const QuantizedWeight &up,
+                                         const QuantizedWeight &down, const DeviceTensor &out) const {
+  const char *call = "moe_mlp";
+  Result<void> r = tensor_len(call, "x", x, rows * hidden);
+  if (!r.is_err()) r = tensor_len(call, "weights", weights, rows * top_k);
+  if (!r.is_err()) r = tensor_len(call, "out", out, rows * hidden);
+  if (r.is_err()) return r;
+  if (gate.tensor_type() != up.tensor_type()) return kernel_err("moe_mlp gate and up must be of one type");
+  for (const QuantizedWeight *w : {&gate, &up, &down}) {
+    const bool d = w == &down;
+    if (w->ne0() != (d ? intermediate : hidden) || w->ne1() != experts * (d ? hidden : intermediate))
+      return kernel_err(std::string("moe_mlp ") + (d ? "down" : "gate or up") + " weight shape does not match");
+    if (!w->device_ptr()) return kernel_err("moe_mlp weights must be on the device");
+  }
+  const uint32_t types[2] = {(uint32_t)gate.tensor_type(), (uint32_t)down.tensor_type()};
+  return check(okq_moe_mlp_q(x.device_ptr(), (int64_t)hidden, (int64_t)rows, (int64_t)hidden, (int64_t)intermediate,
+                             (int64_t)experts, (int64_t)top_k, ids, weights.device_ptr(), types[0], gate.device_ptr(),
+                             gate.byte_len(), up.device_ptr(), up.byte_len(), types[1], down.device_ptr(),
+                             down.byte_len(), out.device_ptr(), (int64_t)hidden, stream_),
+               types[0]);
+}
+
 Result<DeviceTensor> HipKernelBackend::embedding_rows(const QuantizedWeight &table, const uint32_t *ids,
                                                       size_t n) const {
   auto a = device_alloc(n * table.ne0() * sizeof(float));

@@ -280,6 +280,15 @@ class KernelBackend {
                                 size_t out_features, const DeviceTensor *bias, const DeviceTensor &out) const;
 };
 
+// How moe_route_d chooses, as okq_moe_route documents it (null: none).
+struct RouteOptions {
+  int score = 0;  // OKQ_SCORE_SOFTMAX or OKQ_SCORE_SIGMOID
+  const DeviceTensor *bias = nullptr, *choice_bias = nullptr;  // [experts]
+  size_t groups = 1, top_groups = 1, group_best = 1, top_k = 1;
+  bool renormalise = true;
+  float scale = 1.0f;
+};
+
 // The parts of logits_process_d that a call has (null or zero: none); device
 // pointers, as okq_logits_process documents them.
 struct LogitsOptions {
@@ -367,6 +376,27 @@ class HipKernelBackend final : public KernelBackend {
   // Penalties, biases and grammar mask, and the greedy token (best may be null).
   Result<void> logits_process_d(const DeviceTensor &logits, size_t rows, size_t vocab, const LogitsOptions &options,
                                 const DeviceTensor &out, int32_t *best) const;
+  // The step between two blocks and a sparse layer's experts (okq.h:
+  // okq_residual_norm, okq_moe_route, okq_moe_mlp_q) on device tensors of
+  // contiguous rows; integer arrays are device pointers.  No counterparts in
+  // the trait.
+  // sum = residual_scale * x + branch_scale * gate * post_norm(branch), and its
+  // norm; post_norm and gate (one row for all, or a row each) may be null, so
+  // may pre_norm and normed together, or sum (which may be x or branch).
+  Result<void> residual_norm_d(const DeviceTensor &x, const DeviceTensor &branch, size_t rows, size_t hidden,
+                               const DeviceTensor *post_norm, const DeviceTensor *gate, float branch_scale,
+                               float residual_scale, const DeviceTensor *pre_norm, float epsilon,
+                               const DeviceTensor *sum, const DeviceTensor *normed) const;
+  // Every row's experts (ids [rows, top_k]) and their weights; logits may be null.
+  Result<void> moe_route_d(const DeviceTensor &x, size_t rows, size_t hidden, const DeviceTensor &weight,
+                           size_t experts, const RouteOptions &options, int32_t *ids, const DeviceTensor &weights,
+                           const DeviceTensor *logits) const;
+  // The experts' gated MLP.  gate and up are stacked tensors [ne0 = hidden,
+  // ne1 = intermediate * experts] of one type, down is [intermediate, hidden *
+  // experts].
+  Result<void> moe_mlp_d(const DeviceTensor &x, size_t rows, size_t hidden, size_t intermediate, size_t experts,
+                         size_t top_k, const int32_t *ids, const DeviceTensor &weights, const QuantizedWeight &gate,
+                         const QuantizedWeight &up, const QuantizedWeight &down, const DeviceTensor &out) const;
   // Waits for the backend's stream.
   Result<void> synchronize() const;
 

@@ -64,6 +64,7 @@ NORM = [
 ROUTE = [
     (dict(wtype=Q8_0), okq.E_TYPE, "supported: F32, F16, BF16"),
     (dict(rows=-1), okq.E_SHAPE, "rows=-1"),
+    (dict(rows=(1 << 26) + 1), okq.E_SHAPE, "at most 2^26"),
     (dict(hidden=0), okq.E_SHAPE, "hidden=0"),
     (dict(experts=0), okq.E_SHAPE, "experts=0"),
     (dict(experts=513, groups=1, top=1), okq.E_SHAPE, "1 to 512"),
@@ -91,6 +92,7 @@ ROUTE = [
 MOE = [
     (dict(rows=-1), okq.E_SHAPE, "rows=-1"),
     (dict(experts=0), okq.E_SHAPE, "experts=0"),
+    (dict(experts=4097), okq.E_SHAPE, "1 to 4096"),
     (dict(k=0), okq.E_SHAPE, "top_k=0"),
     (dict(k=65), okq.E_SHAPE, "top_k=65"),
     (dict(gutype=F32), okq.E_TYPE, "Q8_0, Q4K, Q5K, Q6K"),
@@ -104,6 +106,7 @@ MOE = [
     (dict(ubytes=GU + 144), okq.E_SHAPE, "up bytes"),
     (dict(dbytes=0), okq.E_SHAPE, "down bytes"),
     (dict(hidden=1 << 20, inner=1 << 20, xs=1 << 20, outs=1 << 20), okq.E_SHAPE, "4 GiB"),
+    (dict(inner=1 << 24), okq.E_SHAPE, "above 2^23"),
     (dict(x=None), okq.E_ARG, "x is null"),
     (dict(ids=None), okq.E_ARG, "ids is null"),
     (dict(weights=None), okq.E_ARG, "weights is null"),

@@ -615,3 +615,37 @@ def test_two_streams_at_once(torch, okq):
     torch.cuda.synchronize()
     for j, a in zip(jobs, alone):
         assert torch.equal(j[5], a)
+
+
+def test_a_larger_call_makes_room_for_a_smaller_captured_one(torch, okq):
+    """Whatever kernels the two take: on a fresh stream, a call of many rows, then captures of fewer."""
+    e, router, norms, x, attn, out, scratch = _layer_inputs(torch, okq, 5000, hidden=4096, inner=256, experts=8, k=2)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _layer(torch, okq, e, router, norms, x, attn, out, scratch, s.cuda_stream)
+        s.synchronize()
+        for rows in (1, 17, 100, 600):
+            part = [x[:rows], attn[:rows], out[:rows], tuple(t[:rows] for t in scratch)]
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                _layer(torch, okq, e, router, norms, *part, torch.cuda.current_stream().cuda_stream)
+            graph.replay()
+            s.synchronize()
+            again, more = torch.empty_like(part[2]), tuple(torch.empty_like(t) for t in part[3])
+            _layer(torch, okq, e, router, norms, part[0], part[1], again, more, s.cuda_stream)
+            s.synchronize()
+            assert torch.equal(out[:rows], again)
+
+
+def test_moe_in_several_passes(torch, okq):
+    """More pairs than a pass takes, streamed and sorted: rows of a first and of a last pass, and of a batch of their own."""
+    for rows, experts, k in ((9000, 8, 8), (1100, 4000, 64)):  # 72000 pairs; 70400 pairs of many experts
+        hidden, inner = 64, 32
+        e = Experts(torch, okq, experts, hidden, inner, Q8_0, Q8_0)
+        x = torch.randn(rows, hidden, generator=_gen(torch, 3), device="cuda")
+        ids = torch.randint(-1, experts, (rows, k), generator=_gen(torch, 4), device="cuda").int()
+        weights = torch.rand(rows, k, generator=_gen(torch, 5), device="cuda") / k
+        got = e(torch, okq, x, ids, weights)
+        for at in (0, rows // 2, rows - 24):
+            part = slice(at, at + 24)
+            _within(got[part], *e.want(torch, x[part], ids[part], weights[part]), "out")
