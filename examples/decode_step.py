@@ -2,7 +2,7 @@
 cache, attention over its pages, the gated MLP, the output head and the choice
 of a token, for a batch of sequences of different lengths.
 
-    python examples/decode_step.py [--layers 2] [--seqs 8] [--steps 32] [--cache BF16]
+    python examples/decode_step.py [--layers 2] [--seqs 8] [--steps 32] [--cache BF16] [--experts 0]
 
 Random weights (Q4_K, N(0, 1 / in_features)) at the attention block's sizes of
 Llama-3-8B; prompts enter the cache one token a step beside sequences that are
@@ -43,6 +43,9 @@ class Config:
     max_tokens: int = 512  # of a sequence
     rope_base: float = 500000.0
     eps: float = 1e-5
+    experts: int = 0  # above 0: sparse layers, each token through top_k of so many gated MLPs
+    top_k: int = 8
+    expert_intermediate: int = 768
 
 
 @dataclass
@@ -68,14 +71,17 @@ class Layer:
         qw, kw = c.q_heads * c.head_dim, c.kv_heads * c.head_dim
         self.wq, self.wk, self.wv = (Weight(n, c.hidden, seed + i) for i, n in enumerate((qw, kw, kw)))
         self.wo = Weight(c.hidden, qw, seed + 3)
-        self.gate, self.up = (Weight(c.intermediate, c.hidden, seed + 4 + i) for i in range(2))
-        self.down = Weight(c.hidden, c.intermediate, seed + 6)
+        n, inner = (c.experts, c.expert_intermediate) if c.experts else (1, c.intermediate)
+        self.gate, self.up = (Weight(n * inner, c.hidden, seed + 4 + i) for i in range(2))
+        self.down = Weight(n * c.hidden, inner, seed + 6)
         g = torch.Generator(device="cuda")
         g.manual_seed(seed)
 
         def norm(n):
             return 1 + 0.1 * torch.randn(n, generator=g, device="cuda")
         self.attn_norm, self.mlp_norm = norm(c.hidden), norm(c.hidden)
+        if c.experts:
+            self.router = torch.randn(c.experts, c.hidden, generator=g, device="cuda") * c.hidden ** -0.5
         self.q_norm, self.k_norm = (norm(c.head_dim), norm(c.head_dim)) if c.qk_norm else (None, None)
         row = c.head_dim // 32 * 34 if c.cache == "Q8_0" else c.head_dim * (4 if c.cache == "F32" else 2)
         page = c.kv_heads * c.page_tokens * row
@@ -112,6 +118,9 @@ class Model:
         self.x, self.q, self.k, self.v, self.attn = (buf(n) for n in (c.hidden, qw, kw, kw, qw))
         self.y, self.normed, self.g, self.u = (buf(n) for n in (c.hidden, c.hidden, c.intermediate, c.intermediate))
         self.logits = buf(c.vocab)
+        if c.experts:
+            self.ids = torch.empty(seqs, c.top_k, dtype=torch.int32, device="cuda")
+            self.shares = buf(c.top_k)
 
     def step(self, ids, positions) -> None:
         """One token of every sequence: ids and positions (host lists); leaves the head's logits in self.logits."""
@@ -128,6 +137,10 @@ class Model:
             self.rotate(l, pos, slot, s)
             self.attend(l, lengths, max(positions) + 1, s)
             self._linear(self.attn, l.wo, self.y, s)
+            if c.experts:
+                self.mix(l, s)
+                self.x += self.y
+                continue
             self.x += self.y
             okq.call("okq_rmsnorm", self.x.data_ptr(), n, c.hidden, l.mlp_norm.data_ptr(), c.eps,
                      self.normed.data_ptr(), s)
@@ -155,6 +168,18 @@ class Model:
         okq.call("okq_paged_attention", self.q.data_ptr(), qw, self.seqs, c.q_heads, ctypes.byref(l.pages),
                  self.table.data_ptr(), self.table.shape[1], lengths.data_ptr(), longest, c.head_dim ** -0.5, 0.0, 0,
                  self.attn.data_ptr(), qw, None, s)
+
+    def mix(self, l: Layer, s: int) -> None:
+        """Attention's residual sum with the norm behind it, every token's experts, and their results in self.y."""
+        c, n = self.c, self.seqs
+        okq.call("okq_residual_norm", self.x.data_ptr(), c.hidden, self.y.data_ptr(), c.hidden, n, c.hidden, None, None, 0,
+                 1.0, 1.0, l.mlp_norm.data_ptr(), c.eps, self.x.data_ptr(), c.hidden, self.normed.data_ptr(), 0, c.hidden, s)
+        okq.call("okq_moe_route", self.normed.data_ptr(), c.hidden, n, c.hidden, 0, l.router.data_ptr(), c.experts, None, 0,
+                 None, 1, 1, 1, c.top_k, 1, 1.0, self.ids.data_ptr(), self.shares.data_ptr(), None, s)
+        okq.call("okq_moe_mlp_q", self.normed.data_ptr(), c.hidden, n, c.hidden, c.expert_intermediate, c.experts, c.top_k,
+                 self.ids.data_ptr(), self.shares.data_ptr(), Q4_K, l.gate.data.data_ptr(), l.gate.data.numel(),
+                 l.up.data.data_ptr(), l.up.data.numel(), Q4_K, l.down.data.data_ptr(), l.down.data.numel(),
+                 self.y.data_ptr(), c.hidden, s)
 
     def choose(self, hist, seen, start, rep, pres, best, s: int) -> None:
         """Penalties on self.logits, in place, and every sequence's token."""
@@ -213,8 +238,9 @@ def main() -> None:
     ap.add_argument("--seqs", type=int, default=8)
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--cache", choices=sorted(CACHE_TYPES), default="BF16")
+    ap.add_argument("--experts", type=int, default=0)
     a = ap.parse_args()
-    model = Model(Config(layers=a.layers, cache=a.cache), a.seqs)
+    model = Model(Config(layers=a.layers, cache=a.cache, experts=a.experts, top_k=min(8, a.experts)), a.seqs)
     prompts = [[(7 * i + j) % model.c.vocab for j in range(1 + 3 * i)] for i in range(a.seqs)]
     model.generate(prompts, 2)
     got = model.generate(prompts, a.steps)
