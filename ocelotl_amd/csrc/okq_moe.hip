@@ -23,6 +23,7 @@ namespace okq {
 namespace {
 
 constexpr int kWaves = 8;
+constexpr int kPassPairs = 65536;  // at most, of a pass: they count in 16 bits
 constexpr int kFewPairs = 64;    // not sorted: a lane each
 constexpr int kBatch = 4;         // column tiles whose waves meet in LDS together
 
@@ -384,6 +385,14 @@ struct MoeProduct {
 // columns, unused experts left CUs idle and one of 17 rows took twice the time
 // of the others: 96 rows of 8 of 256 experts, gate and up 169 -> 87 us.
 //
+// What bounds it: for many experts memory (48 rows of 8 of 128, 2048 x 768 in
+// Q4_K: gate and up 47 us, down 33, for 208 and 104 MB: 4.4 and 3.2 TB/s with
+// 9 us of launch, sort, rows and their planes ahead of the stream; 13 rows of 2
+// of 8, 4096 x 14336: 528 MB in 121 us, Q6_K down 385 MB in 112); for one row
+// the chain ids, rows, weights, join: 10.7 and 8.0 us.  A tile costs a wave
+// some 170 VALU instructions an item, which with 8 waves a CU take 40-50% of
+// the cycles.
+//
 // A few pairs (kFewPairs at most) whose experts mostly differ are not sorted (a
 // launch of 5 us): every workgroup has a pair's expert and lists its pairs by
 // itself, going on if no earlier pair has the same, `rounds` steps and as many
@@ -564,6 +573,7 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
   constexpr int kPer = kMoeMaxExperts / 1024, kHeld = 16;
   __shared__ int next[kMoeMaxExperts];
   __shared__ int2 waves[16];
+  __shared__ uint16_t sorted[kPassPairs];  // stored in order: scattered from one CU, 32768 words took 8 us more
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int e = tid; e < kMoeMaxExperts; e += 1024) next[e] = 0;
   __syncthreads();
@@ -618,11 +628,12 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
     }
     r += m[i];
   }
+  __syncthreads();  // (the waves' sums are read)
   if (tid == 1023) {
     count[0] = t;
     count[1] = r;
+    waves[0].x = r;
   }
-  __syncthreads();
   for (int p0 = 0; p0 <= last; p0 += 1024 * kHeld) {
     if (p0) get(p0);
     int at[kHeld];
@@ -632,9 +643,13 @@ __global__ __launch_bounds__(1024) void moe_sort_kernel(const int32_t *__restric
     for (int i = 0; i < kHeld; ++i) {
       const int p = p0 + 1024 * i + tid;
       if (p < pairs) place[p] = at[i];
-      if (at[i] >= 0) order[at[i]] = p;
+      if (at[i] >= 0) sorted[at[i]] = (uint16_t)p;
     }
   }
+  __syncthreads();
+  const int n = waves[0].x;  // pairs with an expert
+#pragma unroll 4
+  for (int i = tid; i < n; i += 1024) order[i] = sorted[i];
 }
 
 // Rows of K values as two fp16 planes of rows of Kp (zeros behind K), their
@@ -764,7 +779,7 @@ static MoePlan plan_of(const MoeArgs &a, bool tiled) {
   // a pass keeps to about 1 GiB of results, and to what its kernels count in
   // 32 bits
   const int64_t one = 4 * ((int64_t)a.inner * (gs > 1 ? 1 + 2 * gs : 2) + (int64_t)a.hidden * ds);
-  const int64_t most = std::min<int64_t>({65536, (1 << 30) / one, (UINT32_MAX - (1 << 20)) / (2 * (int64_t)whole(std::max(a.inner, a.hidden)))});
+  const int64_t most = std::min<int64_t>({kPassPairs, (1 << 30) / one, (UINT32_MAX - (1 << 20)) / (2 * (int64_t)whole(std::max(a.inner, a.hidden)))});
   p.pass_rows = std::max<int64_t>(1, std::min<int64_t>(a.rows, most / a.top_k));
   const size_t pairs = (size_t)p.pass_rows * a.top_k;
   p.off_inner = 0;

@@ -68,7 +68,11 @@ __device__ __forceinline__ void get(const float *p, float *v) {
 
 // A row stays in its workgroup's registers from the first load to the last
 // store, V groups of N values a thread, and everything it needs is requested
-// at once: one wait for memory, two joins in LDS.
+// at once: one wait for memory, two joins in LDS.  Bounded by memory for many
+// rows (4096 x 4096: 268 MB in 51 us called with new rows each time, 5.2 TB/s,
+// the rate of a large copy; 39 us on the same ones), by that wait for few
+// (1 x 4096: 2.9 us, 48 x 2560: 3.9).  Where rows are not 16-byte aligned a
+// value a load: 1531 x 1111, gated, 8.3 us, 3.7 TB/s.
 template <int N, int V>
 __global__ __launch_bounds__(1024) void residual_norm_kernel(ResidualArgs a) {
   __shared__ float red[2][16];
