@@ -431,7 +431,7 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
  * ids, weights [rows, top_k]; an id outside [0, experts) adds nothing whatever
  * its weight is, so a row of such ids gets zeros; the same id twice in a row
  * adds twice.  experts at most 4096, top_k at most 64.  Each expert's weights are read once for up
- * to 16 of its rows.  Activations keep 22 bits, sums are f32; a row's result
+ * to 16 of its rows, 128 where it has many.  Activations keep 22 bits, sums are f32; a row's result
  * does not depend on the rows around it beyond the choice of a kernel by the
  * call's sizes, nor on timing.  A row of x that holds an infinity or a NaN, or
  * whose gated values do, gets NaN throughout (where it has an expert).  rows

@@ -649,3 +649,44 @@ def test_moe_in_several_passes(torch, okq):
         for at in (0, rows // 2, rows - 24):
             part = slice(at, at + 24)
             _within(got[part], *e.want(torch, x[part], ids[part], weights[part]), "out")
+
+
+@pytest.mark.parametrize("rows", [3, 56000])
+def test_moe_stacks_beyond_4_gib(torch, okq, rows):
+    """The last two of 2000 experts, 4.7 GB into their stacks; what the others hold is not read."""
+    experts, hidden, inner = 2000, 2048, 2048
+    e = Experts(torch, okq, 2, hidden, inner, Q4_K, Q4_K)
+    x = torch.randn(rows, hidden, generator=_gen(torch, 1), device="cuda")
+    ids, weights = _pairs(torch, rows, 2, 1, 3)
+    want, far = e.want(torch, x, ids, weights)
+    for name in ("gate", "up", "down"):
+        stack = torch.full((experts // 2, getattr(e, name).numel()), 0xFF, dtype=torch.uint8, device="cuda")
+        stack[-1] = getattr(e, name)
+        setattr(e, name, stack.view(-1))
+    assert e.gate.numel() > 1 << 32
+    e.experts = experts
+    _within(e(torch, okq, x, ids + experts - 2, weights), want, far, "out")
+
+
+def test_two_host_threads_on_one_stream(torch, okq):
+    """Each call's launches go in as one sequence, so the stream's workspaces serve one call at a time."""
+    import threading
+    jobs = [_layer_inputs(torch, okq, 60, seed=s) for s in (2, 3)]
+    alone, stream = [], torch.cuda.Stream()
+    for e, router, norms, x, attn, out, scratch in jobs:
+        _layer(torch, okq, e, router, norms, x, attn, out, scratch, stream.cuda_stream)
+        torch.cuda.synchronize()
+        alone.append(out.clone())
+
+    def work(job):
+        e, router, norms, x, attn, out, scratch = job
+        for _ in range(20):
+            _layer(torch, okq, e, router, norms, x, attn, out, scratch, stream.cuda_stream)
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for j, a in zip(jobs, alone):
+        assert torch.equal(j[5], a)
