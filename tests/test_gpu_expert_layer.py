@@ -690,3 +690,47 @@ def test_two_host_threads_on_one_stream(torch, okq):
     torch.cuda.synchronize()
     for j, a in zip(jobs, alone):
         assert torch.equal(j[5], a)
+
+
+@pytest.mark.parametrize("case", [
+    (1, 4096, 2560, 8, 2, Q6_K, Q4_K),      # one row, its items in two slices each way
+    (2, 2304, 4608, 16, 2, Q5_K, Q6_K),     # nine items in slices of five and four, eighteen in three of six
+    (1, 288, 8480, 5, 3, Q8_0, Q8_0),       # 33 and a half items: slices of seven and six, the last one cut
+    (4, 1280, 768, 128, 8, Q4_K, Q5_K),     # rows that share some experts, unsorted
+    (64, 2560, 256, 3, 1, Q5_K, Q4_K),      # more than 16 rows an expert
+    (130, 4352, 1280, 2, 2, Q8_0, Q6_K),    # tiles of 128 and of 2 rows
+], ids=str)
+def test_moe_of_long_rows(torch, okq, case):
+    rows, hidden, inner, experts, k, gu, dn = case
+    e = Experts(torch, okq, experts, hidden, inner, gu, dn)
+    x = torch.randn(rows, hidden, generator=_gen(torch, rows), device="cuda")
+    ids, weights = _pairs(torch, rows, experts, k, 11)
+    _within(e(torch, okq, x, ids, weights), *e.want(torch, x, ids, weights), "out")
+
+
+def test_moe_rows_do_not_depend_on_each_other(torch, okq):
+    """Alone (not sorted), in a batch (sorted), in another one: the same bits; so in batches of tiles."""
+    e = Experts(torch, okq, 6, 512, 768, Q4_K, Q6_K)
+    x = torch.randn(900, 512, generator=_gen(torch, 2), device="cuda")
+    ids, weights = _pairs(torch, 900, 6, 2, 6)
+    some = e(torch, okq, x[:70], ids[:70], weights[:70])
+    assert torch.equal(e(torch, okq, x[20:60], ids[20:60], weights[20:60]), some[20:60])
+    for r in (0, 33, 69):
+        assert torch.equal(e(torch, okq, x[r:r + 1], ids[r:r + 1], weights[r:r + 1])[0], some[r])
+    many = e(torch, okq, x, ids, weights)
+    assert torch.equal(e(torch, okq, x[100:500], ids[100:500], weights[100:500]), many[100:500])
+
+
+@pytest.mark.parametrize("rows", [2, 50, 400])
+def test_moe_rows_without_experts_may_hold_anything(torch, okq, rows):
+    e = Experts(torch, okq, 4, 256, 256, Q8_0, Q5_K)
+    x = torch.randn(rows, 256, generator=_gen(torch, 2), device="cuda")
+    ids, weights = _pairs(torch, rows, 4, 2, 6)
+    clean = e(torch, okq, x, ids, weights)
+    x[1] = math.nan
+    x[rows - 1, 3] = math.inf
+    weights[[1, rows - 1]] = math.inf
+    ids[[1, rows - 1]] = -7
+    got = e(torch, okq, x, ids, weights)
+    assert not bool(got[1].any()) and not bool(got[rows - 1].any())
+    assert torch.equal(got[2:rows - 1], clean[2:rows - 1]) and torch.equal(got[0], clean[0])
