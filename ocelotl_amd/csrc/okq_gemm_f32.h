@@ -323,6 +323,14 @@ __device__ __forceinline__ void f32_body(const _Float16 *__restrict__ xhi, const
       const auto d = __builtin_amdgcn_permlane32_swap(dd, dd, false, false);
       cur.d01 = d[0];
       cur.d23 = d[1];
+      if constexpr (kExperts != 0) {
+        // blocks behind the row's last one are the next row's, the next
+        // expert's or nothing: a d of zero, since any other that is no number
+        // would make NaN of the zeros it meets
+        const int left = em.row_bytes / (int)kQ8Bytes - 4 * st;
+        cur.d01 &= left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        cur.d23 &= left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
+      }
     }
   };
 

@@ -74,7 +74,7 @@ struct ExpQ4K {
     c.dmin = f16_bits_hw(hd.x >> 16);
     return c;
   }
-  __device__ static Cur begin(const Item &it, int g) { return header(it.hd, g); }
+  __device__ static Cur begin(const Item &it, int g, int) { return header(it.hd, g); }
   __device__ static void frag(const Item &it, const Cur &c, int t, int, h8 &b1, h8 &) {
     const int nib = t & 1, p8 = t >> 1;
     const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0;
@@ -103,7 +103,7 @@ struct ExpQ5K {
     it.q0 = bload4(rs, blk + 48u + 32u * (uint32_t)g);
     it.q1 = bload4(rs, blk + 64u + 32u * (uint32_t)g);
   }
-  __device__ static Cur begin(const Item &it, int g) { return ExpQ4K::header(it.hd, g); }
+  __device__ static Cur begin(const Item &it, int g, int) { return ExpQ4K::header(it.hd, g); }
   __device__ static void frag(const Item &it, const Cur &c, int t, int g, h8 &b1, h8 &) {
     const int nib = t & 1, p8 = t >> 1;
     const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0, hc = (p8 >> 1) ? it.h1 : it.h0;
@@ -153,7 +153,7 @@ struct ExpQ6K {
     it.sc1 = __builtin_amdgcn_raw_buffer_load_b32(rs, a + 208u, 0, 0);
     it.r = r;
   }
-  __device__ static Cur begin(const Item &it, int) {
+  __device__ static Cur begin(const Item &it, int, int) {
     Cur c;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -191,7 +191,9 @@ struct ExpQ6K {
 
 // Eight blocks of 34 bytes, 2 g and 2 g + 1 the lane group's.  d goes into the
 // two exact planes of d * q.  A row of K not a multiple of 256 ends inside an
-// item: what follows it (the next row's blocks, or nothing) meets zeros.
+// item: what follows it (the next row's blocks, or nothing) gets a d of zero and
+// meets zeros (both: a scale that is no number, or a product past fp16, times
+// zero would be NaN).
 struct ExpQ80 {
   static constexpr int kType = kQ8_0;
   static constexpr bool kMins = false, kLow = true;
@@ -215,14 +217,14 @@ struct ExpQ80 {
     it.w4 = __builtin_amdgcn_raw_buffer_load_b64(rs, a + 64u, 0, 0);
     it.r = r;
   }
-  __device__ static Cur begin(const Item &it, int) {
+  __device__ static Cur begin(const Item &it, int g, int left) {
     const uint32_t raw[18] = {it.w0.x, it.w0.y, it.w0.z, it.w0.w, it.w1.x, it.w1.y, it.w1.z, it.w1.w, it.w2.x,
                               it.w2.y, it.w2.z, it.w2.w, it.w3.x, it.w3.y, it.w3.z, it.w3.w, it.w4.x, it.w4.y};
     Cur c;
 #pragma unroll
     for (int i = 0; i < 17; ++i) c.w[i] = realign(raw[i + 1], raw[i], it.r);
-    const _Float16 d0 = __builtin_bit_cast(_Float16, (uint16_t)(c.w[0] & 0xffffu));
-    const _Float16 d1 = __builtin_bit_cast(_Float16, (uint16_t)(c.w[8] >> 16));
+    const uint32_t e0 = 64 * g < left ? c.w[0] & 0xffffu : 0u, e1 = 64 * g + 32 < left ? c.w[8] >> 16 : 0u;
+    const _Float16 d0 = __builtin_bit_cast(_Float16, (uint16_t)e0), d1 = __builtin_bit_cast(_Float16, (uint16_t)e1);
     c.d0 = h2{d0, d0};
     c.d1 = h2{d1, d1};
     c.d = 1.0f;
@@ -326,11 +328,12 @@ __device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
 }
 
 // acc (rows 4 g .. 4 g + 3 of the lane's column) += the item's products; rs:
-// the rows' scales.
+// the rows' scales; left: the values of the row from the item on.
 template <class F>
-__device__ __forceinline__ void contract(f4 &acc, const typename F::Item &it, const ActA &A, const f4 &rs, int g) {
+__device__ __forceinline__ void contract(f4 &acc, const typename F::Item &it, const ActA &A, const f4 &rs, int g,
+                                         int left) {
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  const typename F::Cur c = F::begin(it, g);
+  const typename F::Cur c = F::begin(it, g, left);
   f4 s = zero, low = zero;  // two chains: a product waits for the one before it in its own
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
@@ -499,7 +502,7 @@ __global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
 #pragma unroll
         for (int k = 0; k < NM; ++k) {
           f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-          contract<F>(acc, S[d][k], A, scales, g);
+          contract<F>(acc, S[d][k], A, scales, g, a.K - 256 * item);
           red[parity][i % kBatch][wave][k][l] = acc;
         }
         // into the registers that this tile's weights have left (issued any

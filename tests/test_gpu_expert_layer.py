@@ -734,3 +734,30 @@ def test_moe_rows_without_experts_may_hold_anything(torch, okq, rows):
     got = e(torch, okq, x, ids, weights)
     assert not bool(got[1].any()) and not bool(got[rows - 1].any())
     assert torch.equal(got[2:rows - 1], clean[2:rows - 1]) and torch.equal(got[0], clean[0])
+
+
+@pytest.mark.parametrize("behind", [0x7E00, 0xFC00, 0x7BFF], ids=["nan", "infinity", "largest"])
+@pytest.mark.parametrize("rows", [1, 20, 400])
+def test_moe_rows_of_q8_end_at_their_own_blocks(torch, okq, rows, behind):
+    """Rows that are no multiple of 256 values: whatever the blocks behind them hold, the next expert's and the next
+    row's, changes no bit."""
+    for hidden, inner in ((288, 352), (32, 96), (1312, 2592)):
+        e = Experts(torch, okq, 5, hidden, inner, Q8_0, Q8_0)
+        x = torch.randn(rows, hidden, generator=_gen(torch, rows), device="cuda")
+        ids, weights = _pairs(torch, rows, 3, 2, 8)
+        ids *= 2  # experts 1 and 3 have no rows
+        clean = e(torch, okq, x, ids, weights)
+        _within(clean, *e.want(torch, x, ids, weights), "out")
+        block = torch.tensor([behind & 255, behind >> 8] + [127] * 32, dtype=torch.uint8, device="cuda")
+        for name in ("gate", "up", "down"):
+            getattr(e, name).view(5, -1, 34)[1::2] = block
+        assert torch.equal(e(torch, okq, x, ids, weights), clean)
+        at = hidden // 2  # one output of expert 2 whose own weights are such blocks
+        e.down.view(5, hidden, -1, 34)[2, at] = block
+        got = e(torch, okq, x, ids, weights)
+        keep = torch.arange(hidden, device="cuda") != at
+        assert torch.equal(got[:, keep], clean[:, keep])
+        used = (ids == 2).any(1)
+        assert torch.equal(got[~used], clean[~used])
+        if behind != 0x7BFF:
+            assert not bool(torch.isfinite(got[used, at]).any())
