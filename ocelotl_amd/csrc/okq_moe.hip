@@ -74,7 +74,7 @@ struct ExpQ4K {
     c.dmin = f16_bits_hw(hd.x >> 16);
     return c;
   }
-  __device__ static Cur begin(const Item &it, int g, int) { return header(it.hd, g); }
+  __device__ static Cur begin(const Item &it, int g, int, int) { return header(it.hd, g); }
   __device__ static void frag(const Item &it, const Cur &c, int t, int, h8 &b1, h8 &) {
     const int nib = t & 1, p8 = t >> 1;
     const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0;
@@ -103,7 +103,7 @@ struct ExpQ5K {
     it.q0 = bload4(rs, blk + 48u + 32u * (uint32_t)g);
     it.q1 = bload4(rs, blk + 64u + 32u * (uint32_t)g);
   }
-  __device__ static Cur begin(const Item &it, int g, int) { return ExpQ4K::header(it.hd, g); }
+  __device__ static Cur begin(const Item &it, int g, int, int) { return ExpQ4K::header(it.hd, g); }
   __device__ static void frag(const Item &it, const Cur &c, int t, int g, h8 &b1, h8 &) {
     const int nib = t & 1, p8 = t >> 1;
     const u32x4 pc = (p8 >> 1) ? it.q1 : it.q0, hc = (p8 >> 1) ? it.h1 : it.h0;
@@ -153,7 +153,7 @@ struct ExpQ6K {
     it.sc1 = __builtin_amdgcn_raw_buffer_load_b32(rs, a + 208u, 0, 0);
     it.r = r;
   }
-  __device__ static Cur begin(const Item &it, int, int) {
+  __device__ static Cur begin(const Item &it, int, int, int) {
     Cur c;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -190,7 +190,8 @@ struct ExpQ6K {
 };
 
 // Eight blocks of 34 bytes, 2 g and 2 g + 1 the lane group's.  d goes into the
-// two exact planes of d * q.  A row of K not a multiple of 256 ends inside an
+// two exact planes of d * q; where that could pass fp16 (|d| >= 256, which no
+// weights of ordinary size have), a tile's item goes in two parts.  A row of K not a multiple of 256 ends inside an
 // item: what follows it (the next row's blocks, or nothing) gets a d of zero and
 // meets zeros (both: a scale that is no number, or a product past fp16, times
 // zero would be NaN).
@@ -217,17 +218,42 @@ struct ExpQ80 {
     it.w4 = __builtin_amdgcn_raw_buffer_load_b64(rs, a + 64u, 0, 0);
     it.r = r;
   }
-  __device__ static Cur begin(const Item &it, int g, int left) {
+  // the scales' bits, zeros behind the row's last block
+  __device__ static void scales(const Item &it, int g, int left, uint32_t &e0, uint32_t &e1) {
+    const uint32_t w0 = realign(it.w0.y, it.w0.x, it.r), w8 = realign(it.w2.y, it.w2.x, it.r);
+    e0 = 64 * g < left ? w0 & 0xffffu : 0u;
+    e1 = 64 * g + 32 < left ? w8 >> 16 : 0u;
+  }
+  // |d| from 256 on (infinities and NaN among them): d * q may pass fp16
+  __device__ static bool large(uint32_t e) { return (e & 0x7fffu) >= 0x5c00u; }
+  __device__ static bool any_large(const Item &it, int g, int left) {
+    uint32_t e0, e1;
+    scales(it, g, left, e0, e1);
+    return __builtin_amdgcn_ballot_w64(large(e0) || large(e1)) != 0;
+  }
+  // part 0: the blocks of ordinary scales; part 1: the large ones, d / 256 (an
+  // exact fp16) in the planes and 256 in front of their sum
+  __device__ static Cur begin(const Item &it, int g, int left, int part) {
     const uint32_t raw[18] = {it.w0.x, it.w0.y, it.w0.z, it.w0.w, it.w1.x, it.w1.y, it.w1.z, it.w1.w, it.w2.x,
                               it.w2.y, it.w2.z, it.w2.w, it.w3.x, it.w3.y, it.w3.z, it.w3.w, it.w4.x, it.w4.y};
     Cur c;
 #pragma unroll
     for (int i = 0; i < 17; ++i) c.w[i] = realign(raw[i + 1], raw[i], it.r);
-    const uint32_t e0 = 64 * g < left ? c.w[0] & 0xffffu : 0u, e1 = 64 * g + 32 < left ? c.w[8] >> 16 : 0u;
-    const _Float16 d0 = __builtin_bit_cast(_Float16, (uint16_t)e0), d1 = __builtin_bit_cast(_Float16, (uint16_t)e1);
+    uint32_t e0, e1;
+    scales(it, g, left, e0, e1);
+    c.d = 1.0f;
+    if (part >= 0) {
+      e0 = large(e0) == (part == 1) ? e0 : 0u;
+      e1 = large(e1) == (part == 1) ? e1 : 0u;
+    }
+    _Float16 d0 = __builtin_bit_cast(_Float16, (uint16_t)e0), d1 = __builtin_bit_cast(_Float16, (uint16_t)e1);
+    if (part == 1) {
+      d0 *= (_Float16)0.00390625f;
+      d1 *= (_Float16)0.00390625f;
+      c.d = 256.0f;
+    }
     c.d0 = h2{d0, d0};
     c.d1 = h2{d1, d1};
-    c.d = 1.0f;
     return c;
   }
   __device__ static void frag(const Item &, const Cur &c, int t, int, h8 &b1, h8 &b2) {
@@ -328,12 +354,13 @@ __device__ __forceinline__ void convert(ActA &A, const float4 raw[16]) {
 }
 
 // acc (rows 4 g .. 4 g + 3 of the lane's column) += the item's products; rs:
-// the rows' scales; left: the values of the row from the item on.
+// the rows' scales; left: the values of the row from the item on; part: of
+// Q8_0's blocks, one of the two or all (-1).
 template <class F>
 __device__ __forceinline__ void contract(f4 &acc, const typename F::Item &it, const ActA &A, const f4 &rs, int g,
-                                         int left) {
+                                         int left, int part = -1) {
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  const typename F::Cur c = F::begin(it, g, left);
+  const typename F::Cur c = F::begin(it, g, left, part);
   f4 s = zero, low = zero;  // two chains: a product waits for the one before it in its own
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
@@ -469,12 +496,15 @@ __global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
     typename F::Item S[D][NM];
     // the weights of the wave's i-th tile (past the steps, or columns past the
     // last: past the stack, nothing)
-    auto load_tile = [&](typename F::Item *it, int i) {
+    auto load_one = [&](typename F::Item &it, int i, int k) {
       const int col = ((step0 + i) * a.slots + slot) * 16 + n;
       const bool in = !idle && i < steps && col < a.N;
       const uint32_t at = (uint32_t)col * (uint32_t)a.row_bytes + (uint32_t)item * sb;
+      F::load(it, rs[k], in ? at + skew[k] : 0xFFFFF000u, g);
+    };
+    auto load_tile = [&](typename F::Item *it, int i) {
 #pragma unroll
-      for (int k = 0; k < NM; ++k) F::load(it[k], rs[k], in ? at + skew[k] : 0xFFFFF000u, g);
+      for (int k = 0; k < NM; ++k) load_one(it[k], i, k);
     };
     ActA A;
     f4 scales, factor = {};  // of the four rows whose sums the lane holds
@@ -502,7 +532,20 @@ __global__ __launch_bounds__(kWaves * 64) void moe_stream_kernel(MoeProduct a) {
 #pragma unroll
         for (int k = 0; k < NM; ++k) {
           f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-          contract<F>(acc, S[d][k], A, scales, g, a.K - 256 * item);
+          const int left = a.K - 256 * item;
+          bool whole = true;
+          if constexpr (F::kType == kQ8_0) whole = !F::any_large(S[d][k], g, left);
+          if (whole) {
+            contract<F>(acc, S[d][k], A, scales, g, left);
+          } else {
+            // in two, the item loaded anew (kept, it would cost every other one registers)
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+              typename F::Item it;
+              load_one(it, i, k);
+              contract<F>(acc, it, A, scales, g, left, part);
+            }
+          }
           red[parity][i % kBatch][wave][k][l] = acc;
         }
         // into the registers that this tile's weights have left (issued any

@@ -761,3 +761,35 @@ def test_moe_rows_of_q8_end_at_their_own_blocks(torch, okq, rows, behind):
         assert torch.equal(got[~used], clean[~used])
         if behind != 0x7BFF:
             assert not bool(torch.isfinite(got[used, at]).any())
+
+
+@pytest.mark.parametrize("rows", [1, 20, 400])
+@pytest.mark.parametrize("hidden,inner", [(512, 256), (288, 1312)])
+def test_moe_q8_of_large_scales(torch, okq, rows, hidden, inner):
+    """Blocks up to the largest scale and code beside ordinary ones: within the bound; and bit for bit those of
+    ordinary scales alone, where what meets the others is zero."""
+    e = Experts(torch, okq, 5, hidden, inner, Q8_0, Q8_0)
+    x = torch.randn(rows, hidden, generator=_gen(torch, rows), device="cuda")
+    ids, weights = _pairs(torch, rows, 5, 2, 8)
+    loud = torch.arange(hidden, device="cuda") // 32 % 4 == 1
+    x[:, loud] = 0.0
+    clean = e(torch, okq, x, ids, weights)
+    g = _gen(torch, 7)
+    for name, columns in (("gate", hidden), ("up", hidden), ("down", inner)):
+        blocks = getattr(e, name).view(-1, columns // 32, 34)
+        at = torch.arange(columns // 32, device="cuda") % 4 == 1
+        if name == "down":  # some rows, which gives those outputs alone other values
+            blocks = blocks[::7]
+        d = torch.rand(blocks[:, at, 0].shape, generator=g, device="cuda") * 65000 + 200
+        d[..., 0] = 65504.0
+        q = torch.randint(0, 256, (*d.shape, 32), generator=g, device="cuda").to(torch.uint8)
+        q[..., 0] = 128
+        blocks[:, at] = torch.cat([d.half().view(torch.uint8).view(*d.shape, 2), q], -1)
+        okq.call("okq_dequantize", Q8_0, getattr(e, name).data_ptr(), getattr(e, name + "_f").numel(),
+                 getattr(e, name + "_f").data_ptr(), _stream(torch))
+    got = e(torch, okq, x, ids, weights)
+    _within(got, *e.want(torch, x, ids, weights), "out")
+    small = (e.down_f.abs().amax((0, 2)) < 10.0)  # outputs that no expert's large blocks reach
+    assert bool(small.any()) and torch.equal(got[:, small], clean[:, small])
+    x[:, loud] = torch.randn(rows, int(loud.sum()), generator=g, device="cuda")
+    _within(e(torch, okq, x, ids, weights), *e.want(torch, x, ids, weights), "out")
