@@ -380,7 +380,9 @@ static void launch_route(const RouteArgs &a, const RoutePlan &p, double *part, u
   const int et = (a.experts + 15) / 16;
   const dim3 grid((unsigned)p.tiles, p.whole ? 1u : (unsigned)et, p.whole ? 1u : (unsigned)p.slices);
   const unsigned lds = (unsigned)p.lds;
-  if (!p.whole || et == 1) launch_timed(route_kernel<kType, kWide, 1>, grid, dim3(waves_of(1) * 64), lds, s, a, p, part, arrived);
+  // a tile a workgroup of 1024 threads, unless the launch would have 2^32 of them (the last 16 of 2^26 rows)
+  const bool one = !p.whole || (et == 1 && (uint64_t)p.tiles * (waves_of(1) * 64) <= UINT32_MAX);
+  if (one) launch_timed(route_kernel<kType, kWide, 1>, grid, dim3(waves_of(1) * 64), lds, s, a, p, part, arrived);
   else if (et <= 4) launch_timed(route_kernel<kType, kWide, 4>, grid, dim3(waves_of(4) * 64), lds, s, a, p, part, arrived);
   else launch_timed(route_kernel<kType, kWide, 8>, grid, dim3(waves_of(8) * 64), lds, s, a, p, part, arrived);
 }

@@ -793,3 +793,15 @@ def test_moe_q8_of_large_scales(torch, okq, rows, hidden, inner):
     assert bool(small.any()) and torch.equal(got[:, small], clean[:, small])
     x[:, loud] = torch.randn(rows, int(loud.sum()), generator=g, device="cuda")
     _within(e(torch, okq, x, ids, weights), *e.want(torch, x, ids, weights), "out")
+
+
+@pytest.mark.parametrize("rows", [(1 << 26) - 16, (1 << 26) - 15, 1 << 26])
+def test_route_of_the_most_rows(torch, okq, rows):
+    """2^26 rows are 2^22 tiles: of 1024 threads each they would be more than a launch has."""
+    x = torch.randn(rows, 1, generator=_gen(torch, 1), device="cuda")
+    w = torch.tensor([[1.0], [-1.0], [0.5]], device="cuda")
+    ids, weights, _ = _route(torch, okq, x, 1, w, F32, None, None, True, 1, 1, 1, 1, False, 1.0, logits=False)
+    want = (x[:, 0] < 0).int()
+    assert torch.equal(ids[:, 0], want)
+    off = (weights[:, 0] - torch.sigmoid(x[:, 0].abs().double())).abs()
+    assert float(off.max()) <= U  # below 1: half a step is 2^-25, and torch's own f64
