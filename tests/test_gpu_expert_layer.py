@@ -805,3 +805,63 @@ def test_route_of_the_most_rows(torch, okq, rows):
     assert torch.equal(ids[:, 0], want)
     off = (weights[:, 0] - torch.sigmoid(x[:, 0].abs().double())).abs()
     assert float(off.max()) <= U  # below 1: half a step is 2^-25, and torch's own f64
+
+
+@pytest.mark.parametrize("case", [  # as ROUTE: whole rows a workgroup, in more than one round of 128 experts
+    (2100, 256, 256, 8, True, 8, 4, 2, False, True, True, F32, 0),
+    (2049, 130, 500, 10, False, 1, 1, 1, True, False, True, BF16, 1),
+    (2033, 64, 129, 5, False, 3, 2, 1, False, True, False, F32, 0),
+    (2050, 96, 512, 64, True, 64, 9, 2, True, True, True, F16, 4),
+], ids=lambda c: str(c[:4]))
+def test_route_of_many_rows_and_experts(torch, okq, case):
+    args = _route_inputs(torch, case)
+    got = _route(torch, okq, *args)
+    x, _, w, _, b, c, *rest = args
+    _check_route(torch, got, _route_want(torch, x, w, b, c, *rest), x, w)
+    for n in (1, 300):  # split over expert tiles: the same experts
+        some = _route(torch, okq, x[:n], *args[1:])
+        assert torch.equal(some[0], got[0][:n])
+        assert bool(((some[1] - got[1][:n]).abs() <= 2 * U * got[1][:n]).all())
+
+
+@pytest.mark.parametrize("rows,k,experts,gu,dn", [
+    (1, 64, 128, Q4_K, Q6_K),  # one row that names one expert 64 times
+    (40, 1, 128, Q8_0, Q4_K),  # all rows with one expert, not sorted
+    (8, 8, 128, Q6_K, Q5_K),   # all rows with the same eight
+    (13, 4, 104, Q5_K, Q8_0),
+])
+def test_moe_pairs_of_few_experts_not_sorted(torch, okq, rows, k, experts, gu, dn):
+    """An expert of more than 16 pairs goes in turns where nothing is sorted."""
+    e = Experts(torch, okq, experts, 512, 768, gu, dn)
+    x = torch.randn(rows, 512, generator=_gen(torch, rows), device="cuda")
+    _, weights = _pairs(torch, rows, experts, k, 4)
+    few = 1 if k in (1, 64) else k
+    ids = (torch.arange(rows * k, device="cuda") % few * 11 + 7).int().view(rows, k)
+    got = e(torch, okq, x, ids, weights)
+    _within(got, *e.want(torch, x, ids, weights), "out")
+
+
+def _off(k):
+    """A product's relative error in root mean square over K values of independent sign: planes 2^-21 of each (the
+    worst of all), sums as a random walk of K / 8 additions."""
+    return 2.0 ** -21 + U * math.sqrt(k / 8)
+
+
+@pytest.mark.parametrize("kind", [Q8_0, Q4_K, Q5_K, Q6_K])
+@pytest.mark.parametrize("rows,hidden,inner,experts", [
+    (1, 512, 768, 8), (24, 768, 512, 40), (9, 4352, 8704, 4),            # streamed: unsorted, sorted, in slices
+    (300, 512, 256, 8), (400, 4352, 5120, 3), (200, 2048, 14336, 2)])    # tiles, of long rows too
+def test_moe_is_as_near_as_its_planes(torch, okq, kind, rows, hidden, inner, experts):
+    """The whole error beside the whole result: one plane of activations less would be 2^-12 of it.
+
+    Q4_K and Q5_K sum q and the min apart: q's mean is 2.7 of its deviations, so each of the two sums is up to 2.9
+    times the result, together 4.  silu's slope of at most 1.1 against its root mean square of 0.6 at deviation 1, and
+    the factor up, make 3 of one product's error in the gated values, taken as 4."""
+    e = Experts(torch, okq, experts, hidden, inner, kind, kind)
+    x = torch.randn(rows, hidden, generator=_gen(torch, rows), device="cuda")
+    ids, weights = _pairs(torch, rows, experts, 2, 12)
+    want, _ = e.want(torch, x, ids, weights)
+    got = e(torch, okq, x, ids, weights)
+    off = float((got - want).square().mean().sqrt() / want.square().mean().sqrt())
+    bound = (4 if kind in (Q4_K, Q5_K) else 1) * (4 * _off(hidden) + _off(inner))
+    assert off <= bound, (off, bound)
