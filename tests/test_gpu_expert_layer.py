@@ -865,3 +865,34 @@ def test_moe_is_as_near_as_its_planes(torch, okq, kind, rows, hidden, inner, exp
     off = float((got - want).square().mean().sqrt() / want.square().mean().sqrt())
     bound = (4 if kind in (Q4_K, Q5_K) else 1) * (4 * _off(hidden) + _off(inner))
     assert off <= bound, (off, bound)
+
+
+@pytest.mark.parametrize("kind", [Q8_0, Q4_K, Q5_K, Q6_K])
+@pytest.mark.parametrize("rows", [1, 30, 400])
+def test_moe_bad_blocks_stay_in_their_outputs(torch, okq, kind, rows):
+    """A block of weights that is no number: one output of down; every output where gate or up has it; of its expert's
+    rows alone.  Experts without rows may hold anything."""
+    hidden, inner = 768, 512
+    e = Experts(torch, okq, 5, hidden, inner, kind, kind)
+    x = torch.randn(rows, hidden, generator=_gen(torch, rows), device="cuda")
+    ids, weights = _pairs(torch, rows, 3, 2, 8)
+    ids *= 2
+    clean = e(torch, okq, x, ids, weights)
+    for name in ("gate", "up", "down"):
+        getattr(e, name).view(5, -1)[1::2] = 0xFF
+    assert torch.equal(e(torch, okq, x, ids, weights), clean)
+    used = (ids == 2).any(1)
+    elems, size = BYTES[kind]
+    for name, outputs, columns in (("down", hidden, inner), ("gate", inner, hidden), ("up", inner, hidden)):
+        blocks = getattr(e, name).view(5, outputs, columns // elems, size)
+        at = outputs - 1  # beside the next expert's
+        held = blocks[2, at, -1].clone()
+        blocks[2, at, -1] = 0xFF
+        got = e(torch, okq, x, ids, weights)
+        blocks[2, at, -1] = held
+        assert torch.equal(got[~used], clean[~used])
+        if name == "down":
+            keep = torch.arange(hidden, device="cuda") != at
+            assert torch.equal(got[:, keep], clean[:, keep]) and bool(torch.isnan(got[used, at]).all())
+        else:
+            assert bool(torch.isnan(got[used]).all())
