@@ -5,27 +5,17 @@
 #pragma once
 #include "okq_device.h"
 #include "okq_internal.h"
+#include "okq_mfma.h"
 
 namespace okq {
 
 namespace {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f16x __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __amdgpu_buffer_rsrc_t Rsrc;
 typedef __attribute__((address_space(3))) void *LdsPtr;
 
 constexpr int kMaxM = 128;           // rows of the taller tile
 constexpr int kFN = 256;             // tile columns (8 waves x 32)
 constexpr int kPlane = kMaxM * 128;  // halves of one plane of a stage
-
-__device__ __forceinline__ Rsrc make_rsrc(const void *base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, 0x00020000);
-}
 
 // Activation stages: two buffers of [2 planes][128 rows][128 halves] and
 // [128 rows][4 (hi, lo) per-32 sums]; distinct objects, so that the fragment
