@@ -408,8 +408,9 @@ enum {
  * (OKQ_TYPE_F32, F16 or BF16); bias, choice_bias [experts] f32 or NULL, the
  * latter finite or -infinity; ids
  * [rows, top_k] int32, weights [rows, top_k] f32, logits [rows, experts] f32
- * or NULL: z.  All of it is computed in 64 bits and rounded at the stores, so
- * a row's experts do not change with the rows around it.  An expert of c =
+ * or NULL: z.  All of it is computed in 64 bits and rounded at the stores; the
+ * order of the sums over hidden goes by the call's sizes, so a row's experts can
+ * change with the number of rows only where two c differ by some 1e-15.  An expert of c =
  * -infinity is never chosen: where too few are left, ids are -1 and weights
  * 0.  A row with a NaN among its z or c gets ids of -1 and weights of NaN.
  * experts at most 512, groups at most 64, top_k at most 64 and at most the
@@ -431,10 +432,13 @@ okq_status okq_moe_route(const float *x, int64_t x_stride, int64_t rows, int64_t
  * ids, weights [rows, top_k]; an id outside [0, experts) adds nothing whatever
  * its weight is, so a row of such ids gets zeros; the same id twice in a row
  * adds twice.  experts at most 4096, top_k at most 64.  Each expert's weights are read once for up
- * to 16 of its rows, 128 where it has many.  Activations keep 22 bits, sums are f32; a row's result
+ * to 16 of its rows, 128 where it has many.  Activations keep 22 bits (of rows
+ * whose largest is 2^-90 or more), sums are f32; a row's result
  * does not depend on the rows around it beyond the choice of a kernel by the
  * call's sizes, nor on timing.  A row of x that holds an infinity or a NaN, or
- * whose gated values do, gets NaN throughout (where it has an expert).  rows
+ * whose gated values do, gets NaN throughout (where it has an expert).  Blocks
+ * whose scale is an infinity or a NaN reach the outputs that they are weights of;
+ * experts that no id names may hold anything.  rows
  * == 0 is a no-op.  Uses a per-stream workspace.  No counterpart in the
  * reference (crates/kernels/src/mlp.rs has the dense MLP). */
 okq_status okq_moe_mlp_q(const float *x, int64_t x_stride, int64_t rows, int64_t hidden, int64_t intermediate,

@@ -3,10 +3,12 @@
 // (okq_gemm_f32.h).
 //
 // What bounds it: the MFMAs, two per weight fragment and row block (Q6_K
-// three), as in okq_gemm_f32.hip: 4096 tokens, 8 of 128 experts, 2048 x 768:
-// gate and up in Q4_K 513-549 us, 750-800 TFLOP/s of them (49% of the cycles),
-// down in Q6_K 363-380.  Tiles of 64 rows wait for their weights, requested one
-// stage ahead: 333 tokens, 6 of 31, 2560 x 1440 in Q8_0: 166 and 90 us.
+// three): 4096 tokens, 8 of 128 experts, 2048 x 768: gate and up in Q4_K 521-549
+// us, 750-790 TFLOP/s of them (49% of the cycles), down in Q6_K 361-384, 810-860.
+// (The dense kernel does 980 and 1070 on 512 x 4096 -> 14336.  A workgroup here
+// has 16 or 6 stages, and nothing runs beside its first loads and its
+// epilogue.)  Tiles of 64 rows wait for their weights, requested one stage
+// ahead: 333 tokens, 6 of 31, 2560 x 1440 in Q8_0: 168 and 92 us.
 // A tile's height is its expert's own: full ones of 128
 // rows, and one of 32, 64, 96 or 128 for the rest, chosen per workgroup.
 #include "okq_gemm_f32.h"

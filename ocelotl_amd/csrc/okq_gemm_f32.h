@@ -518,7 +518,7 @@ __device__ __forceinline__ void f32_body(const _Float16 *__restrict__ xhi, const
     float f = 0.0f;
     if (tid < rows) {
       f = rscale[source(tid)];
-      if constexpr (kExperts == 2) f *= em.weights[em.order[et.row0 + tid]];  // a power of two: exact
+      if constexpr (kExperts == 2) f *= em.weights[em.order[et.row0 + tid]];  // by a power of two: exact down to 2^-126
     }
     fR[tid] = f;
   }
@@ -536,6 +536,9 @@ __device__ __forceinline__ void f32_body(const _Float16 *__restrict__ xhi, const
   // from float64, 2.4e-7 for exact d * q planes in three MFMAs), so after every
   // kSegment stages the sums so far wait in the output (or partial) and a new
   // segment starts from zero: 2.1e-7, and 516 -> 554 us (825 with the planes).
+  // Experts' tiles fold to the end, since gate and up have one output between
+  // them to wait in: a whole call is 4.6e-7 from float64 in root mean square at
+  // 2048 x 14336, as against 3.3e-7 in Q6_K and 7.2e-7 in Q4_K.
   constexpr int kSegment = 28;
   float *const dst0 = kExperts ? nullptr : (ksplit > 1 ? sarg(mt.part) + (size_t)z * M * N : sarg(mt.y)) + (size_t)m0 * N + col;
   // this lane's sums plus those parked (add), parked again (keep) or taken;

@@ -847,6 +847,8 @@ MoePlan moe_plan(const MoeArgs &a) {
   // faster ones: at 24 and 32, us streamed / tiled, 2048 x 768 Q4_K and Q6_K with
   // 128 experts 237 / 248 and 298 / 275, 2048 x 1536 Q5_K and Q8_0 with 32 150 /
   // 157 and 173 / 168, 4096 x 4096 Q6_K with 8 199 / 215 and 251 / 239.
+  // The average is the call's: every pass over it goes the same way, also where
+  // a pass has fewer rows an expert (of more than 2340 experts, or the last one).
   const int64_t least = 28 * (int64_t)a.experts;  // pairs
   const bool tiled = (int64_t)a.rows * a.top_k >= least;
   MoePlan p = plan_of(a, tiled);
@@ -915,7 +917,12 @@ static hipError_t launch_product(MoeProduct a, int cu_count, hipStream_t s) {
     a.rounds = (int)((a.pairs * (int64_t)a.steps + groups - 1) / groups);
     grid = dim3((a.steps + a.rounds - 1) / a.rounds, a.pairs, a.slices);
   }
-  // Two tiles in flight a wave, where the registers hold them and there are more
+  // Two tiles in flight a wave where a workgroup has more than two.  us a call
+  // with two / with one: 48 rows, 8 of 128, 2048 x 768 Q4_K 92 / 97, Q5_K 116 /
+  // 120, Q6_K 146 / 148 and 2048 x 1440 Q8_0 234 / 243, though the latter two's
+  // down spills 17 and 10 registers for it (their gate and up would spill 63 and
+  // 33).  Two steps in all, one row, 8 of 128, 2048 x 768: 25.3 / 22.6
+  // in Q4_K and Q6_K, 28.7 / 26.7 in Q8_0.
   if ((a.order || a.rounds > 2) && (NM == 1 || !F::kLow))
     launch_timed(moe_stream_kernel<F, NM, NM == 1 || !F::kLow ? 2 : 1>, grid, block, 0u, s, a);
   else
@@ -1000,7 +1007,9 @@ static hipError_t stream_pass(const MoeArgs &a, const MoePlan &plan, uint8_t *ws
   g.pairs = (int)(rows * a.top_k);
   // One row's experts differ; of more rows', half of the experts' number still
   // mostly do (26 pairs of 8 experts, 4096 x 14336, unsorted: 590 us, most
-  // workgroups having found an earlier pair of their expert; sorted: 300)
+  // workgroups having found an earlier pair of their expert; sorted: 300).  Where
+  // they do not, the same happens: 64 pairs of one expert, 2048 x 768 of 128 in
+  // Q4_K, 166 us, as many of different ones 51; 65 pairs, sorted, 35.
   if (g.pairs > kFewPairs || (rows > 1 && 2 * g.pairs > a.experts)) {
     const Sorted so(ws, plan, a.top_k);
     launch_timed(moe_sort_kernel, dim3(1), dim3(1024), 0u, s, g.ids, g.pairs, a.experts, 16, so.order, so.place, so.count,

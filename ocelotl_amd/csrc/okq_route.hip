@@ -10,7 +10,8 @@
 // values that may lie next to each other: in 32 bits the order of a sum would
 // decide it, and a token's experts would change with the batch that it came
 // in.  In 64 the products of f32 values are exact and a sum of thousands is
-// off by some 1e-15, so no split or tile shows in the ids.
+// off by some 1e-15, so a split or tile shows in the ids only where two experts
+// are that near each other (equal rows of W give equal sums, whatever the split).
 #include <algorithm>
 
 #include "okq_device.h"
